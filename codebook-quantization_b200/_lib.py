@@ -89,6 +89,11 @@ SIGNATURES = {
                                           _P, _P, _P, _I64, ct.c_float, _P, _P, _I64, _P]),
     "cbq_attn_decode_split": (_INT, [_P, _P, _P, _INT, _I64, _I64, _I64, _I64, _I64, _P, ct.c_float, _P, _P,
                                      _I64, _P]),
+    "cbq_paged_append_rope": (_INT, [_P, _P, _I64, _P, _I64, _P, _I64, _P, _I64, _I64, ct.c_float, _P, _P, _P, _P,
+                                     _I64, _P, _P]),
+    "cbq_paged_attn_workspace_bytes": (_I64, [_P, _P, _I64, _I64, _INT]),
+    "cbq_paged_attn_decode": (_INT, [_P, _P, _I64, _P, _I64, _I64, ct.c_float, _P, _P, _I64, _P]),
+    "cbq_paged_attn_extend": (_INT, [_P, _P, _I64, _P, _I64, _I64, ct.c_float, _P, _P, _I64, _P]),
 }
 CBQ_EPI_STORE, CBQ_EPI_RESIDUAL, CBQ_EPI_SILU_MUL = 0, 1, 2
 

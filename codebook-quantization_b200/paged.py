@@ -1,0 +1,217 @@
+"""Paged key/value cache: ragged batches, prompts of any length, shared prefixes.
+
+``PagedKVCache`` wraps the two page pools of one layer and ``PagedBatch`` the
+device tensors that say which rows each sequence owns; the three operators run
+``libcbq``'s kernels (``cbq_paged_*`` in ``include/cbq.h``) on the caller's
+current stream:
+
+* ``append_rope`` -- q/k RMSNorm and rotary embedding of the new tokens, keys
+  and values written to their rows;
+* ``attend_decode`` -- one new token per sequence over its group's prefix
+  (computed once for the whole group) and its own rows;
+* ``attend_extend`` -- any number of new tokens per sequence, causally.
+
+Lengths and tables stay on the device and may be updated in place between
+calls, so a step can be captured in a CUDA graph.  No counterpart in the
+reference, which uses HF's cache and attention.
+"""
+from __future__ import annotations
+
+import ctypes as ct
+import struct
+from typing import Optional
+
+import torch
+
+from . import _lib
+
+__all__ = ["PagedKVCache", "PagedBatch"]
+
+_CODES = {torch.float32: _lib.CBQ_F32, torch.bfloat16: _lib.CBQ_BF16}
+
+
+def _need(ok: bool, what: str) -> None:
+    if not ok:
+        raise ValueError(what)
+
+
+def _ints(t: Optional[torch.Tensor], name: str, ndim: int, device: torch.device) -> Optional[torch.Tensor]:
+    if t is None:
+        return None
+    _need(isinstance(t, torch.Tensor) and t.dtype == torch.int32 and t.dim() == ndim,
+          f"{name}: int32 tensor of {ndim} dimension(s) expected")
+    _need(t.device == device, f"{name}: on {t.device}, expected {device}")
+    _need(t.shape[-1] <= 1 or t.stride(-1) == 1, f"{name}: last dimension must be contiguous")
+    return t
+
+
+class PagedBatch:
+    """The sequences of a step.
+
+    ``page_table`` int32 [seqs, width], ``kv_lens`` int32 [seqs] (rows of each
+    sequence, its new tokens included); ``cu_tokens`` int32 [seqs + 1]: where
+    each sequence's new tokens begin (None: one token each).  Shared prefixes:
+    group g holds the sequences ``group_starts[g] .. group_starts[g+1] - 1``
+    and its prefix the first ``prefix_lens[g]`` rows of the pages in
+    ``prefix_table[g]``.  ``max_kv_len`` / ``max_prefix_len`` bound the values
+    the two length tensors will ever hold (default: what the tables can name).
+    ``status`` int32 [4]: see :meth:`new_status` and :func:`check_status`.
+    The tensors are kept, not copied: write new values into them in place."""
+
+    def __init__(self, page_table: torch.Tensor, kv_lens: torch.Tensor, cu_tokens: Optional[torch.Tensor] = None,
+                 group_starts: Optional[torch.Tensor] = None, prefix_lens: Optional[torch.Tensor] = None,
+                 prefix_table: Optional[torch.Tensor] = None, max_kv_len: Optional[int] = None,
+                 max_prefix_len: Optional[int] = None, status: Optional[torch.Tensor] = None):
+        dev = page_table.device
+        self.device = dev
+        self.page_table = _ints(page_table, "page_table", 2, dev)
+        self.kv_lens = _ints(kv_lens, "kv_lens", 1, dev)
+        self.cu_tokens = _ints(cu_tokens, "cu_tokens", 1, dev)
+        self.group_starts = _ints(group_starts, "group_starts", 1, dev)
+        self.prefix_lens = _ints(prefix_lens, "prefix_lens", 1, dev)
+        self.prefix_table = _ints(prefix_table, "prefix_table", 2, dev)
+        self.status = _ints(status, "status", 1, dev)
+        self.seqs = n = kv_lens.shape[0]
+        _need(page_table.shape[0] == n, f"page_table has {page_table.shape[0]} rows for {n} sequences")
+        _need(cu_tokens is None or cu_tokens.shape[0] == n + 1, "cu_tokens must have one entry more than kv_lens")
+        shared = (group_starts is None, prefix_lens is None, prefix_table is None)
+        _need(len(set(shared)) == 1, "group_starts, prefix_lens and prefix_table come together")
+        groups = 0
+        if prefix_lens is not None:
+            groups = prefix_lens.shape[0]
+            _need(group_starts.shape[0] == groups + 1 and prefix_table.shape[0] == groups,
+                  "group_starts needs one entry more than prefix_lens, prefix_table one row for each")
+        _need(status is None or status.shape[0] == 4, "status must have four entries")
+        self.groups = groups
+        ptr = lambda t: 0 if t is None else t.data_ptr()  # noqa: E731
+        big = 0x7fffff00
+        raw = struct.pack(
+            "<qqqqqqqqqqqqqqq", n, ptr(cu_tokens), ptr(kv_lens), ptr(page_table), page_table.shape[1],
+            max(page_table.stride(0), page_table.shape[1]), big if max_kv_len is None else int(max_kv_len), groups,
+            ptr(group_starts), ptr(prefix_lens), ptr(prefix_table), prefix_table.shape[1] if groups else 0,
+            max(prefix_table.stride(0), prefix_table.shape[1]) if groups else 0,
+            big if max_prefix_len is None else int(max_prefix_len), ptr(status))
+        self._desc = ct.create_string_buffer(raw, len(raw))
+        self._addr = ct.addressof(self._desc)
+        self._ws = {}                      # (cache layout, tokens, heads, extend) -> workspace bytes
+
+    @staticmethod
+    def new_status(device) -> torch.Tensor:
+        """A status word for ``status=``: flags, first row, count, spare."""
+        return torch.tensor([0, -1, 0, 0], dtype=torch.int32, device=device)
+
+
+def check_status(status: torch.Tensor) -> None:
+    """Raise if a call recorded lengths or pages outside the tables (reads the device)."""
+    flags = int(status[0].item())
+    if flags:
+        raise _lib.CbqError("paged cache", _lib.CBQ_ERR_CORRUPT)
+
+
+class PagedKVCache:
+    """One layer's keys and values: ``k_pages``, ``v_pages`` [pages, kv_heads,
+    page_size, head_dim] (fp32 or bf16, head_dim contiguous, equal strides; a
+    pool stored as [pages, page_size, kv_heads, head_dim] is passed transposed)."""
+
+    def __init__(self, k_pages: torch.Tensor, v_pages: torch.Tensor):
+        if not k_pages.is_cuda:
+            raise RuntimeError("the paged cache lives on a CUDA device; there is no CPU fallback")
+        _need(k_pages.dim() == 4, "pools are [pages, kv_heads, page_size, head_dim]")
+        _need(k_pages.dtype in _CODES, f"cache dtype {k_pages.dtype}: float32 or bfloat16 expected")
+        _need(v_pages.shape == k_pages.shape and v_pages.dtype == k_pages.dtype and
+              v_pages.stride() == k_pages.stride() and v_pages.device == k_pages.device,
+              "k_pages and v_pages must agree in shape, strides, dtype and device")
+        _need(k_pages.stride(3) == 1, "head_dim must be contiguous")
+        self.k_pages, self.v_pages = k_pages, v_pages
+        self.device, self.dtype = k_pages.device, k_pages.dtype
+        self.pages, self.kv_heads, self.page_size, self.head_dim = k_pages.shape
+        st = k_pages.stride()
+        raw = struct.pack("<qqqqqqqqqq", k_pages.data_ptr(), v_pages.data_ptr(), *k_pages.shape, st[0], st[1], st[2],
+                          _CODES[k_pages.dtype])
+        self._desc = ct.create_string_buffer(raw, len(raw))
+        self._addr = ct.addressof(self._desc)
+        self._key = (tuple(k_pages.shape), self.dtype)
+
+    def _rows(self, t: torch.Tensor, name: str, heads: Optional[int]) -> int:
+        """Checks [tokens, heads, head_dim] of the cache's dtype, heads and
+        head_dim contiguous; the stride from token to token."""
+        if t.dim() != 3 or t.shape[2] != self.head_dim or (heads is not None and t.shape[1] != heads):
+            raise ValueError(f"{name}: [tokens, {'heads' if heads is None else heads}, {self.head_dim}] expected, "
+                             f"got {tuple(t.shape)}")
+        if t.dtype != self.dtype or t.device != self.device:
+            raise ValueError(f"{name}: {t.dtype} on {t.device}, the cache is {self.dtype} on {self.device}")
+        st = t.stride()
+        if st[2] != 1 or (st[1] != self.head_dim and t.shape[1] != 1):
+            raise ValueError(f"{name}: the heads of a token must be contiguous")
+        return st[0] if t.shape[0] > 1 else t.shape[1] * self.head_dim
+
+    def append_rope(self, batch: PagedBatch, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: torch.Tensor,
+                    sin: torch.Tensor, eps: float = 1e-6, q_weight: Optional[torch.Tensor] = None,
+                    k_weight: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """Normalise and rotate q [tokens, heads, d] and k [tokens, kv_heads, d]
+        at the tokens' positions, write k and v to the cache, return the rotated
+        q.  ``eps`` < 0: no RMSNorm; weights fp32 [d] or None (ones); cos / sin
+        fp32 [positions, d] (``qwen3_decode.rope_tables``)."""
+        tokens, heads, d = q.shape
+        qs, ks, vs = self._rows(q, "q", None), self._rows(k, "k", self.kv_heads), self._rows(v, "v", self.kv_heads)
+        _need(k.shape[0] == tokens and v.shape[0] == tokens, "q, k and v must have the same tokens")
+        _need(cos.shape == sin.shape and cos.dim() == 2 and cos.shape[1] == d and cos.dtype == torch.float32 and
+              sin.dtype == torch.float32 and cos.is_contiguous() and sin.is_contiguous(),
+              f"cos and sin: contiguous float32 [positions, {d}] expected")
+        for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
+            _need(w is None or (w.dtype == torch.float32 and w.shape == (d,) and w.is_contiguous()),
+                  f"{name}: contiguous float32 [{d}] expected")
+        if out is None:
+            out = torch.empty((tokens, heads, d), dtype=self.dtype, device=self.device)
+        else:
+            self._out(out, tokens, heads)
+        _lib.call("cbq_paged_append_rope", self._addr, batch._addr, tokens, q.data_ptr(), qs, k.data_ptr(),
+                  ks, v.data_ptr(), vs, heads, eps, None if q_weight is None else q_weight.data_ptr(),
+                  None if k_weight is None else k_weight.data_ptr(), cos.data_ptr(), sin.data_ptr(), cos.shape[0],
+                  out.data_ptr(), torch.cuda.current_stream(self.device).cuda_stream)
+        return out
+
+    def _out(self, out: torch.Tensor, tokens: int, heads: int) -> None:
+        _need(out.shape == (tokens, heads, self.head_dim) and out.dtype == self.dtype and out.is_contiguous() and
+              out.device == self.device, f"out: contiguous [{tokens}, {heads}, {self.head_dim}] of the cache's dtype")
+
+    def workspace_bytes(self, batch: PagedBatch, tokens: int, heads: int, extend: bool) -> int:
+        """Bytes of scratch one attention call needs."""
+        key = (self._key, tokens, heads, extend)
+        n = batch._ws.get(key)
+        if n is None:
+            n = _lib.query("cbq_paged_attn_workspace_bytes", self._addr, batch._addr, tokens, heads, int(extend))
+            batch._ws[key] = n
+        return n
+
+    def _attend(self, name: str, extend: bool, batch: PagedBatch, q: torch.Tensor, scale: Optional[float],
+                out: Optional[torch.Tensor], workspace: Optional[torch.Tensor]) -> torch.Tensor:
+        tokens, heads, d = q.shape
+        stride = self._rows(q, "q", None)
+        if out is None:
+            out = torch.empty((tokens, heads, d), dtype=self.dtype, device=self.device)
+        else:
+            self._out(out, tokens, heads)
+        if workspace is None:
+            # from torch's caching allocator: safe on any stream, and inside a captured graph
+            workspace = torch.empty(self.workspace_bytes(batch, tokens, heads, extend), dtype=torch.uint8,
+                                    device=self.device)
+        _lib.call(name, self._addr, batch._addr, tokens, q.data_ptr(), stride, heads,
+                  d ** -0.5 if scale is None else scale, out.data_ptr(), workspace.data_ptr(), workspace.numel(),
+                  torch.cuda.current_stream(self.device).cuda_stream)
+        return out
+
+    def attend_decode(self, batch: PagedBatch, q: torch.Tensor, scale: Optional[float] = None,
+                      out: Optional[torch.Tensor] = None, workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """q [seqs, heads, d], one token per sequence (``cu_tokens`` is not
+        read) -> [seqs, heads, d]: softmax(q k^T scale) v over the group's
+        prefix and the sequence's rows (``scale`` None: d^-1/2); zeros where
+        there is nothing to read."""
+        return self._attend("cbq_paged_attn_decode", False, batch, q, scale, out, workspace)
+
+    def attend_extend(self, batch: PagedBatch, q: torch.Tensor, scale: Optional[float] = None,
+                      out: Optional[torch.Tensor] = None, workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """q [tokens, heads, d], the sequences' new tokens one after the other
+        (``cu_tokens``) -> [tokens, heads, d]; token i of sequence s sees the
+        prefix and the rows up to its own."""
+        return self._attend("cbq_paged_attn_extend", True, batch, q, scale, out, workspace)

@@ -532,6 +532,95 @@ int cbq_attn_decode_split(const void *q_dev, const void *k_cache_dev, const void
                           const int64_t *pos_dev, float scale, void *out_dev, void *workspace_dev,
                           int64_t workspace_bytes, void *stream);
 
+/* ======================================================================
+ * Paged key/value cache: ragged batches, prompts of any length, shared
+ * prefixes.  No counterpart in the reference (its cache is HF's).
+ *
+ * A cache is a pool of pages; a page holds page_size rows (one per position)
+ * of every kv head.  Sequence s owns the rows 0..kv_lens[s]-1 of the pages
+ * listed in its row of the page table.  Sequences may be sorted into groups;
+ * the sequences group_starts[g]..group_starts[g+1]-1 of group g all begin with
+ * the prefix_lens[g] rows of the pages in row g of the prefix table, which
+ * exist once.  Row r of a sequence is position prefix_lens[g] + r.
+ *
+ * Everything in cbq_paged_batch that changes from step to step is read on the
+ * device, so a captured graph follows the tables and lengths.  Lengths above
+ * a table's width are cut to it and page numbers outside the pool are read as
+ * rows of zeros (never accessed); both set CBQ_FLAG_CORRUPT in status_dev.
+ * ====================================================================== */
+
+typedef struct cbq_paged_cache {
+    void *k_dev, *v_dev;     /* pools; 16-byte aligned */
+    int64_t pages;           /* pages in the pool */
+    int64_t kv_heads;
+    int64_t page_size;       /* 16, 32, 64, 128 or 256 */
+    int64_t head_dim;        /* 64, 128 or 256 */
+    int64_t page_stride, head_stride, row_stride;  /* elements, multiples of 16 bytes; the same for k and v */
+    int64_t dtype;           /* CBQ_F32 or CBQ_BF16, of the cache and the activations */
+} cbq_paged_cache;
+
+typedef struct cbq_paged_batch {
+    int64_t seqs;                       /* at most 65536 */
+    const int32_t *cu_tokens_dev;       /* [seqs + 1] first new token of each sequence; NULL: one each */
+    const int32_t *kv_lens_dev;         /* [seqs] rows of each sequence, its new tokens included */
+    const int32_t *page_table_dev;      /* [seqs][table_stride], table_width entries in use */
+    int64_t table_width, table_stride;
+    int64_t max_kv_len;                 /* no kv_lens value is larger (table_width * page_size does) */
+    int64_t groups;                     /* 0: no shared prefixes; at most seqs */
+    const int32_t *group_starts_dev;    /* [groups + 1], 0 .. seqs, never falling */
+    const int32_t *prefix_lens_dev;     /* [groups] */
+    const int32_t *prefix_table_dev;    /* [groups][prefix_stride], prefix_width entries in use */
+    int64_t prefix_width, prefix_stride;
+    int64_t max_prefix_len;             /* no prefix_lens value is larger */
+    uint32_t *status_dev;               /* uint32_t[4] as elsewhere, or NULL */
+} cbq_paged_batch;
+
+/* The new tokens' queries, keys and values: q [tokens, Hq, d], k and v
+ * [tokens, Hkv, d] (token strides in elements, multiples of 16 bytes; heads
+ * contiguous: slices of one projection's output do).  Per head of q and k
+ * RMSNorm with weight (fp32 [d], NULL = 1) and eps (eps < 0: no norm), then
+ * rotate-half rotary embedding with row `position` of the cos / sin tables
+ * (fp32 [rope_len, d]); q -> q_out [tokens, Hq, d] contiguous, k and v -> the
+ * token's row of the cache: row kv_lens[s] - T_s + i for the i-th of the T_s
+ * new tokens of sequence s.  fp32 throughout, each value rounded once.  A
+ * token whose row is negative (a sequence that is switched off has kv_len 0)
+ * is skipped and its q_out row is zero; so is one whose row, page or position
+ * lies outside the tables, which also sets CBQ_FLAG_CORRUPT. */
+int cbq_paged_append_rope(const cbq_paged_cache *cache, const cbq_paged_batch *batch, int64_t tokens,
+                          const void *q_dev, int64_t q_stride, const void *k_dev, int64_t k_stride,
+                          const void *v_dev, int64_t v_stride, int64_t q_heads, float eps,
+                          const float *q_weight_dev, const float *k_weight_dev, const float *cos_dev,
+                          const float *sin_dev, int64_t rope_len, void *q_out_dev, void *stream);
+
+/* Workspace bytes of cbq_paged_attn_decode (extend = 0) or
+ * cbq_paged_attn_extend (extend = 1); need not be zeroed, holds nothing from
+ * one call to the next.  -1: arguments the functions refuse. */
+int64_t cbq_paged_attn_workspace_bytes(const cbq_paged_cache *cache, const cbq_paged_batch *batch,
+                                       int64_t tokens, int64_t q_heads, int extend);
+
+/* Attention of one new token per sequence (tokens == seqs, cu_tokens_dev is
+ * not read): q [seqs, Hq, d] (token stride q_stride) over the sequence's
+ * prefix and its own kv_lens[s] rows, softmax(q k^T * scale) v -> out
+ * [seqs, Hq, d] contiguous; query head h reads kv head h / (Hq / Hkv).  A
+ * group's prefix is read once for all its sequences.  A sequence with nothing
+ * to read gives zeros.  Rows outside the lengths are never used, whatever they
+ * hold.  Scores, softmax and sums in fp32; bf16: products of bf16 on the
+ * tensor cores (the softmax weights rounded to bf16).  The split of the keys
+ * depends on the lengths and the SM count only: the same call gives the same
+ * bits.  Hq / Hkv <= 64. */
+int cbq_paged_attn_decode(const cbq_paged_cache *cache, const cbq_paged_batch *batch, int64_t tokens,
+                          const void *q_dev, int64_t q_stride, int64_t q_heads, float scale, void *out_dev,
+                          void *workspace_dev, int64_t workspace_bytes, void *stream);
+
+/* Attention of any number of new tokens per sequence (cu_tokens_dev; NULL:
+ * one each) over the prefix and the sequence's own rows, causally: the i-th
+ * of the T_s new tokens sees the prefix and own rows 0 .. kv_lens[s] - T_s + i.
+ * Otherwise as cbq_paged_attn_decode.  A non-finite value in a later row of
+ * the same sequence may reach earlier tokens of the same call. */
+int cbq_paged_attn_extend(const cbq_paged_cache *cache, const cbq_paged_batch *batch, int64_t tokens,
+                          const void *q_dev, int64_t q_stride, int64_t q_heads, float scale, void *out_dev,
+                          void *workspace_dev, int64_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

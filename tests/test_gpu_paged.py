@@ -1,0 +1,363 @@
+"""The paged key/value cache: append with rotation, attention of single tokens
+over shared prefixes, attention of prompts, each against a 64-bit oracle that
+works sequence by sequence; bounds as derived in ``paged_helpers``."""
+import math
+
+import pytest
+import torch
+
+from helpers import cbq, need_cuda
+from paged_helpers import Setup, check_attention
+
+pytestmark = pytest.mark.gpu
+L = cbq._lib
+DT = {"bf16": torch.bfloat16, "f32": torch.float32}
+
+
+def run(s, op, dev, scale=None, **kw):
+    k, v = s.pools(dev)
+    c = cbq.PagedKVCache(k, v)
+    b = s.batch(cbq, dev, decode=op == "decode", **kw)
+    f = c.attend_decode if op == "decode" else c.attend_extend
+    return f(b, s.q.to(dev), scale=scale)
+
+
+def verify(s, op, dev, scale=None, **kw):
+    got = run(s, op, dev, scale, **kw)
+    check_attention(got, *s.attention(s.d ** -0.5 if scale is None else scale, op == "extend"))
+    return got
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f32"])
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("heads,kv_heads", [(2, 2), (8, 2), (6, 2), (5, 1), (16, 1), (40, 1), (64, 1)])
+def test_decode_heads(dt, d, heads, kv_heads):
+    dev = need_cuda()
+    verify(Setup([1, 16, 17, 0, 33, 300], heads=heads, kv_heads=kv_heads, d=d, dtype=DT[dt]), "decode", dev)
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f32"])
+@pytest.mark.parametrize("page", [16, 32, 64, 128, 256])
+@pytest.mark.parametrize("layout", ["hnd", "nhd", "joint"])
+def test_decode_pages_and_layouts(dt, page, layout):
+    dev = need_cuda()
+    verify(Setup([5, 255, 256, 257, 0, 1030], d=128, page=page, dtype=DT[dt], layout=layout, slack=2), "decode", dev)
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f32"])
+@pytest.mark.parametrize("kv", [[1], [63], [64], [65], [4097], [0], [0, 0, 0]])
+def test_decode_single_lengths(dt, kv):
+    dev = need_cuda()
+    got = verify(Setup(kv, heads=8, kv_heads=2, d=128, dtype=DT[dt]), "decode", dev)
+    if not any(kv):
+        assert not got.any()
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f32"])
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("groups", [[(9, 500)], [(4, 33), (5, 700)], [(1, 1), (3, 0), (5, 129)]],
+                         ids=["one", "two", "three"])
+def test_decode_shared_prefix(dt, d, groups):
+    dev = need_cuda()
+    kv = [0, 1, 40, 0, 17, 300, 64, 5, 128]
+    verify(Setup(kv, groups=groups, heads=8, kv_heads=2, d=d, dtype=DT[dt]), "decode", dev)
+
+
+@pytest.mark.parametrize("n", [1, 31, 33, 150])
+def test_decode_prefix_of_many_sequences(n):
+    dev = need_cuda()
+    verify(Setup([(7 * i) % 50 for i in range(n)], groups=[(n, 1000)], heads=8, kv_heads=2, d=128), "decode", dev)
+
+
+def test_decode_more_sequences_than_threads():
+    """The line of tiles is planned in blocks of owners."""
+    dev = need_cuda()
+    verify(Setup([(i * 13) % 37 for i in range(700)], heads=2, kv_heads=1, d=64), "decode", dev)
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f32"])
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("heads,kv_heads", [(2, 2), (8, 2), (7, 1), (12, 4)])
+def test_extend_ragged(dt, d, heads, kv_heads):
+    dev = need_cuda()
+    verify(Setup([5, 0, 140, 64, 31, 1], new=[5, 0, 30, 64, 1, 1], heads=heads, kv_heads=kv_heads, d=d, dtype=DT[dt]),
+           "extend", dev)
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f32"])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("groups", [[(4, 100)], [(1, 17), (3, 300)]], ids=["one", "two"])
+def test_extend_behind_prefix(dt, d, groups):
+    dev = need_cuda()
+    verify(Setup([20, 130, 3, 64], new=[20, 70, 0, 2], groups=groups, heads=8, kv_heads=2, d=d, dtype=DT[dt], page=32),
+           "extend", dev)
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f32"])
+@pytest.mark.parametrize("new,kv", [(1, 1), (1, 3000), (7, 2000), (127, 127), (128, 128), (129, 129), (257, 700),
+                                    (600, 600)])
+def test_extend_one_sequence(dt, new, kv):
+    dev = need_cuda()
+    verify(Setup([kv], new=[new], heads=8, kv_heads=2, d=128, dtype=DT[dt], page=64), "extend", dev)
+
+
+@pytest.mark.parametrize("page", [16, 128, 256])
+@pytest.mark.parametrize("layout", ["nhd", "joint"])
+def test_extend_pages_and_layouts(page, layout):
+    dev = need_cuda()
+    verify(Setup([400, 333], new=[150, 333], groups=[(2, 77)], heads=4, kv_heads=2, d=128, page=page, layout=layout),
+           "extend", dev)
+
+
+@pytest.mark.parametrize("op", ["decode", "extend"])
+@pytest.mark.parametrize("dt", ["bf16", "f32"])
+def test_tokens_without_rows_see_the_prefix_only(op, dt):
+    """More new tokens than rows: the first ones see nothing of their own, and without a prefix give zeros."""
+    dev = need_cuda()
+    if op == "decode":
+        s = Setup([0, 3], heads=4, kv_heads=2, dtype=DT[dt])
+    else:
+        s = Setup([2, 0, 40], new=[5, 4, 40], heads=4, kv_heads=2, dtype=DT[dt])
+    got = verify(s, op, dev)
+    assert not got[0].any()
+
+
+def test_scores_of_one_sign_and_large_scores():
+    """Softmax over scores far from zero: only differences count."""
+    dev = need_cuda()
+    s = Setup([300, 80], heads=4, kv_heads=2, d=128)
+    s.q *= 30
+    verify(s, "decode", dev)
+    s.k[..., 0] = torch.where(s.k[..., 0].isnan(), s.k[..., 0], torch.full_like(s.k[..., 0], -50.0))
+    verify(s, "decode", dev)
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.1, 1.0])
+@pytest.mark.parametrize("op", ["decode", "extend"])
+def test_scales(op, scale):
+    dev = need_cuda()
+    new = None if op == "decode" else [40, 3]
+    verify(Setup([90, 33], new=new, heads=4, kv_heads=2, d=64), op, dev, scale=scale)
+
+
+@pytest.mark.parametrize("op", ["decode", "extend"])
+def test_infinite_rows_outside_the_lengths(op):
+    dev = need_cuda()
+    new = None if op == "decode" else [40, 3]
+    for stale in (math.inf, -math.inf, torch.finfo(torch.bfloat16).min):
+        verify(Setup([90, 33], new=new, groups=[(2, 21)], heads=4, kv_heads=2, d=64, stale=stale), op, dev)
+
+
+@pytest.mark.parametrize("op", ["decode", "extend"])
+@pytest.mark.parametrize("dt", ["bf16", "f32"])
+def test_same_bits_every_time_and_on_another_stream(op, dt):
+    dev = need_cuda()
+    n = 40
+    kv = [(91 * i) % 400 for i in range(n)]
+    new = None if op == "decode" else [min(k, (7 * i) % 60) for i, k in enumerate(kv)]
+    s = Setup(kv, new=new, groups=[(15, 210), (25, 33)], heads=8, kv_heads=2, d=128, dtype=DT[dt])
+    k, v = s.pools(dev)
+    c, b, q = cbq.PagedKVCache(k, v), s.batch(cbq, dev, decode=op == "decode"), s.q.to(dev)
+    f = c.attend_decode if op == "decode" else c.attend_extend
+    first = f(b, q)
+    side = torch.cuda.Stream(dev)
+    side.wait_stream(torch.cuda.current_stream(dev))
+    with torch.cuda.stream(side):
+        others = [f(b, q) for _ in range(5)]
+    torch.cuda.current_stream(dev).wait_stream(side)
+    for o in others:
+        assert torch.equal(o, first)
+
+
+def test_graph_follows_the_lengths():
+    """A captured decode step reads tables and lengths on the device."""
+    dev = need_cuda()
+    s = Setup([200, 100, 50], groups=[(3, 64)], heads=8, kv_heads=2, d=128, stale=0.0)
+    k, v = s.pools(dev)
+    c, b, q = cbq.PagedKVCache(k, v), s.batch(cbq, dev, decode=True), s.q.to(dev)
+    out = torch.empty_like(q)
+    c.attend_decode(b, q, out=out)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        c.attend_decode(b, q, out=out)
+    for kv in ([200, 100, 50], [1, 0, 37], [180, 99, 2]):
+        s.kv = kv
+        b.kv_lens.copy_(torch.tensor(kv, dtype=torch.int32))
+        g.replay()
+        torch.cuda.synchronize()
+        check_attention(out, *s.attention(s.d ** -0.5, False))
+
+
+def test_query_slices_of_one_projection():
+    dev = need_cuda()
+    s = Setup([70, 33, 9], heads=4, kv_heads=2, d=64)
+    k, v = s.pools(dev)
+    qkv = torch.randn(3, 4 + 2 * 2, 64, device=dev).to(torch.bfloat16)
+    qkv[:, :4] = s.q.to(dev)
+    got = cbq.PagedKVCache(k, v).attend_decode(s.batch(cbq, dev, decode=True), qkv[:, :4])
+    check_attention(got, *s.attention(s.d ** -0.5, False))
+
+
+@pytest.mark.parametrize("op", ["decode", "extend"])
+@pytest.mark.parametrize("bad", [-1, 1 << 20])
+def test_pages_outside_the_pool_read_as_zeros(op, bad):
+    dev = need_cuda()
+    s = Setup([40, 33], new=None if op == "decode" else [3, 2], heads=4, kv_heads=2, d=64, stale=0.0, spare=1)
+    # the oracle's page of zeros: a spare one
+    used = set(s.table[s.table >= 0].tolist())
+    spare = next(i for i in range(s.pages) if i not in used)
+    s.table[0, 1] = spare
+    ref = s.attention(s.d ** -0.5, op == "extend")
+    s.table[0, 1] = bad
+    status = cbq.PagedBatch.new_status(dev)
+    got = run(s, op, dev, status=status)
+    check_attention(got, *ref)
+    assert int(status[0]) & L.FLAG_CORRUPT
+    with pytest.raises(L.CbqError):
+        cbq.paged.check_status(status)
+
+
+def test_lengths_above_the_table_are_cut():
+    dev = need_cuda()
+    s = Setup([48, 33], heads=4, kv_heads=2, d=64)
+    ref = s.attention(s.d ** -0.5, False)
+    status = cbq.PagedBatch.new_status(dev)
+    b = s.batch(cbq, dev, decode=True, status=status)
+    b.kv_lens[0] = 1000
+    k, v = s.pools(dev)
+    check_attention(cbq.PagedKVCache(k, v).attend_decode(b, s.q.to(dev)), *ref)
+    assert int(status[0]) & L.FLAG_CORRUPT
+    status = cbq.PagedBatch.new_status(dev)
+    run(s, "decode", dev, status=status)
+    assert int(status[0]) == 0
+    cbq.paged.check_status(status)
+
+
+def test_sequences_that_share_pages():
+    """Two sequences may name the same pages (a forked conversation)."""
+    dev = need_cuda()
+    s = Setup([100, 90], heads=4, kv_heads=2, d=64)
+    s.table[1] = s.table[0]
+    verify(s, "decode", dev)
+
+
+def test_offsets_past_32_bits():
+    """A pool of more than 2^31 elements: rows at its end."""
+    dev = need_cuda()
+    page, d, hkv = 256, 128, 8
+    pages = (1 << 31) // (page * d * hkv) + 40
+    k = torch.empty(pages, hkv, page, d, dtype=torch.bfloat16, device=dev)
+    v = torch.empty_like(k)
+    s = Setup([700, 513], heads=8, kv_heads=hkv, d=d, page=page)
+    far = pages - s.pages
+    k[far:] = s.k.to(dev)
+    v[far:] = s.v.to(dev)
+    ref = s.attention(s.d ** -0.5, False)
+    s.table = torch.where(s.table >= 0, s.table + far, s.table)
+    got = cbq.PagedKVCache(k, v).attend_decode(s.batch(cbq, dev, decode=True), s.q.to(dev))
+    check_attention(got, *ref)
+
+
+def test_empty_calls():
+    dev = need_cuda()
+    s = Setup([3, 4], new=[0, 0], heads=4, kv_heads=2, d=64)
+    assert run(s, "extend", dev).shape == (0, 4, 64)
+    e = torch.empty(0, 1, dtype=torch.int32, device=dev)
+    b = cbq.PagedBatch(e, torch.empty(0, dtype=torch.int32, device=dev))
+    k, v = s.pools(dev)
+    assert cbq.PagedKVCache(k, v).attend_decode(b, s.q.to(dev)).shape == (0, 4, 64)
+
+
+# ------------------------------------------------------------------- append
+def tables(d, n):
+    qd = __import__("importlib").import_module("codebook-quantization_b200.qwen3_decode")
+    return qd.rope_tables(d, n, 1e6, "cpu")
+
+
+def append_oracle(s, q, k, v, cos, sin, eps, qw, kw):
+    kp, vp, out, scale = s.k.double(), s.v.double(), torch.zeros(s.tokens, s.heads, s.d, dtype=torch.float64), None
+    h, t = s.d // 2, 0
+
+    def turn(x, w, p):
+        x = x.double()
+        if eps >= 0:
+            x = x / torch.sqrt((x * x).mean(-1, keepdim=True) + eps)
+            x = x if w is None else x * w.double()
+        c, z = cos[p].double(), sin[p].double()
+        return torch.cat((x[..., :h] * c[:h] - x[..., h:] * z[:h], x[..., h:] * c[h:] + x[..., :h] * z[h:]), -1)
+
+    for i in range(s.n):
+        for a in range(s.new[i]):
+            r = s.kv[i] - s.new[i] + a
+            if r >= 0:
+                p = r + (s.plens[s.group_of[i]] if s.group_of[i] >= 0 else 0)
+                page, line = s.table[i, r // s.page], r % s.page
+                out[t] = turn(q[t], qw, p)
+                kp[page, :, line] = turn(k[t], kw, p)
+                vp[page, :, line] = v[t].double()
+            t += 1
+    return out, kp, vp
+
+
+def same(got, ref):
+    """One rounding of an fp32 result: half an ulp of the type, and the fp32
+    arithmetic of a norm and a rotation (a few 2^-24 of the values' size; the
+    size of a rotated pair is bounded by the row's largest element times 2)."""
+    g = got.double().cpu()
+    assert torch.equal(g.isnan(), ref.isnan())
+    u = 2.0 ** -8 if got.dtype == torch.bfloat16 else 2.0 ** -24
+    size = ref.nan_to_num(0.0).abs().amax(-1, keepdim=True) * 2
+    tol = u * ref.abs() + 16 * 2.0 ** -24 * size
+    assert bool(((g - ref).abs() <= tol).logical_or(ref.isnan()).all())
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f32"])
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("case", ["one", "decode", "prompts", "prefix"])
+@pytest.mark.parametrize("norm", ["weights", "unit", "none"])
+def test_append(dt, d, case, norm):
+    dev = need_cuda()
+    kw = dict(d=d, dtype=DT[dt], heads=6, kv_heads=2)
+    s = {"one": lambda: Setup([33], **kw),
+         "decode": lambda: Setup([1, 0, 16, 17, 300], page=32, layout="nhd", **kw),
+         "prompts": lambda: Setup([40, 5, 90, 64], new=[40, 0, 3, 17], page=16, layout="joint", **kw),
+         "prefix": lambda: Setup([40, 5, 90, 64], new=[7, 5, 1, 64], groups=[(1, 9), (3, 100)], page=64, **kw)}[case]()
+    qkv = torch.randn(s.tokens, s.heads + 2 * s.kv_heads, d).to(DT[dt])
+    q, k, v = qkv.split((s.heads, s.kv_heads, s.kv_heads), 1)
+    cos, sin = tables(d, 500)
+    qw, kw_ = (torch.rand(d) + 0.5, torch.rand(d) + 0.5) if norm == "weights" else (None, None)
+    eps = -1.0 if norm == "none" else 1e-6
+    kp, vp = s.pools(dev)
+    status = cbq.PagedBatch.new_status(dev)
+    on = qkv.to(dev)
+    b = s.batch(cbq, dev, decode=case in ("one", "decode"), status=status)
+    got = cbq.PagedKVCache(kp, vp).append_rope(
+        b, on[:, :s.heads], on[:, s.heads:s.heads + s.kv_heads], on[:, s.heads + s.kv_heads:], cos.to(dev),
+        sin.to(dev), eps=eps, q_weight=None if qw is None else qw.to(dev),
+        k_weight=None if kw_ is None else kw_.to(dev))
+    ref, rk, rv = append_oracle(s, q, k, v, cos, sin, eps, qw, kw_)
+    same(got, ref)
+    same(kp, rk)
+    assert torch.equal(vp.cpu().nan_to_num(7.0), rv.to(DT[dt]).nan_to_num(7.0))
+    assert int(status[0]) == 0
+
+
+def test_append_outside_the_tables_writes_nothing():
+    dev = need_cuda()
+    s = Setup([33, 16, 20, 8], heads=4, kv_heads=2, d=64, stale=0.0)
+    s.table[0, 2] = s.pages                            # no such page
+    cos, sin = tables(64, 18)                          # no position 19 (sequence 2)
+    qkv = torch.randn(4, 8, 64, device=dev).to(torch.bfloat16)
+    kp, vp = s.pools(dev)
+    k0, v0 = kp.clone(), vp.clone()
+    status = cbq.PagedBatch.new_status(dev)
+    b = s.batch(cbq, dev, decode=True, status=status)
+    b.kv_lens[1] = 500                                 # beyond the table's row
+    got = cbq.PagedKVCache(kp, vp).append_rope(b, qkv[:, :4], qkv[:, 4:6], qkv[:, 6:], cos.to(dev), sin.to(dev))
+    assert not got[:3].any() and got[3].any()
+    page = int(s.table[3, 0])
+    assert not torch.equal(kp[page], k0[page])
+    kp[page], vp[page] = k0[page], v0[page]
+    assert torch.equal(kp, k0) and torch.equal(vp, v0)
+    assert int(status[0]) & L.FLAG_CORRUPT and int(status[2]) == 3

@@ -1,0 +1,93 @@
+"""What the paged-cache operators refuse, on the host, before any CUDA call."""
+import ctypes as ct
+import struct
+
+import pytest
+import torch
+
+from helpers import cbq
+
+L = cbq._lib
+lib = L.lib
+
+
+def cache(**kw):
+    f = dict(k=4096, v=8192, pages=4, kv_heads=2, page_size=16, head_dim=64, page_stride=2048, head_stride=1024,
+             row_stride=64, dtype=L.CBQ_BF16)
+    f.update(kw)
+    return ct.create_string_buffer(struct.pack("<10q", *f.values()), 80)
+
+
+def batch(**kw):
+    f = dict(seqs=2, cu=0, lens=64, table=64, width=3, stride=3, max_kv=48, groups=0, gs=0, plens=0, ptable=0, pwidth=0,
+             pstride=0, max_prefix=0, status=0)
+    f.update(kw)
+    return ct.create_string_buffer(struct.pack("<15q", *f.values()), 120)
+
+
+def attend(c, b, tokens=2, q=256, qs=256, heads=4, out=512, ws=0, nws=0, name="cbq_paged_attn_decode"):
+    return getattr(lib(), name)(c, b, tokens, q, qs, heads, 0.125, out, ws, nws, None)
+
+
+def append(c, b, tokens=2, q=256, qs=256, k=256, ks=128, v=256, vs=128, heads=4, cos=256, sin=256, n=10, out=512):
+    return lib().cbq_paged_append_rope(c, b, tokens, q, qs, k, ks, v, vs, heads, 1e-6, None, None, cos, sin, n, out, None)
+
+
+ARG, NO = L.CBQ_ERR_ARG, L.CBQ_ERR_UNSUPPORTED
+
+
+@pytest.mark.parametrize("bad,rc", [
+    (dict(dtype=2), ARG), (dict(pages=-1), ARG), (dict(kv_heads=0), ARG), (dict(kv_heads=3), ARG),
+    (dict(head_dim=96), NO), (dict(page_size=8), NO), (dict(page_size=48), NO), (dict(page_size=512), NO),
+    (dict(k=0), ARG), (dict(v=0), ARG), (dict(k=4100), ARG), (dict(row_stride=32), ARG), (dict(row_stride=68), ARG),
+    (dict(page_stride=2052), ARG), (dict(head_stride=-64), ARG)], ids=str)
+def test_cache_refusals(bad, rc):
+    assert attend(cache(**bad), batch()) == rc
+    assert attend(cache(**bad), batch(), name="cbq_paged_attn_extend") == rc
+    assert append(cache(**bad), batch()) == rc
+
+
+@pytest.mark.parametrize("bad,rc", [
+    (dict(seqs=-1), ARG), (dict(lens=0), ARG), (dict(table=0), ARG), (dict(stride=2), ARG), (dict(width=-1), ARG),
+    (dict(max_kv=-1), ARG), (dict(groups=3), ARG), (dict(groups=1), ARG), (dict(groups=-1), ARG),
+    (dict(groups=1, gs=64, plens=64, ptable=64, pwidth=2, pstride=1), ARG), (dict(seqs=70000), NO),
+    (dict(seqs=3), ARG), (dict(width=1 << 28, stride=1 << 28), NO)], ids=str)
+def test_batch_refusals(bad, rc):
+    assert attend(cache(), batch(**bad)) == rc
+    assert append(cache(), batch(**bad)) == rc
+
+
+def test_null_descriptors():
+    assert attend(None, batch()) == ARG and attend(cache(), None) == ARG
+    assert append(None, batch()) == ARG and append(cache(), None) == ARG
+    assert lib().cbq_paged_attn_workspace_bytes(None, None, 1, 1, 0) == -1
+
+
+def test_append_argument_refusals():
+    c, b = cache(), batch()
+    for bad in (dict(q=0), dict(k=0), dict(v=0), dict(cos=0), dict(sin=0), dict(out=0), dict(q=264), dict(out=520),
+                dict(qs=128), dict(ks=64), dict(vs=132), dict(qs=260), dict(n=-1), dict(heads=3), dict(heads=0),
+                dict(tokens=-1), dict(tokens=1)):
+        assert append(c, b, **bad) == ARG, bad
+    assert append(c, b, heads=2 * 65, qs=2 * 65 * 64) == NO
+    assert append(cache(), batch(seqs=0, lens=0, table=0), tokens=0) == L.CBQ_OK
+
+
+def test_nothing_to_do_is_ok():
+    assert attend(cache(), batch(seqs=0), tokens=0) == L.CBQ_OK
+    assert attend(cache(), batch(cu=64), tokens=0, name="cbq_paged_attn_extend") == L.CBQ_OK
+    assert attend(cache(), batch(seqs=0, cu=64), tokens=3, name="cbq_paged_attn_extend") == ARG
+
+
+def test_python_refusals():
+    k = torch.zeros(4, 2, 16, 64)
+    with pytest.raises(RuntimeError):
+        cbq.PagedKVCache(k, k)                         # no CPU fallback
+    t, n = torch.zeros(2, 3, dtype=torch.int32), torch.zeros(2, dtype=torch.int32)
+    cbq.PagedBatch(t, n)
+    for a, kw in (((t.long(), n), {}), ((t, n.long()), {}), ((t[0], n), {}), ((t[:1], n), {}),
+                  ((t, n), dict(cu_tokens=n)), ((t, n), dict(prefix_lens=n)),
+                  ((t, n), dict(prefix_lens=n, group_starts=n, prefix_table=t)),
+                  ((t, n), dict(status=n)), ((t.T.contiguous().T, n), {})):
+        with pytest.raises(ValueError):
+            cbq.PagedBatch(*a, **kw)
