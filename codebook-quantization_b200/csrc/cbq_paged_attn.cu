@@ -8,100 +8,22 @@
 // scaled by 2^(m - M) and added.  m, l and o are fp32 everywhere.
 //
 // k_paged_stream is the kernel for few query rows per kv head: the cache is
-// read once and its bytes bound it.  The work is one line of key tiles
-// (owner, kv head, row tile, tile): an owner is a sequence (its own rows, or
-// for extend its prefix and own rows) or a group (its prefix, the query rows of
-// all its sequences).  The line is cut into equal parts, one per resident CTA,
-// so ragged lengths balance by themselves and a single long sequence spreads
-// over all SMs.  A CTA whose part holds all of a unit writes the result; other
-// units leave one (m, l, o) per part in the workspace, joined in part order by
-// k_paged_join.  All of it is found from the lengths on the device.
-#include <algorithm>
+// read once and its bytes bound it.  A CTA whose part of the line (see
+// cbq_paged_line.cuh) holds all of a unit writes the result; other units leave
+// one (m, l, o) per part in the workspace, joined in part order by k_join_cut
+// (whole units written directly) or k_join_rows (every unit has parts: the own
+// rows' and the prefix's).
 #include <mutex>
 
-#include "cbq_paged.cuh"
+#include "cbq_paged_line.cuh"
 
 namespace {
 
 using namespace cbq;
 
 constexpr int kKeys = 16;              // keys of a stage (one warp's unit of loads); page_size is a multiple
-constexpr float kLog2e = 1.4426950408889634f;
-
-enum StreamMode : int {
-    kOwn = 0,                          // owner = sequence, keys = its own rows (decode)
-    kPrefix = 1,                       // owner = group, keys = its prefix, rows = all its sequences' (decode)
-    kFull = 2,                         // owner = sequence, keys = prefix then own rows, causal (extend)
-};
-
-struct StreamArgs {
-    const void *q;
-    int64_t qs;                        // token stride, elements
-    int hq, G;
-    float sc;                          // scale * log2(e)
-    void *out;
-    float *part;                       // [slot][R * D + 2 * R] fp32: o, m, l
-    uint64_t *cum;                     // [owners + 1] units << 32 | tiles before each owner (for k_paged_join)
-    int64_t slots;                     // slots of `part` (starts that are not in order could name more)
-    int owners;
-    int mode;
-    int direct;                        // whole units go to `out`
-    int wait_first;                    // wait for the previous kernel before reading (else before the end only)
-};
-
-struct Owner {
-    int t0, nt;                        // its query tokens
-    int plen, olen;                    // prefix and own rows
-    int group;
-};
-
-// Largest i in [0, n) with a[i] <= x (one thread).
-__device__ __forceinline__ int upper(const int32_t *a, int n, int x) {
-    int lo = 0, hi = n;
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (a[mid] <= x) lo = mid; else hi = mid;
-    }
-    return lo;
-}
-
-__device__ __forceinline__ int clampi(int v, int lo, int hi) { return min(max(v, lo), hi); }
-
-__device__ __forceinline__ Owner owner_of(const PagedView &pv, int mode, int o) {
-    Owner w{};
-    w.group = -1;
-    if (mode == kPrefix) {
-        w.t0 = clampi(pv.gs[o], 0, pv.tokens);
-        w.nt = clampi(pv.gs[o + 1], w.t0, pv.tokens) - w.t0;
-        w.plen = clampi(pv.plens[o], 0, pv.pcap);
-        w.group = o;
-        return w;
-    }
-    if (pv.cu && mode == kFull) {
-        w.t0 = clampi(pv.cu[o], 0, pv.tokens);
-        w.nt = clampi(pv.cu[o + 1], w.t0, pv.tokens) - w.t0;
-    } else {
-        w.t0 = o;
-        w.nt = 1;
-    }
-    w.olen = clampi(pv.lens[o], 0, pv.cap);
-    if (mode == kFull && pv.groups) {
-        w.group = upper(pv.gs, pv.groups, o);
-        w.plen = clampi(pv.plens[w.group], 0, pv.pcap);
-    }
-    return w;
-}
-
-__device__ __forceinline__ int stages_of(const Owner &w) {
-    return (w.plen + kKeys - 1) / kKeys + (w.olen + kKeys - 1) / kKeys;
-}
 
 // ---------------------------------------------------------------- small PTX
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, bool ok) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
 }
@@ -126,17 +48,6 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
-    const __nv_bfloat162 b = __floats2bfloat162_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t *>(&b);
-}
-__device__ __forceinline__ void st4(float *p, float a, float b, float c, float d) {
-    *reinterpret_cast<float4 *>(p) = make_float4(a, b, c, d);
-}
-__device__ __forceinline__ void st4(__nv_bfloat16 *p, float a, float b, float c, float d) {
-    *reinterpret_cast<uint2 *>(p) = make_uint2(pack_bf16(a, b), pack_bf16(c, d));
-}
-
 // ------------------------------------------------------------ configuration
 template <typename T, int D, int NB> struct StreamCfg {
     static constexpr bool kF32 = sizeof(T) == 4;
@@ -155,59 +66,11 @@ template <typename T, int D, int NB> struct StreamCfg {
     static constexpr int kSlot = R * D + 2 * R;                         // floats of a workspace slot
 };
 
-// Position on the line of tiles: the unit it is in and where that ends.
-struct Cursor {
-    uint32_t w;                        // next tile
-    uint32_t base;                     // first tile of owner o
-    uint32_t ubase;                    // units before owner o
-    int o, tiles, rts;                 // tiles of a unit, row tiles of owner o
-    Owner ow;
-};
-struct Piece {
-    int h, rt, tb, te;                 // unit (h, rt) of the cursor's owner, its tiles [tb, te)
-};
-
-template <int R, int NW>
-__device__ __forceinline__ void cursor_owner(Cursor &c, const PagedView &pv, int mode, int G, int o) {
-    c.o = o;
-    c.ow = owner_of(pv, mode, o);
-    c.tiles = (stages_of(c.ow) + NW - 1) / NW;
-    c.rts = (c.ow.nt * G + R - 1) / R;
-}
-
-// The next piece of [.., w1); false at the end.  Leaves c.w behind it.
-template <int R, int NW>
-__device__ __forceinline__ bool next_piece(Cursor &c, const PagedView &pv, const StreamArgs &a, uint32_t w1, Piece &p) {
-    if (c.w >= w1) return false;
-    while (true) {
-        const uint32_t units = (uint32_t)(pv.kv_heads * c.rts), n = units * (uint32_t)c.tiles;
-        if (c.w < c.base + n) break;
-        if (c.o + 1 >= a.owners) return false;
-        c.base += n;
-        c.ubase += units;
-        cursor_owner<R, NW>(c, pv, a.mode, a.G, c.o + 1);
-    }
-    const uint32_t at = c.w - c.base, u = at / (uint32_t)c.tiles;
-    p.h = (int)(u / (uint32_t)c.rts);
-    p.rt = (int)(u - (uint32_t)p.h * c.rts);
-    p.tb = (int)(at - u * (uint32_t)c.tiles);
-    p.te = (int)min((uint32_t)c.tiles, p.tb + (w1 - c.w));
-    c.w += (uint32_t)(p.te - p.tb);
-    return true;
-}
-
-// Own rows visible to query row r of an owner (row r is token r / G).
-__device__ __forceinline__ int own_limit(const Owner &w, int r, int G) {
-    return clampi(w.olen - w.nt + r / G + 1, 0, w.olen);
-}
-
 // Stages of a unit that any of its rows can see.
-template <int R>
-__device__ __forceinline__ int unit_stages(const Owner &w, int rt, int G, int mode) {
+__device__ __forceinline__ int unit_stages(const Owner &w, int tt, const LineArgs &a) {
     const int np = (w.plen + kKeys - 1) / kKeys;
-    if (mode == kPrefix) return np;
-    const int last = min(rt * R + R, w.nt * G) - 1;
-    return np + (own_limit(w, last, G) + kKeys - 1) / kKeys;
+    if (a.mode == kPrefix) return np;
+    return np + (own_limit(w, min((tt + 1) * a.geo.tq, w.nt) - 1) + kKeys - 1) / kKeys;
 }
 
 // One warp's 16 keys starting at `key0` of a table, into its slot: K then V,
@@ -234,78 +97,6 @@ __device__ __forceinline__ void load_stage(const PagedView &pv, int page, int ke
     }
 }
 
-// The tile line: total, this CTA's part [w0, w1) and the owner w0 falls into.
-// CTA 0 leaves the sums before each owner in a.cum.
-template <int R, int NW>
-__device__ __forceinline__ bool plan_line(const PagedView &pv, const StreamArgs &a, Cursor &c, uint32_t &w1) {
-    constexpr int NT = 32 * NW;
-    __shared__ uint64_t red[NW];
-    __shared__ uint64_t found_base;
-    __shared__ int found;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    auto weight = [&](int o) -> uint64_t {
-        if (o >= a.owners) return 0;
-        const Owner w = owner_of(pv, a.mode, o);
-        if (blockIdx.x == 0 && (a.mode == kPrefix ? pv.plens[o] > pv.pcap : pv.lens[o] > pv.cap))
-            report(pv.status, CBQ_FLAG_CORRUPT, (uint32_t)o);
-        const uint32_t units = (uint32_t)(pv.kv_heads * ((w.nt * a.G + R - 1) / R));
-        return (uint64_t)units << 32 | units * (uint32_t)((stages_of(w) + NW - 1) / NW);
-    };
-    const uint64_t first = weight(tid);
-    uint64_t sum = first;
-    for (int o = tid + NT; o < a.owners; o += NT) sum += weight(o);
-#pragma unroll
-    for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-    if (lane == 0) red[warp] = sum;
-    if (tid == 0) found = -1;
-    __syncthreads();
-    uint64_t total = 0;
-#pragma unroll
-    for (int i = 0; i < NW; ++i) total += red[i];
-    const uint32_t W = (uint32_t)total;
-    const uint32_t per = (W + gridDim.x - 1) / gridDim.x;
-    const uint32_t w0 = min((uint64_t)per * blockIdx.x, (uint64_t)W);
-    w1 = min(w0 + per, W);
-    const bool writer = blockIdx.x == 0;
-    if (writer && tid == 0) a.cum[a.owners] = total;
-    if (w0 >= w1 && !writer) return false;
-    uint64_t run = 0;
-    for (int o0 = 0; o0 < a.owners; o0 += NT) {
-        const int o = o0 + tid;
-        const uint64_t x = o0 == 0 ? first : weight(o);
-        uint64_t inc = x;
-#pragma unroll
-        for (int d = 1; d < 32; d <<= 1) {
-            const uint64_t y = __shfl_up_sync(0xffffffffu, inc, d);
-            if (lane >= d) inc += y;
-        }
-        __syncthreads();                              // red[] of the previous use
-        if (lane == 31) red[warp] = inc;
-        __syncthreads();
-        uint64_t before = run, all = 0;
-#pragma unroll
-        for (int i = 0; i < NW; ++i) {
-            if (i < warp) before += red[i];
-            all += red[i];
-        }
-        const uint64_t ex = before + inc - x;
-        if (writer && o < a.owners) a.cum[o] = ex;
-        if (o < a.owners && (uint32_t)ex <= w0 && w0 < (uint32_t)ex + (uint32_t)x) {
-            found = o;
-            found_base = ex;
-        }
-        run += all;
-        if (!writer && (uint32_t)run > w0) break;      // the owner is in this block of owners
-    }
-    __syncthreads();
-    if (w0 >= w1 || found < 0) return false;
-    c.w = w0;
-    c.base = (uint32_t)found_base;
-    c.ubase = (uint32_t)(found_base >> 32);
-    cursor_owner<R, NW>(c, pv, a.mode, a.G, found);
-    return true;
-}
-
 // bf16: the warp computes S^T = K Q^T and O^T = V^T P^T with m16n8k16, keys
 // (then dimensions of V) on the 16-row side and the query rows on the 8-column
 // side, so 1..8 query rows waste none of the long side; P^T turns into the
@@ -313,7 +104,7 @@ __device__ __forceinline__ bool plan_line(const PagedView &pv, const StreamArgs 
 // takes key l % 16 and half the 8 query rows for the scores, and D / 32
 // dimensions of all rows for the sums; fp32 FMAs.
 template <typename T, int D, int NB>
-__global__ void __launch_bounds__(StreamCfg<T, D, NB>::NT) k_paged_stream(const PagedView pv, const StreamArgs a) {
+__global__ void __launch_bounds__(StreamCfg<T, D, NB>::NT) k_paged_stream(const PagedView pv, const LineArgs a) {
     using Cfg = StreamCfg<T, D, NB>;
     constexpr bool kF32 = Cfg::kF32;
     constexpr int R = Cfg::R, NW = Cfg::NW, NT = Cfg::NT, S = Cfg::S, kPitch = Cfg::kPitch;
@@ -328,22 +119,22 @@ __global__ void __launch_bounds__(StreamCfg<T, D, NB>::NT) k_paged_stream(const 
 
     Cursor cons{};
     uint32_t w1 = 0;
-    const bool any = plan_line<R, NW>(pv, a, cons, w1);
+    const bool any = plan_line<NT>(pv, a, cons, w1);
     if (any) {
         Cursor load = cons;
         Piece lp{};
-        bool lgo = next_piece<R, NW>(load, pv, a, w1, lp);
+        bool lgo = next_piece(load, pv, a, w1, lp);
         int lt = lp.tb;
         const uint32_t ring = smem_u32(smem) + warp * S * Cfg::kStage;
         // fills ring slot `slot` with this warp's next stage on the line, or with nothing
         auto issue = [&](int slot) {
             while (lgo && lt == lp.te) {
-                lgo = next_piece<R, NW>(load, pv, a, w1, lp);
+                lgo = next_piece(load, pv, a, w1, lp);
                 lt = lp.tb;
             }
             if (lgo) {
                 const int st = lt * NW + warp;
-                if (st < unit_stages<R>(load.ow, lp.rt, a.G, a.mode)) {
+                if (st < unit_stages(load.ow, lp.tt, a)) {
                     const int np = (load.ow.plen + kKeys - 1) / kKeys;
                     const bool pre = st < np;
                     const int key0 = (pre ? st : st - np) * kKeys, lim = pre ? load.ow.plen : load.ow.olen;
@@ -363,16 +154,21 @@ __global__ void __launch_bounds__(StreamCfg<T, D, NB>::NT) k_paged_stream(const 
         for (int i = 0; i < S - 1; ++i) issue(i);
         int it = 0;                                    // ring uses
         Piece p;
-        while (next_piece<R, NW>(cons, pv, a, w1, p)) {
+        while (next_piece(cons, pv, a, w1, p)) {
             const Owner &ow = cons.ow;
-            const int r0 = p.rt * R, nrows = min(R, ow.nt * a.G - r0);
-            const int np = (ow.plen + kKeys - 1) / kKeys, nst = unit_stages<R>(ow, p.rt, a.G, a.mode);
-            // query row r: token t0 + (r0 + r) / G, head h G + (r0 + r) % G
-            auto q_row = [&](int r) {
-                const int x = r0 + r, tk = x / a.G;
-                return static_cast<const T *>(a.q) + (int64_t)(ow.t0 + tk) * a.qs + (p.h * a.G + x - tk * a.G) * D;
+            const int np = (ow.plen + kKeys - 1) / kKeys, nst = unit_stages(ow, p.tt, a);
+            // row r of the unit: token tok0 + r / gb, query head head0 + r % gb
+            const int gb = min(a.geo.G, R), tok0 = p.tt * a.geo.tq;
+            const int hleft = min(a.geo.G - p.hc * R, gb);            // heads of this chunk
+            const int head0 = p.h * a.geo.G + p.hc * R;
+            const int nrows = hleft < gb ? hleft : min(a.geo.tq, ow.nt - tok0) * gb;
+            auto token = [&](int r) { return tok0 + r / gb; };
+            auto row_at = [&](int r, int64_t stride) {
+                const int tk = r / gb;
+                return (int64_t)(ow.t0 + tok0 + tk) * stride + (int64_t)(head0 + r - tk * gb) * D;
             };
-            const int lim_first = a.mode == kPrefix ? 0 : own_limit(ow, r0, a.G);
+            auto q_row = [&](int r) { return static_cast<const T *>(a.q) + row_at(r, a.qs); };
+            const int lim_first = a.mode == kPrefix ? 0 : own_limit(ow, tok0);
             if constexpr (!kF32) {
                 constexpr int KK = D / 16;
                 const int rq = lane >> 2, cq = (lane & 3) * 2;
@@ -393,7 +189,7 @@ __global__ void __launch_bounds__(StreamCfg<T, D, NB>::NT) k_paged_stream(const 
                 for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
-                        lim[nb][e] = a.mode == kPrefix ? 0 : own_limit(ow, r0 + nb * 8 + cq + e, a.G);
+                        lim[nb][e] = a.mode == kPrefix ? 0 : own_limit(ow, token(nb * 8 + cq + e));
                         m[nb][e] = -INFINITY;
                         l[nb][e] = 0.f;
 #pragma unroll
@@ -502,7 +298,7 @@ __global__ void __launch_bounds__(StreamCfg<T, D, NB>::NT) k_paged_stream(const 
                 float m[4], l[4], o[8][E];
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    lim[r] = a.mode == kPrefix ? 0 : own_limit(ow, r0 + rh + r, a.G);
+                    lim[r] = a.mode == kPrefix ? 0 : own_limit(ow, token(rh + r));
                     m[r] = -INFINITY;
                     l[r] = 0.f;
                 }
@@ -604,10 +400,9 @@ __global__ void __launch_bounds__(StreamCfg<T, D, NB>::NT) k_paged_stream(const 
             }
             __syncthreads();
             // the NW warps' states joined in warp order; a whole unit is the
-            // result, a part of one goes to its slot (units started so far + CTA:
-            // one number per piece, in line order)
-            const bool whole = a.direct && p.tb == 0 && p.te == cons.tiles;
-            const int64_t slot = (int64_t)cons.ubase + p.h * cons.rts + p.rt + blockIdx.x;
+            // result, a part of one goes to its slot
+            const bool whole = a.direct && p.tb == 0 && p.te == p.tiles;
+            const int64_t slot = slot_of(cons, p, a, (int)blockIdx.x);
             float *ps = a.part + slot * Cfg::kSlot;
             for (int e = tid; e < nrows * (D / 4); e += NT) {
                 const int r = e / (D / 4), d = (e - r * (D / 4)) * 4;
@@ -628,10 +423,7 @@ __global__ void __launch_bounds__(StreamCfg<T, D, NB>::NT) k_paged_stream(const 
                 }
                 if (whole) {
                     const float inv = L == 0.f ? 0.f : 1.f / L;
-                    const int x = r0 + r, tk = x / a.G;
-                    T *dst = static_cast<T *>(a.out) +
-                             ((int64_t)(ow.t0 + tk) * a.hq + p.h * a.G + x - tk * a.G) * D + d;
-                    st4(dst, y[0] * inv, y[1] * inv, y[2] * inv, y[3] * inv);
+                    st4(static_cast<T *>(a.out) + row_at(r, (int64_t)a.hq * D) + d, y[0] * inv, y[1] * inv, y[2] * inv, y[3] * inv);
                 } else if (slot < a.slots) {
                     st4(ps + r * D + d, y[0], y[1], y[2], y[3]);
                     if (d == 0) {
@@ -648,78 +440,47 @@ __global__ void __launch_bounds__(StreamCfg<T, D, NB>::NT) k_paged_stream(const 
 }
 
 // ------------------------------------------------------------------- joining
-// Where the parts of a query row lie.
+// The parts of a line that a launch left.
 struct JoinSource {
     const float *part;
     const uint64_t *cum;
     int64_t slots;
-    int owners, grid, R;               // of the k_paged_stream launch that left them
-};
-struct JoinArgs {
-    JoinSource own, pre;               // pre.part null: no prefix parts
-    int hq, G, full;                   // full: own parts belong to extend units
-    void *out;
+    int owners, grid, min_tiles, rows, tile_rows, mode, direct;
+    LineGeo geo;
 };
 
+// A query row's parts: the slot of part k and the row's place in it.
 struct Parts {
-    const float *base;                 // first part's slot
-    int64_t step;                      // floats to the next
-    int n, R, r;                       // parts, rows of a slot, this row
+    const JoinSource *s;
+    int64_t slot0;
+    int i0, n, row;
+
+    __device__ __forceinline__ const float *slot(int k, int d) const {
+        int64_t at = slot0 + k;
+        if (s->direct) at = 2 * (int64_t)(i0 + k) + (k == 0 ? 1 : 0);
+        return s->part + at * ((int64_t)s->rows * (d + 2));
+    }
 };
 
-template <int D>
-__device__ __forceinline__ Parts stream_parts(const JoinSource &s, int kv_heads, int o, int h, int r) {
-    Parts p{};
-    const uint64_t c0 = s.cum[o], c1 = s.cum[o + 1], all = s.cum[s.owners];
-    const int hkv_rts = (int)((c1 >> 32) - (c0 >> 32));
-    const uint32_t n = (uint32_t)c1 - (uint32_t)c0;
-    p.R = s.R;
-    const int rts = hkv_rts / kv_heads, rt = r / s.R;
-    if (n == 0 || r < 0 || rt >= rts) return p;
-    const uint32_t W = (uint32_t)all, per = (W + s.grid - 1) / s.grid;
-    const int tiles = (int)(n / (uint32_t)hkv_rts);
-    const int u = h * rts + rt;
-    const uint32_t w0 = (uint32_t)c0 + (uint32_t)u * tiles;
-    const uint32_t i0 = w0 / per, i1 = (w0 + tiles - 1) / per;
-    const int64_t slot = (int64_t)(c0 >> 32) + u + i0;
-    if (slot + (i1 - i0) >= s.slots) return p;
-    p.step = s.R * D + 2 * s.R;
-    p.base = s.part + slot * p.step;
-    p.n = (int)(i1 - i0 + 1);
-    p.r = r - rt * s.R;
-    return p;
+// Slot row of head gi of a unit's tl-th token (head chunk by head chunk where a token's heads are cut).
+__device__ __forceinline__ int slot_row(const JoinSource &s, int tl, int gi) {
+    if (s.tile_rows) {
+        const int tb = s.tile_rows / s.geo.G;
+        return tl / tb * s.tile_rows + tl % tb * s.geo.G + gi;
+    }
+    return s.geo.G <= s.rows ? tl * s.geo.G + gi : gi % s.rows;
 }
 
-// One warp per (token, query head): parts of the prefix then of the own rows.
+// One warp joins one query row over two lists of parts.
 template <typename T, int D>
-__global__ void __launch_bounds__(128) k_paged_join(const PagedView pv, const JoinArgs a) {
+__device__ __forceinline__ void join_row(const Parts &pa, const Parts &pb, T *dst) {
     constexpr int E = D / 32;
-    pdl_launch_dependents();
-    pdl_wait();
-    const int lane = threadIdx.x & 31;
-    const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-    if (row >= (int64_t)pv.tokens * a.hq) return;
-    const int t = (int)(row / a.hq), hq = (int)(row - (int64_t)t * a.hq);
-    const int h = hq / a.G, gi = hq - h * a.G;
-    int s = t, t0 = t;
-    if (a.full && pv.cu) {
-        s = warp_upper(pv.cu, pv.seqs, t);
-        t0 = pv.cu[s];
-    }
-    Parts po = stream_parts<D>(a.own, pv.kv_heads, s, h, (t - t0) * a.G + gi), pp{};
-    if (a.pre.part) {
-        const int g = warp_upper(pv.gs, pv.groups, s);
-        pp = stream_parts<D>(a.pre, pv.kv_heads, g, h, (s - pv.gs[g]) * a.G + gi);
-    } else if (po.n == 1) {
-        return;                                        // a whole unit: written already
-    }
-    const int n = pp.n + po.n;
-    auto part = [&](int i) { return i < pp.n ? pp.base + i * pp.step : po.base + (i - pp.n) * po.step; };
+    const int lane = threadIdx.x & 31, n = pa.n + pb.n;
     auto stat = [&](int i, float &m, float &l) {
-        const Parts &x = i < pp.n ? pp : po;
-        const float *b = part(i) + (int64_t)x.R * D;
-        m = __ldcg(b + x.r);
-        l = __ldcg(b + x.R + x.r);
+        const Parts &x = i < pa.n ? pa : pb;
+        const float *b = x.slot(i < pa.n ? i : i - pa.n, D) + (int64_t)x.s->rows * D;
+        m = __ldcg(b + x.row);
+        l = __ldcg(b + x.s->rows + x.row);
     };
     float M = -INFINITY;
     for (int i0 = 0; i0 < n; i0 += 32) {
@@ -741,8 +502,8 @@ __global__ void __launch_bounds__(128) k_paged_join(const PagedView pv, const Jo
 #pragma unroll 4
         for (int i = 0; i < top; ++i) {
             const float fi = __shfl_sync(0xffffffffu, f, i);
-            const Parts &x = i0 + i < pp.n ? pp : po;
-            const float *b = part(i0 + i) + (int64_t)x.r * D + lane * E;
+            const Parts &x = i0 + i < pa.n ? pa : pb;
+            const float *b = x.slot(i0 + i < pa.n ? i0 + i : i0 + i - pa.n, D) + (int64_t)x.row * D + lane * E;
             if constexpr (E == 2) {
                 const float2 v = __ldcg(reinterpret_cast<const float2 *>(b));
                 y[0] = fmaf(v.x, fi, y[0]);
@@ -761,59 +522,108 @@ __global__ void __launch_bounds__(128) k_paged_join(const PagedView pv, const Jo
     }
     L = warp_sum(L);
     const float inv = L == 0.f ? 0.f : 1.f / L;
-    T *dst = static_cast<T *>(a.out) + row * D + lane * E;
+    if constexpr (E == 2) {
+        dst[lane * 2] = from_f32<T>(y[0] * inv);
+        dst[lane * 2 + 1] = from_f32<T>(y[1] * inv);
+    } else {
 #pragma unroll
-    for (int e = 0; e < E; ++e) dst[e] = from_f32<T>(y[e] * inv);
+        for (int e = 0; e < E; e += 4)
+            st4(dst + lane * E + e, y[e] * inv, y[e + 1] * inv, y[e + 2] * inv, y[e + 3] * inv);
+    }
+}
+
+// Decode over a shared prefix: every unit left parts, all units of an owner
+// have the same tiles.  Parts of the row of token `tl` of owner o, head (h, gi).
+__device__ __forceinline__ Parts even_parts(const JoinSource &s, int kv_heads, int o, int tl, int h, int gi) {
+    Parts p{};
+    p.s = &s;
+    const uint64_t c0 = s.cum[o], c1 = s.cum[o + 1], all = s.cum[s.owners];
+    const uint32_t nu = (uint32_t)(c1 >> 32) - (uint32_t)(c0 >> 32), n = (uint32_t)c1 - (uint32_t)c0;
+    const int per_h = (int)(nu / (uint32_t)kv_heads), tts = per_h / s.geo.hc, tt = tl / s.geo.tq;
+    if (n == 0 || tl < 0 || tt >= tts) return p;
+    const uint32_t per = tiles_per_cta((uint32_t)all, (uint32_t)s.grid, (uint32_t)s.min_tiles), tiles = n / nu;
+    const int hc = s.geo.hc > 1 ? gi / s.rows : 0;
+    const uint32_t u = (uint32_t)(h * per_h + tt * s.geo.hc + hc), w0 = (uint32_t)c0 + u * tiles;
+    p.i0 = (int)(w0 / per);
+    p.slot0 = (int64_t)(c0 >> 32) + u + p.i0;
+    p.n = (int)((w0 + tiles - 1) / per) - p.i0 + 1;
+    p.row = slot_row(s, tl - tt * s.geo.tq, gi);
+    if (p.slot0 + p.n > s.slots) p.n = 0;
+    return p;
+}
+
+// One warp per (token, query head).
+template <typename T, int D>
+__global__ void __launch_bounds__(128) k_join_rows(const PagedView pv, const JoinSource own, const JoinSource pre, int hq,
+                                                   void *out) {
+    pdl_launch_dependents();
+    pdl_wait();
+    const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
+    if (row >= (int64_t)pv.tokens * hq) return;
+    const int t = (int)(row / hq), x = (int)(row - (int64_t)t * hq), h = x / own.geo.G, gi = x - h * own.geo.G;
+    const int g = warp_upper(pv.gs, pv.groups, t);
+    const Parts pp = even_parts(pre, pv.kv_heads, g, t - pv.gs[g], h, gi);
+    const Parts po = even_parts(own, pv.kv_heads, t, 0, h, gi);
+    join_row<T, D>(pp, po, static_cast<T *>(out) + row * D);
+}
+
+// Whole units are written; block x joins the unit cut by the boundary between
+// CTA x and CTA x + 1, if that is the first boundary inside it.  One warp per
+// row, blockIdx.y over blocks of rows.
+constexpr int kCutRows = 16;
+template <typename T, int D>
+__global__ void __launch_bounds__(128) k_join_cut(const PagedView pv, const LineArgs a, const JoinSource s) {
+    pdl_launch_dependents();
+    pdl_wait();
+    const uint32_t W = (uint32_t)s.cum[s.owners];
+    const uint32_t per = tiles_per_cta(W, (uint32_t)s.grid, (uint32_t)s.min_tiles);
+    const uint64_t wb = (uint64_t)per * (blockIdx.x + 1);
+    if (wb >= W) return;
+    const uint32_t w = (uint32_t)wb;
+    // the owner of tile w: the last whose first tile is not behind it (owners without units come before)
+    const int lane = threadIdx.x & 31;
+    int lo = 0, hi = s.owners;
+    while (hi - lo > 1) {
+        const int step = (hi - lo + 31) >> 5, i = lo + (lane + 1) * step;
+        const int c = __popc(__ballot_sync(0xffffffffu, i < hi && (uint32_t)s.cum[i] <= w));
+        lo += c * step;
+        hi = min(hi, lo + step);
+    }
+    Cursor c{};
+    c.base = (uint32_t)s.cum[lo];
+    cursor_owner(c, pv, a, lo);
+    if (c.wh == 0 || w - c.base >= (uint32_t)pv.kv_heads * c.wh) return;   // starts that are not in order
+    const Piece p = unit_at(c, s.geo, w - c.base);
+    const uint32_t w0 = w - (uint32_t)p.tb;
+    if (p.tb == 0 || (uint64_t)(w0 / per + 1) * per != wb) return;
+    Parts pa{}, none{};
+    pa.s = none.s = &s;
+    pa.i0 = (int)(w0 / per);
+    pa.n = (int)((w0 + (uint32_t)p.tiles - 1) / per) - pa.i0 + 1;
+    const int G = s.geo.G, gb = s.geo.hc > 1 ? min(s.rows, G - p.hc * s.rows) : G, tok0 = p.tt * s.geo.tq;
+    const int nrows = min(s.geo.tq, c.ow.nt - tok0) * gb;
+    for (int r = blockIdx.y * kCutRows + (threadIdx.x >> 5); r < min(nrows, ((int)blockIdx.y + 1) * kCutRows); r += 4) {
+        const int tl = r / gb, gi = p.hc * s.rows + r - tl * gb;
+        pa.row = slot_row(s, tl, gi);
+        join_row<T, D>(pa, none, static_cast<T *>(a.out) + ((int64_t)(c.ow.t0 + tok0 + tl) * a.hq + p.h * G + gi) * D);
+    }
 }
 
 // ---------------------------------------------------------------- host side
 
-// CTAs of `kern` that fit an SM (asked once per kernel and device), its
-// shared memory limit raised first.
-int resident(const void *kern, int threads, int smem, int *out) {
-    static std::mutex mu;
-    struct Entry { const void *kern; int dev, n; };
-    static Entry seen[256];
-    static int nseen = 0;
-    int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess) return CBQ_ERR_CUDA;
-    std::lock_guard<std::mutex> g(mu);
-    for (int i = 0; i < nseen; ++i)
-        if (seen[i].kern == kern && seen[i].dev == dev) {
-            *out = seen[i].n;
-            return CBQ_OK;
-        }
-    CBQ_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-    int n = 0;
-    CBQ_CUDA_TRY(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kern, threads, smem));
-    if (n < 1) return CBQ_ERR_UNSUPPORTED;
-    if (nseen < 256) seen[nseen++] = Entry{kern, dev, n};
-    *out = n;
-    return CBQ_OK;
-}
-
-// A k_paged_stream launch: its instantiation by row count, and its part of the workspace.
-struct StreamPlan {
-    int NB, R, NW, grid, slot;         // slot: floats
-    int owners;
-    int64_t units, cum_off, part_off, end;   // workspace bytes
-};
-
-template <typename T, int D, int NB> int stream_grid(StreamPlan *p) {
+template <typename T, int D, int NB> int stream_grid(cbq_host::LinePlan *p) {
     using Cfg = StreamCfg<T, D, NB>;
     int n = 0;
-    const int rc = resident(reinterpret_cast<const void *>(k_paged_stream<T, D, NB>), Cfg::NT, Cfg::kSmem, &n);
+    const int rc = cbq_host::resident_ctas(reinterpret_cast<const void *>(k_paged_stream<T, D, NB>), Cfg::NT, Cfg::kSmem, &n);
     if (rc != CBQ_OK) return rc;
-    p->NB = NB;
-    p->R = Cfg::R;
-    p->NW = Cfg::NW;
-    p->slot = Cfg::kSlot;
+    p->rows = Cfg::R;
+    p->geo.keys = kKeys * Cfg::NW;
     p->grid = n * cbq_host::sm_count();
     return CBQ_OK;
 }
 
 template <typename T, int D, int NB>
-int stream_launch(const PagedView &pv, const StreamArgs &a, int grid, cudaStream_t s) {
+int stream_launch(const PagedView &pv, const LineArgs &a, int grid, cudaStream_t s) {
     using Cfg = StreamCfg<T, D, NB>;
     CBQ_CUDA_TRY(cbq_host::launch_pdl(k_paged_stream<T, D, NB>, dim3((unsigned)grid), dim3(Cfg::NT), (size_t)Cfg::kSmem,
                                       s, pv, a));
@@ -836,41 +646,38 @@ int stream_launch(const PagedView &pv, const StreamArgs &a, int grid, cudaStream
         if ((nb) == 1) { CALL(__nv_bfloat16, 256, 1); } else { CALL(__nv_bfloat16, 256, 2); }        \
     }
 
-// Rows of a unit: as few blocks of 8 as hold an owner's rows (rows <= max_rows), at most 32.
-int plan_stream(const PagedView &pv, int dtype, int d, int G, int mode, int64_t max_rows, int64_t off, StreamPlan *p) {
-    const int nb = max_rows <= 8 ? 1 : (max_rows <= 16 ? 2 : 4);
+int row_blocks(int64_t rows) { return rows <= 8 ? 1 : (rows <= 16 ? 2 : 4); }
+
+// Plan of a k_paged_stream launch whose owners have about `rows` query rows
+// per kv head: as few blocks of 8 as hold them, at most 32.
+int stream_plan(const PagedView &pv, int dtype, int d, int G, int64_t rows, int64_t off, cbq_host::LinePlan *p) {
     int rc = CBQ_OK;
 #define CBQ_CALL(T, DD, NN) rc = stream_grid<T, DD, NN>(p)
-    CBQ_STREAM_DISPATCH(dtype, d, nb, CBQ_CALL)
+    CBQ_STREAM_DISPATCH(dtype, d, row_blocks(rows), CBQ_CALL)
 #undef CBQ_CALL
     if (rc != CBQ_OK) return rc;
-    p->owners = mode == kPrefix ? pv.groups : pv.seqs;
-    // row tiles of all owners: at most one per R rows and one more per owner
-    const int64_t rows = (int64_t)pv.tokens * G;
-    const int64_t rts = mode == kOwn ? (int64_t)pv.seqs * ((G + p->R - 1) / p->R) : rows / p->R + p->owners;
-    p->units = rts * pv.kv_heads;
-    const int64_t tile = (int64_t)kKeys * p->NW;
-    const int64_t keys = mode == kOwn ? pv.cap : (mode == kPrefix ? pv.pcap : (int64_t)pv.cap + pv.pcap);
-    if (p->units * ((keys + 2 * kKeys) / tile + 1) > 0x7fffffffll) return CBQ_ERR_UNSUPPORTED;   // tiles are counted in 32 bits
-    p->cum_off = off;
-    p->part_off = cbq_host::align_up(off + (p->owners + 1) * 8, 256);
-    p->end = cbq_host::align_up(p->part_off + (p->units + p->grid) * (int64_t)p->slot * 4, 256);
-    return CBQ_OK;
+    p->tile_rows = 0;
+    p->geo.G = G;
+    p->geo.tq = std::max(1, p->rows / G);
+    p->geo.hc = (G + p->rows - 1) / p->rows;
+    p->geo.join = 1;
+    p->min_tiles = 1;
+    return cbq_host::line_room(pv, d, off, p) ? CBQ_OK : CBQ_ERR_UNSUPPORTED;
 }
 
 struct AttnPlan {
     PagedView pv;
     int dtype, d, G;
-    bool extend, prefix;
-    StreamPlan own, pre;
+    bool extend, prefix, own_tile, pre_tile;           // *_tile: the tensor-core kernel takes that line
+    cbq_host::LinePlan own, pre;
     int64_t bytes;
 };
 
 int plan_attn(const cbq_paged_cache *c, const cbq_paged_batch *b, int64_t tokens, int64_t q_heads, bool extend,
               AttnPlan *p) {
+    *p = AttnPlan{};
     const int rc = cbq_host::paged_view(c, b, tokens, q_heads, &p->pv);
     if (rc != CBQ_OK) return rc;
-    p->bytes = 0;
     if (b->seqs == 0 || tokens == 0) return CBQ_OK;
     if (!extend && tokens != b->seqs) return CBQ_ERR_ARG;
     p->dtype = (int)c->dtype;
@@ -881,34 +688,61 @@ int plan_attn(const cbq_paged_cache *c, const cbq_paged_batch *b, int64_t tokens
     p->pv.cap = (int)std::min<int64_t>(p->pv.cap, b->max_kv_len);
     p->pv.pcap = (int)std::min<int64_t>(p->pv.pcap, b->groups ? b->max_prefix_len : 0);
     p->prefix = !extend && b->groups && p->pv.pcap > 0;
-    // rows of an owner: the mean, for extend (units of one size serve all owners)
-    const int64_t mean = extend ? (tokens * p->G + b->seqs - 1) / b->seqs : p->G;
-    int e = plan_stream(p->pv, p->dtype, p->d, p->G, extend ? kFull : kOwn, mean, 0, &p->own);
+    const bool tile = cbq_host::tile_takes(c);
+    // query rows that share a kv head's keys, on the mean of the owners
+    const int64_t own_rows = extend ? (tokens * p->G + b->seqs - 1) / b->seqs : p->G;
+    p->own.mode = extend ? kFull : kOwn;
+    p->own.direct = !p->prefix;
+    p->own_tile = tile && extend && own_rows > 32;
+    int e = p->own_tile ? cbq_host::tile_plan(p->pv, p->d, p->G, kFull, own_rows > 128, 0, &p->own)
+                        : stream_plan(p->pv, p->dtype, p->d, p->G, own_rows, 0, &p->own);
     if (e != CBQ_OK) return e;
     p->bytes = p->own.end;
     if (p->prefix) {
         const int64_t rows = ((int64_t)b->seqs + b->groups - 1) / b->groups * p->G;
-        e = plan_stream(p->pv, p->dtype, p->d, p->G, kPrefix, rows, p->bytes, &p->pre);
+        p->pre.mode = kPrefix;
+        p->pre.direct = 0;
+        p->pre_tile = tile && rows > 32;
+        e = p->pre_tile ? cbq_host::tile_plan(p->pv, p->d, p->G, kPrefix, rows > 128, p->bytes, &p->pre)
+                        : stream_plan(p->pv, p->dtype, p->d, p->G, rows, p->bytes, &p->pre);
         if (e != CBQ_OK) return e;
         p->bytes = p->pre.end;
     }
     return CBQ_OK;
 }
 
-int run_stream(const AttnPlan &p, const StreamPlan &sp, StreamArgs a, int mode, uint8_t *ws, cudaStream_t s) {
-    a.mode = mode;
-    a.owners = sp.owners;
-    a.slots = sp.units + sp.grid;
-    a.cum = reinterpret_cast<uint64_t *>(ws + sp.cum_off);
-    a.part = reinterpret_cast<float *>(ws + sp.part_off);
-#define CBQ_CALL(T, DD, NN) return stream_launch<T, DD, NN>(p.pv, a, sp.grid, s)
-    CBQ_STREAM_DISPATCH(p.dtype, p.d, sp.NB, CBQ_CALL)
+LineArgs line_args(const cbq_host::LinePlan &lp, LineArgs a, uint8_t *ws) {
+    a.geo = lp.geo;
+    a.mode = lp.mode;
+    a.owners = lp.owners;
+    a.slots = lp.slots;
+    a.min_tiles = lp.min_tiles;
+    a.direct = lp.direct;
+    a.cum = reinterpret_cast<uint64_t *>(ws + lp.cum_off);
+    a.part = reinterpret_cast<float *>(ws + lp.part_off);
+    return a;
+}
+
+int run_line(const cbq_paged_cache *c, const AttnPlan &p, const cbq_host::LinePlan &lp, bool tile, const LineArgs &a,
+             cudaStream_t s) {
+    if (tile) return cbq_host::tile_launch(c, p.pv, lp, a, s);
+#define CBQ_CALL(T, DD, NN) return stream_launch<T, DD, NN>(p.pv, a, lp.grid, s)
+    CBQ_STREAM_DISPATCH(p.dtype, p.d, lp.rows / 8, CBQ_CALL)
 #undef CBQ_CALL
 }
 
-template <typename T, int D> int join_launch(const PagedView &pv, const JoinArgs &j, cudaStream_t s) {
-    const int64_t blocks = ((int64_t)pv.tokens * j.hq + 3) / 4;
-    CBQ_CUDA_TRY(cbq_host::launch_pdl(k_paged_join<T, D>, dim3((unsigned)blocks), dim3(128), 0, s, pv, j));
+template <typename T, int D>
+int join_launch(const AttnPlan &p, const LineArgs &own, const JoinSource &so, const JoinSource &sp, cudaStream_t s) {
+    if (p.prefix) {
+        const int64_t blocks = ((int64_t)p.pv.tokens * own.hq + 3) / 4;
+        CBQ_CUDA_TRY(cbq_host::launch_pdl(k_join_rows<T, D>, dim3((unsigned)blocks), dim3(128), 0, s, p.pv, so, sp,
+                                          own.hq, own.out));
+    } else if (p.own.grid > 1) {
+        const int rows = p.own.geo.hc > 1 ? p.own.rows : p.own.geo.tq * p.G;
+        CBQ_CUDA_TRY(cbq_host::launch_pdl(k_join_cut<T, D>,
+                                          dim3((unsigned)(p.own.grid - 1), (unsigned)((rows + kCutRows - 1) / kCutRows)),
+                                          dim3(128), 0, s, p.pv, own, so));
+    }
     return CBQ_OK;
 }
 
@@ -925,40 +759,62 @@ int paged_attn(const cbq_paged_cache *c, const cbq_paged_batch *b, int64_t token
         (reinterpret_cast<uintptr_t>(ws) & 255))
         return CBQ_ERR_ARG;
     uint8_t *w = static_cast<uint8_t *>(ws);
-    StreamArgs a{};
+    LineArgs a{};
     a.q = q;
     a.qs = q_stride;
     a.hq = (int)q_heads;
-    a.G = p.G;
     a.sc = scale * kLog2e;
     a.out = out;
     a.wait_first = 1;
+    auto source = [&](const cbq_host::LinePlan &lp) {
+        return JoinSource{reinterpret_cast<const float *>(w + lp.part_off),
+                          reinterpret_cast<const uint64_t *>(w + lp.cum_off), lp.slots, lp.owners, lp.grid, lp.min_tiles,
+                          lp.rows, lp.tile_rows, lp.mode, lp.direct, lp.geo};
+    };
+    JoinSource so = source(p.own), sp{};
     if (p.prefix) {
-        if ((rc = run_stream(p, p.pre, a, kPrefix, w, s)) != CBQ_OK) return rc;
+        sp = source(p.pre);
+        if ((rc = run_line(c, p, p.pre, p.pre_tile, line_args(p.pre, a, w), s)) != CBQ_OK) return rc;
         a.wait_first = 0;                              // the prefix launch passed its wait before this one can start
     }
-    a.direct = !p.prefix;
-    if ((rc = run_stream(p, p.own, a, extend ? kFull : kOwn, w, s)) != CBQ_OK) return rc;
-    JoinArgs j{};
-    auto source = [&](const StreamPlan &sp) {
-        return JoinSource{reinterpret_cast<const float *>(w + sp.part_off), reinterpret_cast<const uint64_t *>(w + sp.cum_off),
-                          sp.units + sp.grid, sp.owners, sp.grid, sp.R};
-    };
-    j.own = source(p.own);
-    if (p.prefix) j.pre = source(p.pre);
-    j.hq = (int)q_heads;
-    j.G = p.G;
-    j.full = extend;
-    j.out = out;
+    const LineArgs own = line_args(p.own, a, w);
+    if ((rc = run_line(c, p, p.own, p.own_tile, own, s)) != CBQ_OK) return rc;
     if (p.dtype == CBQ_F32)
-        return p.d == 64 ? join_launch<float, 64>(p.pv, j, s)
-                         : (p.d == 128 ? join_launch<float, 128>(p.pv, j, s) : join_launch<float, 256>(p.pv, j, s));
-    return p.d == 64 ? join_launch<__nv_bfloat16, 64>(p.pv, j, s)
-                     : (p.d == 128 ? join_launch<__nv_bfloat16, 128>(p.pv, j, s)
-                                   : join_launch<__nv_bfloat16, 256>(p.pv, j, s));
+        return p.d == 64 ? join_launch<float, 64>(p, own, so, sp, s)
+                         : (p.d == 128 ? join_launch<float, 128>(p, own, so, sp, s)
+                                       : join_launch<float, 256>(p, own, so, sp, s));
+    return p.d == 64 ? join_launch<__nv_bfloat16, 64>(p, own, so, sp, s)
+                     : (p.d == 128 ? join_launch<__nv_bfloat16, 128>(p, own, so, sp, s)
+                                   : join_launch<__nv_bfloat16, 256>(p, own, so, sp, s));
 }
 
 }  // namespace
+
+namespace cbq_host {
+
+int resident_ctas(const void *kern, int threads, int smem, int *out) {
+    static std::mutex mu;
+    struct Entry { const void *kern; int dev, n; };
+    static Entry seen[256];
+    static int nseen = 0;
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return CBQ_ERR_CUDA;
+    std::lock_guard<std::mutex> g(mu);
+    for (int i = 0; i < nseen; ++i)
+        if (seen[i].kern == kern && seen[i].dev == dev) {
+            *out = seen[i].n;
+            return CBQ_OK;
+        }
+    CBQ_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    int n = 0;
+    CBQ_CUDA_TRY(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kern, threads, smem));
+    if (n < 1) return CBQ_ERR_UNSUPPORTED;
+    if (nseen < 256) seen[nseen++] = Entry{kern, dev, n};
+    *out = n;
+    return CBQ_OK;
+}
+
+}  // namespace cbq_host
 
 extern "C" int64_t cbq_paged_attn_workspace_bytes(const cbq_paged_cache *cache, const cbq_paged_batch *batch,
                                                   int64_t tokens, int64_t q_heads, int extend) {

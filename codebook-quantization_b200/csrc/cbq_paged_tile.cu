@@ -1,0 +1,559 @@
+// cbq_paged_tile.cu -- paged attention for many query rows per kv head on the
+// 5th-generation tensor cores (sm_100a: tcgen05.mma, TMEM, TMA): prompts
+// (extend), and the shared prefix of a group of sequences (decode).
+//
+// A unit's query rows (whole tokens, the G heads of a kv head side by side) lie
+// in NQ blocks of 128.  Per key tile of 128 keys and row block:
+//   S = Q K^T          tcgen05.mma, Q and K in shared memory, S fp32 in TMEM
+//   P = 2^(sc S - m)   one thread per row, S from TMEM, P (bf16) over S's columns
+//   O += P V           tcgen05.mma with P from TMEM, O fp32 in TMEM
+// The running maximum m of a row is only moved when a tile exceeds it by more
+// than 2^kGrow: until then the weights are taken relative to the old one (they
+// stay below 2^kGrow, and sums and O are fp32), so O is rescaled in TMEM a few
+// times per unit instead of once per tile.  The result does not depend on m
+// beyond rounding: o = (sum 2^(x - m) v) / (sum 2^(x - m)).
+//
+// Warp roles: NQ softmax warpgroups (one row block each), a TMA warp (one
+// cp.async.bulk.tensor per page, or part of one, and 64 dimensions; K and V
+// tiles alternate in a ring of 128-key slots), an MMA warp.  With NQ = 2 the
+// MMA warp's order is P0 V, Q0 K', P1 V, Q1 K': each softmax works while the
+// tensor core does the other row block's products.
+// Work is the tile line of cbq_paged_line.cuh, one persistent CTA per part.
+// Every mbarrier wait is bounded; a wait that gives up sets CBQ_FLAG_TIMEOUT,
+// all roles stop at their next wait, and TMEM is released on the way out.
+#include <cuda.h>
+
+#include <mutex>
+
+#include "cbq_paged_line.cuh"
+
+namespace {
+
+using namespace cbq;
+
+constexpr int kBlk = 128;              // rows of a block, keys of a tile
+constexpr float kGrow = 8.f;           // log2 growth of a row's maximum that moves its reference
+
+template <int D, int NQ> struct TileCfg {
+    static constexpr int kHalves = D / 64;                             // 128-byte wide column blocks
+    static constexpr int kHalfB = kBlk * 128;                           // one of them: 16 KB
+    static constexpr int kTileB = kHalves * kHalfB;
+    static constexpr int kSlots = NQ == 2 ? (D == 128 ? 5 : 8) : (D == 128 ? 2 : 4);   // K / V tiles in flight
+    static constexpr int kSoft = NQ * 128;
+    static constexpr int kThreads = kSoft + 64;
+    static constexpr int kCtas = NQ == 2 ? 1 : 2;                       // per SM: TMEM has 512 columns
+    static constexpr int kCols = NQ == 2 ? 512 : 256;
+    static constexpr int kSmem = 1024 + (NQ + kSlots) * kTileB + 512;
+    static __host__ __device__ constexpr uint32_t sCol(int b) { return (uint32_t)b * 128u; }
+    static __host__ __device__ constexpr uint32_t oCol(int b) { return (uint32_t)NQ * 128u + (uint32_t)b * 128u; }
+};
+
+struct Bars {
+    uint64_t q_full[2], s_full[2], p_full[2], o_full[2];
+    uint64_t kv_full[8], kv_empty[8];
+    uint64_t drain;
+    uint32_t tmem;
+    int abort_flag;
+};
+static_assert(sizeof(Bars) <= 512, "barriers outgrow their region");
+
+// ---------------------------------------------------------------- PTX helpers
+__device__ __forceinline__ uint64_t desc_k(uint32_t addr) {
+    // K-major operand, 128-byte swizzle: rows of 128 bytes, 8-row groups 1024 bytes apart
+    return (uint64_t)((addr >> 4) & 0x3FFFu) | ((uint64_t)1 << 16) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) |
+           ((uint64_t)2 << 61);
+}
+__device__ __forceinline__ uint64_t desc_mn(uint32_t addr, uint32_t block_bytes) {
+    // MN-major operand (rows are K), 128-byte swizzle: 64-wide column blocks block_bytes apart, 8-row groups 1024 bytes apart
+    return (uint64_t)((addr >> 4) & 0x3FFFu) | ((uint64_t)(block_bytes >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
+           ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+// kind::f16: D fp32, A and B bf16, A K-major, B K-major or (bt) MN-major.
+__host__ __device__ constexpr uint32_t idesc(int M, int N, int bt) {
+    return (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)bt << 16) | ((uint32_t)(N >> 3) << 17) |
+           ((uint32_t)(M >> 4) << 24);
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t acc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(id), "r"(acc));
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t id, uint32_t acc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(id), "r"(acc));
+}
+__device__ __forceinline__ void mma_commit(uint64_t *bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
+                 : "memory");
+}
+__device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tma_4d(uint32_t dst, const CUtensorMap *map, int c0, int c1, int c2, int c3, uint64_t *bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
+        ::"r"(dst), "l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(smem_u32(bar)) : "memory");
+}
+// 32 columns of this thread's TMEM lane, without waiting for them.
+__device__ __forceinline__ void tld32(uint32_t a, uint32_t *v) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
+          "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(v[16]),
+          "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]),
+          "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+        : "r"(a));
+}
+__device__ __forceinline__ void tld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tst16(uint32_t a, const uint32_t *v) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(a),
+        "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
+        "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]) : "memory");
+}
+__device__ __forceinline__ void tst32(uint32_t a, const uint32_t *v) {
+    tst16(a, v);
+    tst16(a + 16, v + 16);
+}
+__device__ __forceinline__ void tst_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// Bounded wait of a whole warp; false (for all its lanes) once the CTA has given up.
+__device__ __forceinline__ bool warp_wait(uint64_t *bar, uint32_t parity, Bars *b, uint32_t *status) {
+    bool ok = !*(volatile int *)&b->abort_flag && mbar_wait_bounded(bar, parity);
+    ok = __all_sync(0xffffffffu, ok);
+    if (!ok && (threadIdx.x & 31) == 0 && !*(volatile int *)&b->abort_flag) {
+        *(volatile int *)&b->abort_flag = 1;
+        report(status, CBQ_FLAG_TIMEOUT, 0u);
+    }
+    return ok;
+}
+
+// A key tile: 128 rows of the prefix or of the own rows from row key0 of it.
+struct TileAt {
+    bool pre;
+    int key0, have;                    // rows of the tile that exist (0..128)
+};
+__device__ __forceinline__ TileAt tile_at(const Owner &w, int t) {
+    const int np = (w.plen + kBlk - 1) / kBlk;
+    TileAt x;
+    x.pre = t < np;
+    x.key0 = (x.pre ? t : t - np) * kBlk;
+    x.have = clampi((x.pre ? w.plen : w.olen) - x.key0, 0, kBlk);
+    return x;
+}
+
+template <int D, int NQ>
+__global__ void __launch_bounds__(TileCfg<D, NQ>::kThreads, TileCfg<D, NQ>::kCtas)
+    k_paged_tile(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const PagedView pv,
+                 const LineArgs a) {
+    using Cfg = TileCfg<D, NQ>;
+    constexpr int kSlots = Cfg::kSlots, kTileB = Cfg::kTileB, kHalfB = Cfg::kHalfB;
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+    uint8_t *sQ = smem, *sKV = smem + NQ * kTileB;
+    Bars *bars = reinterpret_cast<Bars *>(sKV + kSlots * kTileB);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    constexpr int kTmaWarp = Cfg::kSoft / 32, kMmaWarp = kTmaWarp + 1;
+
+    if (tid == 0) {
+        for (int q = 0; q < NQ; ++q) {
+            mbar_init(&bars->q_full[q], 128);
+            mbar_init(&bars->s_full[q], 1);
+            mbar_init(&bars->p_full[q], 128);
+            mbar_init(&bars->o_full[q], 1);
+        }
+        for (int s = 0; s < kSlots; ++s) {
+            mbar_init(&bars->kv_full[s], 1);
+            mbar_init(&bars->kv_empty[s], 1);
+        }
+        mbar_init(&bars->drain, 1);
+        bars->abort_flag = 0;
+        mbar_fence_init();
+    }
+    if (warp == kMmaWarp) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&bars->tmem)),
+                     "r"(Cfg::kCols) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    if (a.wait_first) pdl_wait();
+    pdl_launch_dependents();
+    tc_before();
+    __syncthreads();
+    tc_after();
+    const uint32_t tmem = bars->tmem;
+    Cursor c{};
+    uint32_t w1 = 0;
+    const bool any = plan_line<Cfg::kThreads>(pv, a, c, w1);
+
+    const int tb = kBlk / a.geo.G;                     // tokens of a row block
+    Piece p{};
+    if (!any) {
+        // nothing of the line for this CTA
+    } else if (warp < kTmaWarp) {
+        // ------------------------------------------- softmax and output: thread = row
+        const int q = warp >> 2, r = tid & 127;
+        const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+        const uint32_t tS = lanes + Cfg::sCol(q), tO = lanes + Cfg::oCol(q);
+        const int rt = r / a.geo.G, rg = r - rt * a.geo.G;            // the row's token in the block, head in the group
+        // a negative scale turns Q's sign at its load, zero its value: sc > 0 below
+        const float sc = a.sc == 0.f ? 1.f : fabsf(a.sc);
+        const uint32_t sign = a.sc < 0.f ? 0x80008000u : 0u, keep = a.sc == 0.f ? 0u : 0xffffffffu;
+        // the block's rows of the unit at cursor c into shared memory (128-byte swizzle)
+        auto load_q = [&]() {
+            uint8_t *dst = sQ + q * kTileB;
+            const int tok0 = p.tt * a.geo.tq + q * tb, left = min(tb, c.ow.nt - tok0);
+            constexpr int CH = D / 8;
+#pragma unroll 4
+            for (int e = r; e < kBlk * CH; e += 128) {
+                const int row = e / CH, ch = e - row * CH, tk = row / a.geo.G;
+                uint4 v = make_uint4(0u, 0u, 0u, 0u);
+                if (tk < left) {
+                    const __nv_bfloat16 *src = static_cast<const __nv_bfloat16 *>(a.q) + (int64_t)(c.ow.t0 + tok0 + tk) * a.qs +
+                                               (int64_t)(p.h * a.geo.G + row - tk * a.geo.G) * D + ch * 8;
+                    v = *reinterpret_cast<const uint4 *>(src);
+                    v.x = (v.x ^ sign) & keep;
+                    v.y = (v.y ^ sign) & keep;
+                    v.z = (v.z ^ sign) & keep;
+                    v.w = (v.w ^ sign) & keep;
+                }
+                *reinterpret_cast<uint4 *>(dst + (ch >> 3) * kHalfB + row * 128 + (((ch & 7) ^ (row & 7)) << 4)) = v;
+            }
+            fence_proxy_async_smem();
+            mbar_arrive(&bars->q_full[q]);
+        };
+        bool go = next_piece(c, pv, a, w1, p);
+        if (go) load_q();
+        uint32_t ns = 0;                               // tiles seen (phases of s_full and o_full)
+        while (go) {
+            const int tok = p.tt * a.geo.tq + q * tb + rt;
+            const bool live = rt < tb && tok < c.ow.nt;
+            const int olim = a.mode == kPrefix ? 0 : own_limit(c.ow, tok);
+            // the piece's place and output, before the cursor moves on
+            const bool whole = a.direct && p.tb == 0 && p.te == p.tiles;
+            const int64_t slot = slot_of(c, p, a, (int)blockIdx.x);
+            const int64_t orow = (int64_t)(c.ow.t0 + tok) * a.hq + p.h * a.geo.G + rg;
+            float m = -INFINITY, l = 0.f;
+            const int t0 = p.tb, t1 = p.te;
+            for (int t = t0; t < t1; ++t, ++ns) {
+                if (!warp_wait(&bars->s_full[q], ns & 1, bars, pv.status)) { go = false; break; }
+                tc_after();
+                uint32_t s[128];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) tld32(tS + i * 32, s + i * 32);
+                tld_wait();
+                const TileAt x = tile_at(c.ow, t);
+                const int vis = x.pre ? x.have : min(x.have, olim - x.key0);   // visible keys of the tile
+                if (__any_sync(0xffffffffu, vis < kBlk)) {
+#pragma unroll
+                    for (int j = 0; j < 128; ++j)
+                        if (j >= vis) s[j] = 0xff800000u;                      // -inf
+                }
+                float mx[4] = {__uint_as_float(s[0]), __uint_as_float(s[1]), __uint_as_float(s[2]), __uint_as_float(s[3])};
+#pragma unroll
+                for (int j = 4; j < 128; j += 4)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) mx[e] = fmaxf(mx[e], __uint_as_float(s[j + e]));
+                const float mn = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+                const bool grow = (mn - m) * sc > kGrow;                       // false where both are -inf
+                if (__any_sync(0xffffffffu, grow)) {
+                    const float f = grow ? ex2((m - mn) * sc) : 1.f;           // 0 from -inf
+                    if (grow) m = mn;
+                    l *= f;
+                    if (t > t0) {
+                        // O holds the tiles before: wait for the last of them, scale it
+                        if (!warp_wait(&bars->o_full[q], (ns - 1) & 1, bars, pv.status)) { go = false; break; }
+                        tc_after();
+#pragma unroll 1
+                        for (int i = 0; i < D; i += 32) {
+                            uint32_t o[32];
+                            tld32(tO + i, o);
+                            tld_wait();
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
+                            tst32(tO + i, o);
+                        }
+                    }
+                }
+                const float mb = m == -INFINITY ? 0.f : m * sc;
+                float ls[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    uint32_t pk[16];
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) {
+                        const float p0 = ex2(fmaf(__uint_as_float(s[i * 32 + 2 * j]), sc, -mb));
+                        const float p1 = ex2(fmaf(__uint_as_float(s[i * 32 + 2 * j + 1]), sc, -mb));
+                        ls[(2 * j) & 3] += p0;
+                        ls[(2 * j + 1) & 3] += p1;
+                        pk[j] = pack_bf16(p0, p1);
+                    }
+                    tst16(tS + i * 16, pk);
+                }
+                l += (ls[0] + ls[1]) + (ls[2] + ls[3]);
+                tst_wait();
+                tc_before();
+                mbar_arrive(&bars->p_full[q]);
+            }
+            if (!go) break;
+            // the last S has been read, so every product with this Q is done
+            const bool more = next_piece(c, pv, a, w1, p);
+            if (more) load_q();
+            if (!warp_wait(&bars->o_full[q], (ns - 1) & 1, bars, pv.status)) { go = false; break; }
+            tc_after();
+            const float inv = l == 0.f ? 0.f : 1.f / l;
+            float *ps = a.part + slot * (int64_t)(NQ * kBlk * (D + 2));
+            const bool fits = slot < a.slots;
+#pragma unroll 1
+            for (int i = 0; i < D; i += 32) {
+                uint32_t o[32];
+                tld32(tO + i, o);
+                tld_wait();
+                if (!live) {
+                } else if (whole) {
+                    __nv_bfloat16 *dst = static_cast<__nv_bfloat16 *>(a.out) + orow * D + i;
+#pragma unroll
+                    for (int j = 0; j < 32; j += 8) {
+                        uint32_t w[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            w[e] = pack_bf16(__uint_as_float(o[j + 2 * e]) * inv, __uint_as_float(o[j + 2 * e + 1]) * inv);
+                        *reinterpret_cast<uint4 *>(dst + j) = make_uint4(w[0], w[1], w[2], w[3]);
+                    }
+                } else if (fits) {
+                    float *dst = ps + (int64_t)(q * kBlk + r) * D + i;
+#pragma unroll
+                    for (int j = 0; j < 32; j += 4)
+                        *reinterpret_cast<uint4 *>(dst + j) = make_uint4(o[j], o[j + 1], o[j + 2], o[j + 3]);
+                }
+                __syncwarp();                          // the next TMEM load is the whole warp's
+            }
+            if (live && !whole && fits) {
+                // joined with parts of either kernel: the maximum in units of log2
+                ps[NQ * kBlk * D + q * kBlk + r] = m == -INFINITY ? m : m * sc;
+                ps[NQ * kBlk * D + NQ * kBlk + q * kBlk + r] = l;
+            }
+            __syncwarp();
+            tc_before();                               // O's reads before the next unit's first product
+            go = more;
+        }
+    } else if (warp == kTmaWarp) {
+        // ------------------------------------------------------------- K and V tiles
+        uint32_t n = 0;                                // tiles issued (K and V)
+        bool go = true;
+        const int ps = 1 << pv.ps_shift, box = min(ps, kBlk);
+        while (go && next_piece(c, pv, a, w1, p)) {
+            for (int t = p.tb; t < p.te && go; ++t) {
+                const TileAt x = tile_at(c.ow, t);
+                const int nbox = (x.have + box - 1) / box;
+                // lane: one box of rows and 64 dimensions
+                const int bx = lane / Cfg::kHalves, hf = lane - bx * Cfg::kHalves;
+                const int key = x.key0 + bx * box;
+                int page = 0;
+                if (bx < nbox) {
+                    const int32_t *tab = x.pre ? pv.ptable + c.ow.group * pv.ptable_stride : pv.table + c.o * pv.table_stride;
+                    page = __ldg(tab + (key >> pv.ps_shift));
+                    if (page < 0 || page >= pv.pages) {
+                        if (hf == 0) report(pv.status, CBQ_FLAG_CORRUPT, (uint32_t)c.o);
+                        page = pv.pages;               // outside the map: the copy fills with zeros
+                    }
+                }
+#pragma unroll
+                for (int kv = 0; kv < 2; ++kv, ++n) {
+                    const int s = n % kSlots;
+                    if (n >= kSlots && !warp_wait(&bars->kv_empty[s], (n / kSlots - 1) & 1, bars, pv.status)) {
+                        go = false;
+                        break;
+                    }
+                    if (lane == 0) mbar_arrive_expect_tx(&bars->kv_full[s], (uint32_t)(nbox * box * D * 2));
+                    __syncwarp();
+                    if (bx < nbox)
+                        tma_4d(smem_u32(sKV + s * kTileB + hf * kHalfB + bx * box * 128), kv ? &vmap : &kmap, hf * 64,
+                               key & (ps - 1), p.h, page, &bars->kv_full[s]);
+                }
+            }
+        }
+        // no copy may still be landing when the CTA ends
+        for (uint32_t s = 0; s < kSlots && s < n; ++s) {
+            const uint32_t last = n - 1 - (n - 1 - s) % kSlots;
+            mbar_wait_bounded(&bars->kv_full[s], (last / kSlots) & 1);
+        }
+    } else {
+        // ------------------------------------------------------------------ products
+        constexpr uint32_t idS = idesc(128, 128, 0), idO = idesc(128, D, 1);
+        uint32_t n = 0, np = 0, nq = 0;                // ring tiles used, p_full phases, pieces
+        bool go = true;
+        auto slot = [&](uint32_t i) { return smem_u32(sKV + (i % kSlots) * kTileB); };
+        auto wait_kv = [&](uint32_t i) {
+            return warp_wait(&bars->kv_full[i % kSlots], (i / kSlots) & 1, bars, pv.status);
+        };
+        auto scores = [&](int q, uint32_t ik) {
+            if (lane == 0) {
+                const uint32_t qa = smem_u32(sQ + q * kTileB), ka = slot(ik);
+#pragma unroll
+                for (int kk = 0; kk < D / 16; ++kk) {
+                    const uint32_t off = (kk >> 2) * kHalfB + (kk & 3) * 32;
+                    mma_ss(tmem + Cfg::sCol(q), desc_k(qa + off), desc_k(ka + off), idS, kk > 0);
+                }
+                mma_commit(&bars->s_full[q]);
+            }
+            __syncwarp();
+        };
+        auto values = [&](int q, uint32_t iv, bool first) {
+            if (lane == 0) {
+                const uint32_t va = slot(iv);
+#pragma unroll
+                for (int kk = 0; kk < kBlk / 16; ++kk)
+                    mma_ts(tmem + Cfg::oCol(q), tmem + Cfg::sCol(q) + kk * 8, desc_mn(va + kk * 2048, kHalfB), idO,
+                           !first || kk > 0);
+                mma_commit(&bars->o_full[q]);
+            }
+            __syncwarp();
+        };
+        auto release = [&](uint32_t i) {
+            if (lane == 0) mma_commit(&bars->kv_empty[i % kSlots]);
+            __syncwarp();
+        };
+        while (go && next_piece(c, pv, a, w1, p)) {
+            // ring: K of tile t at n + 2 t, V at n + 2 t + 1
+            const int nt = p.te - p.tb;
+            go = wait_kv(n);
+            for (int q = 0; q < NQ && go; ++q) {
+                go = warp_wait(&bars->q_full[q], nq & 1, bars, pv.status);
+                tc_after();
+                if (go) scores(q, n);
+            }
+            if (!go) break;
+            release(n);
+            for (int t = 0; t < nt; ++t, ++np) {
+                const uint32_t iv = n + 2 * t + 1;
+                if (!(go = wait_kv(iv))) break;
+                const TileAt x = tile_at(c.ow, p.tb + t);
+                if (x.have < kBlk) {
+                    // rows that do not exist (rest of a page, pages not copied) must not meet a weight of 0
+                    for (int e = x.have * 8 + lane; e < kBlk * 8; e += 32)
+#pragma unroll
+                        for (int hf = 0; hf < Cfg::kHalves; ++hf)
+                            *reinterpret_cast<uint4 *>(sKV + (iv % kSlots) * kTileB + hf * kHalfB + e * 16) =
+                                make_uint4(0u, 0u, 0u, 0u);
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                }
+                const bool next = t + 1 < nt;
+                for (int q = 0; q < NQ; ++q) {
+                    if (!(go = warp_wait(&bars->p_full[q], np & 1, bars, pv.status))) break;
+                    tc_after();
+                    values(q, iv, t == 0);
+                    if (next) {
+                        if (q == 0 && !(go = wait_kv(iv + 1))) break;
+                        scores(q, iv + 1);
+                    }
+                }
+                if (!go) break;
+                release(iv);
+                if (next) release(iv + 1);
+            }
+            n += 2 * nt;
+            ++nq;
+        }
+        if (!go) {                                     // gave up: products in flight end first
+            if (lane == 0) mma_commit(&bars->drain);
+            __syncwarp();
+            mbar_wait_bounded(&bars->drain, 0);
+        }
+    }
+    tc_before();
+    __syncthreads();
+    if (warp == kMmaWarp) {
+        tc_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(Cfg::kCols) : "memory");
+    }
+    if (!a.wait_first) pdl_wait();
+}
+
+// ---------------------------------------------------------------- host side
+using EncodeFn = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *,
+                              const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle,
+                              CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeFn encoder() {
+    static EncodeFn fn = [] {
+        void *f = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) != cudaSuccess ||
+            q != cudaDriverEntryPointSuccess)
+            return (EncodeFn) nullptr;
+        return reinterpret_cast<EncodeFn>(f);
+    }();
+    return fn;
+}
+
+// The pool as {dimension, row, head, page}; a box is a page's rows (at most 128) by 64 dimensions.
+bool pool_map(const cbq_paged_cache *c, void *pool, CUtensorMap *map) {
+    EncodeFn enc = encoder();
+    if (!enc) return false;
+    const cuuint64_t dims[4] = {(cuuint64_t)c->head_dim, (cuuint64_t)c->page_size, (cuuint64_t)c->kv_heads,
+                                (cuuint64_t)c->pages};
+    const cuuint64_t strides[3] = {(cuuint64_t)c->row_stride * 2, (cuuint64_t)c->head_stride * 2,
+                                   (cuuint64_t)c->page_stride * 2};
+    const cuuint32_t box[4] = {64, (cuuint32_t)std::min<int64_t>(c->page_size, kBlk), 1, 1}, es[4] = {1, 1, 1, 1};
+    return enc(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, pool, dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) ==
+           CUDA_SUCCESS;
+}
+
+template <int D, int NQ> int grid_of(int *ctas) {
+    using Cfg = TileCfg<D, NQ>;
+    return cbq_host::resident_ctas(reinterpret_cast<const void *>(k_paged_tile<D, NQ>), Cfg::kThreads, Cfg::kSmem, ctas);
+}
+
+template <int D, int NQ>
+int launch_tile(const CUtensorMap &km, const CUtensorMap &vm, const PagedView &pv, const LineArgs &a, int grid,
+                cudaStream_t s) {
+    using Cfg = TileCfg<D, NQ>;
+    CBQ_CUDA_TRY(cbq_host::launch_pdl(k_paged_tile<D, NQ>, dim3((unsigned)grid), dim3(Cfg::kThreads), (size_t)Cfg::kSmem, s,
+                                      km, vm, pv, a));
+    return CBQ_OK;
+}
+
+}  // namespace
+
+namespace cbq_host {
+
+bool tile_takes(const cbq_paged_cache *c) {
+    // strides that a tensor map holds: positive, below 2^40 bytes
+    const int64_t top = (int64_t)1 << 39;
+    return c->dtype == CBQ_BF16 && (c->head_dim == 64 || c->head_dim == 128) && c->pages > 0 && c->row_stride > 0 &&
+           c->head_stride > 0 && c->page_stride > 0 && c->row_stride < top && c->head_stride < top && c->page_stride < top &&
+           encoder() != nullptr;
+}
+
+int tile_plan(const cbq::PagedView &pv, int d, int G, int mode, bool two, int64_t off, LinePlan *p) {
+    int n = 0;
+    const int rc = d == 64 ? (two ? grid_of<64, 2>(&n) : grid_of<64, 1>(&n))
+                           : (two ? grid_of<128, 2>(&n) : grid_of<128, 1>(&n));
+    if (rc != CBQ_OK) return rc;
+    const int nq = two ? 2 : 1;
+    p->mode = mode;
+    p->rows = nq * kBlk;
+    p->tile_rows = kBlk;
+    p->geo.G = G;
+    p->geo.tq = nq * (kBlk / G);
+    p->geo.hc = 1;
+    p->geo.keys = kBlk;
+    p->geo.join = 0;
+    p->min_tiles = 2;
+    p->grid = n * sm_count();
+    return line_room(pv, d, off, p) ? CBQ_OK : CBQ_ERR_UNSUPPORTED;
+}
+
+int tile_launch(const cbq_paged_cache *c, const cbq::PagedView &pv, const LinePlan &p, cbq::LineArgs a, cudaStream_t s) {
+    CUtensorMap km, vm;
+    if (!pool_map(c, c->k_dev, &km) || !pool_map(c, c->v_dev, &vm)) return CBQ_ERR_UNSUPPORTED;
+    const bool two = p.rows > kBlk;
+    if (c->head_dim == 64)
+        return two ? launch_tile<64, 2>(km, vm, pv, a, p.grid, s) : launch_tile<64, 1>(km, vm, pv, a, p.grid, s);
+    return two ? launch_tile<128, 2>(km, vm, pv, a, p.grid, s) : launch_tile<128, 1>(km, vm, pv, a, p.grid, s);
+}
+
+}  // namespace cbq_host
