@@ -28,18 +28,17 @@ struct AppendArgs {
 template <typename T> struct Vec16;    // 16 bytes of T as floats
 template <> struct Vec16<float> {
     static constexpr int N = 4;
-    static __device__ __forceinline__ void ld(const float *p, float (&x)[4]) {
-        const float4 v = *reinterpret_cast<const float4 *>(p);
-        x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
+    static __device__ __forceinline__ void get(const uint4 &v, float (&x)[4]) {
+        x[0] = __uint_as_float(v.x); x[1] = __uint_as_float(v.y);
+        x[2] = __uint_as_float(v.z); x[3] = __uint_as_float(v.w);
     }
-    static __device__ __forceinline__ void st(float *p, const float (&x)[4]) {
-        *reinterpret_cast<float4 *>(p) = make_float4(x[0], x[1], x[2], x[3]);
+    static __device__ __forceinline__ uint4 put(const float (&x)[4]) {
+        return make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3]));
     }
 };
 template <> struct Vec16<__nv_bfloat16> {
     static constexpr int N = 8;
-    static __device__ __forceinline__ void ld(const __nv_bfloat16 *p, float (&x)[8]) {
-        const uint4 v = *reinterpret_cast<const uint4 *>(p);
+    static __device__ __forceinline__ void get(const uint4 &v, float (&x)[8]) {
         const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -47,27 +46,49 @@ template <> struct Vec16<__nv_bfloat16> {
             x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
         }
     }
-    static __device__ __forceinline__ void st(__nv_bfloat16 *p, const float (&x)[8]) {
+    static __device__ __forceinline__ uint4 put(const float (&x)[8]) {
         uint32_t w[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const __nv_bfloat162 b = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
             w[i] = *reinterpret_cast<const uint32_t *>(&b);
         }
-        *reinterpret_cast<uint4 *>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+        return make_uint4(w[0], w[1], w[2], w[3]);
     }
 };
 
 // One CTA per token.  LPH = D / (2 N) neighbouring lanes hold a head: lane l
 // the elements [l N, l N + N) of each half, so a rotation pair sits in one
 // lane, loads and stores are 16 bytes, and the sum of squares is a shuffle
-// over LPH lanes.
+// over LPH lanes.  A thread takes kHeads heads at a time: their loads go out
+// before the chain of small loads that finds the token's row and table entries,
+// and the cos / sin values serve all of them.
+constexpr int kThreads = 128;
+constexpr int kHeads = 3;
+
 template <typename T, int D>
-__global__ void __launch_bounds__(512) k_paged_append(const PagedView pv, const AppendArgs a) {
-    constexpr int N = Vec16<T>::N, LPH = D / (2 * N), H = D / 2;
+__global__ void __launch_bounds__(kThreads) k_paged_append(const PagedView pv, const AppendArgs a) {
+    constexpr int N = Vec16<T>::N, LPH = D / (2 * N), H = D / 2, HPP = kThreads / LPH;   // heads per pass
     pdl_launch_dependents();
     pdl_wait();
     const int t = blockIdx.x;
+    const int sub = threadIdx.x % LPH, hd = threadIdx.x / LPH;
+    const int heads = a.hq + 2 * pv.kv_heads;
+    uint4 raw[kHeads][2];
+    auto fetch = [&](int h0) {
+#pragma unroll
+        for (int i = 0; i < kHeads; ++i) {
+            const int h = h0 + i * HPP + hd;
+            if (h >= heads) continue;
+            const T *src = h < a.hq ? static_cast<const T *>(a.q) + t * a.qs + h * D
+                                    : (h < a.hq + pv.kv_heads ? static_cast<const T *>(a.kn) + t * a.ks + (h - a.hq) * D
+                                                              : static_cast<const T *>(a.vn) + t * a.vs +
+                                                                    (h - a.hq - pv.kv_heads) * D);
+            raw[i][0] = __ldcs(reinterpret_cast<const uint4 *>(src + sub * N));
+            raw[i][1] = __ldcs(reinterpret_cast<const uint4 *>(src + sub * N + H));
+        }
+    };
+    fetch(0);
     // the token's sequence, row, position and page
     int s = t, row;
     if (pv.cu) {
@@ -76,19 +97,15 @@ __global__ void __launch_bounds__(512) k_paged_append(const PagedView pv, const 
     } else {
         row = pv.lens[s] - 1;
     }
+    int page = -1;
+    bool ok = row >= 0 && row < pv.cap;
+    if (ok) page = pv.table[s * pv.table_stride + (row >> pv.ps_shift)];
     int64_t pos = row;
     if (pv.groups) pos += pv.plens[warp_upper(pv.gs, pv.groups, s)];
-    int page = -1;
-    bool ok = row >= 0 && row < pv.cap && pos >= 0 && pos < a.rope_len;
-    if (ok) {
-        page = pv.table[s * pv.table_stride + (row >> pv.ps_shift)];
-        ok = page >= 0 && page < pv.pages;
-    }
+    ok = ok && pos >= 0 && pos < a.rope_len && page >= 0 && page < pv.pages;
     if (!ok && row >= 0 && threadIdx.x == 0) report(pv.status, CBQ_FLAG_CORRUPT, (uint32_t)t);
     const int line = row & ((1 << pv.ps_shift) - 1);
     const int64_t at = page * pv.page_stride + line * pv.row_stride;
-    const int sub = threadIdx.x % LPH;
-    const int heads = a.hq + 2 * pv.kv_heads;
     float c0[N], c1[N], s0[N], s1[N];
     if (ok) {
         const float *cr = a.cosT + pos * D + sub * N, *sr = a.sinT + pos * D + sub * N;
@@ -103,65 +120,57 @@ __global__ void __launch_bounds__(512) k_paged_append(const PagedView pv, const 
         }
     }
     // every lane of a warp runs every pass, so the shuffles are whole
-    for (int h0 = 0; h0 < heads; h0 += blockDim.x / LPH) {
-        const int h = h0 + threadIdx.x / LPH;
-        const bool live = h < heads;
-        const int kind = h < a.hq ? 0 : (h < a.hq + pv.kv_heads ? 1 : 2);
-        const int hh = kind == 0 ? h : (kind == 1 ? h - a.hq : h - a.hq - pv.kv_heads);
-        float x0[N], x1[N];
-        float ss = 0.f;
-        if (live && ok) {
-            const T *src = kind == 0 ? static_cast<const T *>(a.q) + t * a.qs
-                                     : (kind == 1 ? static_cast<const T *>(a.kn) + t * a.ks
-                                                  : static_cast<const T *>(a.vn) + t * a.vs);
-            src += hh * D + sub * N;
-            Vec16<T>::ld(src, x0);
-            Vec16<T>::ld(src + H, x1);
+    for (int h0 = 0; h0 < heads; h0 += kHeads * HPP) {
+        if (h0) fetch(h0);
 #pragma unroll
-            for (int i = 0; i < N; ++i) ss += x0[i] * x0[i] + x1[i] * x1[i];
-        }
+        for (int i = 0; i < kHeads; ++i) {
+            const int h = h0 + i * HPP + hd;
+            const bool live = h < heads;
+            float x0[N], x1[N];
+            Vec16<T>::get(raw[i][0], x0);
+            Vec16<T>::get(raw[i][1], x1);
+            float ss = 0.f;
 #pragma unroll
-        for (int o = LPH / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-        if (!live) continue;
-        T *dst;
-        if (kind == 0) {
-            dst = static_cast<T *>(a.q_out) + ((int64_t)t * a.hq + hh) * D + sub * N;
+            for (int j = 0; j < N; ++j) ss += x0[j] * x0[j] + x1[j] * x1[j];
+#pragma unroll
+            for (int o = LPH / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+            if (!live) continue;
+            const bool isq = h < a.hq, isv = h >= a.hq + pv.kv_heads;
+            if (!ok && !isq) continue;
+            T *dst = isq ? static_cast<T *>(a.q_out) + ((int64_t)t * a.hq + h) * D
+                         : const_cast<T *>(static_cast<const T *>(isv ? pv.v : pv.k)) + at +
+                               (h - a.hq - (isv ? pv.kv_heads : 0)) * pv.head_stride;
+            uint4 *d0 = reinterpret_cast<uint4 *>(dst + sub * N), *d1 = reinterpret_cast<uint4 *>(dst + sub * N + H);
             if (!ok) {
-#pragma unroll
-                for (int i = 0; i < N; ++i) x0[i] = 0.f;
-                Vec16<T>::st(dst, x0);
-                Vec16<T>::st(dst + H, x0);
+                *d0 = *d1 = make_uint4(0u, 0u, 0u, 0u);
                 continue;
             }
-        } else {
-            if (!ok) continue;
-            dst = const_cast<T *>(static_cast<const T *>(kind == 1 ? pv.k : pv.v)) + at + hh * pv.head_stride + sub * N;
-        }
-        if (kind != 2) {
-            const float scale = a.eps >= 0.f ? rsqrtf(ss / (float)D + a.eps) : 1.f;
-            const float *w = kind == 0 ? a.qw : a.kw;
-#pragma unroll
-            for (int i = 0; i < N; ++i) {
-                float y0 = x0[i] * scale, y1 = x1[i] * scale;
-                if (w && a.eps >= 0.f) {
-                    y0 *= w[sub * N + i];
-                    y1 *= w[H + sub * N + i];
-                }
-                x0[i] = y0 * c0[i] - y1 * s0[i];
-                x1[i] = y1 * c1[i] + y0 * s1[i];
+            if (isv) {
+                *d0 = raw[i][0];
+                *d1 = raw[i][1];
+                continue;
             }
+            const float scale = a.eps >= 0.f ? rsqrtf(ss / (float)D + a.eps) : 1.f;
+            const float *w = a.eps >= 0.f ? (isq ? a.qw : a.kw) : nullptr;
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+                float y0 = x0[j] * scale, y1 = x1[j] * scale;
+                if (w) {
+                    y0 *= w[sub * N + j];
+                    y1 *= w[H + sub * N + j];
+                }
+                x0[j] = y0 * c0[j] - y1 * s0[j];
+                x1[j] = y1 * c1[j] + y0 * s1[j];
+            }
+            *d0 = Vec16<T>::put(x0);
+            *d1 = Vec16<T>::put(x1);
         }
-        Vec16<T>::st(dst, x0);
-        Vec16<T>::st(dst + H, x1);
     }
 }
 
 template <typename T, int D>
 int launch_append(const PagedView &pv, const AppendArgs &a, cudaStream_t s) {
-    constexpr int LPH = D / (2 * Vec16<T>::N);
-    const int lanes = (a.hq + 2 * pv.kv_heads) * LPH;
-    const int threads = std::min(512, (lanes + 31) / 32 * 32);
-    CBQ_CUDA_TRY(cbq_host::launch_pdl(k_paged_append<T, D>, dim3((unsigned)pv.tokens), dim3(threads), 0, s, pv, a));
+    CBQ_CUDA_TRY(cbq_host::launch_pdl(k_paged_append<T, D>, dim3((unsigned)pv.tokens), dim3(kThreads), 0, s, pv, a));
     return CBQ_OK;
 }
 

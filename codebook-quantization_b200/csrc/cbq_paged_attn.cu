@@ -10,9 +10,9 @@
 // k_paged_stream is the kernel for few query rows per kv head: the cache is
 // read once and its bytes bound it.  A CTA whose part of the line (see
 // cbq_paged_line.cuh) holds all of a unit writes the result; other units leave
-// one (m, l, o) per part in the workspace, joined in part order by k_join_cut
-// (whole units written directly) or k_join_rows (every unit has parts: the own
-// rows' and the prefix's).
+// one (m, l, o) per part in the workspace, joined in part order: by the CTA that
+// arrives last at a cut unit, or, where a prefix adds its parts to every unit,
+// by k_join_rows.
 #include <mutex>
 
 #include "cbq_paged_line.cuh"
@@ -97,6 +97,65 @@ __device__ __forceinline__ void load_stage(const PagedView &pv, int page, int ke
     }
 }
 
+// All NT threads of a CTA join the parts of a cut unit of R rows.  Thread t
+// holds D / 4 * R / NT float4 of the result; weights pass through shared
+// memory in blocks of kWB parts.
+constexpr int kWB = 32;
+template <typename T, int D, int R, int NT, typename F>
+__device__ __forceinline__ void join_unit(const LineArgs &a, const Cut &cut, int nrows, float *sm, F dst_row) {
+    constexpr int SL = R * D + 2 * R, V = R * D / 4 / NT, TPR = NT / R;
+    static_assert(V >= 1 && TPR >= 1 && (TPR & (TPR - 1)) == 0 && TPR <= 32, "a row's threads are lanes of one warp");
+    const int tid = threadIdx.x;
+    float *sW = sm, *sI = sm + kWB * R;                // [kWB][R] weights, [R] 1 / l
+    // each row's maximum and sum: TPR lanes over its parts
+    const int row = tid / TPR, sub = tid % TPR;
+    float M = -INFINITY;
+    for (int k = sub; k < cut.n; k += TPR) M = fmaxf(M, __ldcg(cut.slot(a, k, SL) + R * D + row));
+#pragma unroll
+    for (int d = TPR / 2; d > 0; d >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, d));
+    float L = 0.f;
+    float4 y[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) y[v] = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int k0 = 0; k0 < cut.n; k0 += kWB) {
+        const int nk = min(kWB, cut.n - k0);
+        __syncthreads();                               // the weights before
+        for (int k = sub; k < nk; k += TPR) {
+            const float *b = cut.slot(a, k0 + k, SL) + R * D + row;
+            const float m = __ldcg(b), f = m == -INFINITY ? 0.f : ex2(m - M);
+            L = fmaf(__ldcg(b + R), f, L);
+            sW[k * R + row] = f;
+        }
+        __syncthreads();
+#pragma unroll 4
+        for (int k = 0; k < nk; ++k) {
+            const float *b = cut.slot(a, k0 + k, SL);
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                const int e = tid + v * NT, r = e / (D / 4);
+                if (r >= nrows) continue;
+                const float4 x = __ldcg(reinterpret_cast<const float4 *>(b) + e);
+                const float f = sW[k * R + r];
+                y[v].x = fmaf(x.x, f, y[v].x);
+                y[v].y = fmaf(x.y, f, y[v].y);
+                y[v].z = fmaf(x.z, f, y[v].z);
+                y[v].w = fmaf(x.w, f, y[v].w);
+            }
+        }
+    }
+#pragma unroll
+    for (int d = TPR / 2; d > 0; d >>= 1) L += __shfl_xor_sync(0xffffffffu, L, d);
+    if (sub == 0) sI[row] = L == 0.f ? 0.f : 1.f / L;
+    __syncthreads();
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+        const int e = tid + v * NT, r = e / (D / 4);
+        if (r >= nrows) continue;
+        const float inv = sI[r];
+        st4(dst_row(r) + (e - r * (D / 4)) * 4, y[v].x * inv, y[v].y * inv, y[v].z * inv, y[v].w * inv);
+    }
+}
+
 // bf16: the warp computes S^T = K Q^T and O^T = V^T P^T with m16n8k16, keys
 // (then dimensions of V) on the 16-row side and the query rows on the 8-column
 // side, so 1..8 query rows waste none of the long side; P^T turns into the
@@ -118,8 +177,9 @@ __global__ void __launch_bounds__(StreamCfg<T, D, NB>::NT) k_paged_stream(const 
     pdl_launch_dependents();
 
     Cursor cons{};
-    uint32_t w1 = 0;
-    const bool any = plan_line<NT>(pv, a, cons, w1);
+    uint32_t w1 = 0, per = 1;
+    __shared__ int last;
+    const bool any = plan_line<NT>(pv, a, cons, w1, per);
     if (any) {
         Cursor load = cons;
         Piece lp{};
@@ -433,6 +493,23 @@ __global__ void __launch_bounds__(StreamCfg<T, D, NB>::NT) k_paged_stream(const 
                 }
             }
             __syncthreads();
+            if (a.direct && !whole) {
+                // the CTA that arrives last at a cut unit joins its parts
+                const Cut cut = cut_of(cons, p, per);
+                if (tid == 0) {
+                    __threadfence();
+                    last = atomicAdd(a.count + cut.i0, 1u) == (uint32_t)(cut.n - 1);
+                }
+                __syncthreads();
+                if (last) {
+                    __threadfence();
+                    join_unit<T, D, R, NT>(a, cut, nrows, mO, [&](int r) {
+                        return static_cast<T *>(a.out) + row_at(r, (int64_t)a.hq * D);
+                    });
+                    if (tid == 0) a.count[cut.i0] = 0u;
+                }
+                __syncthreads();
+            }
         }
         cp_wait<0>();
     }
@@ -445,20 +522,18 @@ struct JoinSource {
     const float *part;
     const uint64_t *cum;
     int64_t slots;
-    int owners, grid, min_tiles, rows, tile_rows, mode, direct;
+    int owners, grid, min_tiles, rows, tile_rows;
     LineGeo geo;
 };
 
-// A query row's parts: the slot of part k and the row's place in it.
+// A query row's parts: the slot of the first one and the row's place in each.
 struct Parts {
     const JoinSource *s;
     int64_t slot0;
-    int i0, n, row;
+    int n, row;
 
     __device__ __forceinline__ const float *slot(int k, int d) const {
-        int64_t at = slot0 + k;
-        if (s->direct) at = 2 * (int64_t)(i0 + k) + (k == 0 ? 1 : 0);
-        return s->part + at * ((int64_t)s->rows * (d + 2));
+        return s->part + (slot0 + k) * ((int64_t)s->rows * (d + 2));
     }
 };
 
@@ -499,7 +574,7 @@ __device__ __forceinline__ void join_row(const Parts &pa, const Parts &pb, T *ds
         const float f = m == -INFINITY ? 0.f : ex2(m - M);
         L = fmaf(l, f, L);
         const int top = min(32, n - i0);
-#pragma unroll 4
+#pragma unroll 8
         for (int i = 0; i < top; ++i) {
             const float fi = __shfl_sync(0xffffffffu, f, i);
             const Parts &x = i0 + i < pa.n ? pa : pb;
@@ -544,9 +619,9 @@ __device__ __forceinline__ Parts even_parts(const JoinSource &s, int kv_heads, i
     const uint32_t per = tiles_per_cta((uint32_t)all, (uint32_t)s.grid, (uint32_t)s.min_tiles), tiles = n / nu;
     const int hc = s.geo.hc > 1 ? gi / s.rows : 0;
     const uint32_t u = (uint32_t)(h * per_h + tt * s.geo.hc + hc), w0 = (uint32_t)c0 + u * tiles;
-    p.i0 = (int)(w0 / per);
-    p.slot0 = (int64_t)(c0 >> 32) + u + p.i0;
-    p.n = (int)((w0 + tiles - 1) / per) - p.i0 + 1;
+    const int i0 = (int)(w0 / per);
+    p.slot0 = (int64_t)(c0 >> 32) + u + i0;
+    p.n = (int)((w0 + tiles - 1) / per) - i0 + 1;
     p.row = slot_row(s, tl - tt * s.geo.tq, gi);
     if (p.slot0 + p.n > s.slots) p.n = 0;
     return p;
@@ -565,48 +640,6 @@ __global__ void __launch_bounds__(128) k_join_rows(const PagedView pv, const Joi
     const Parts pp = even_parts(pre, pv.kv_heads, g, t - pv.gs[g], h, gi);
     const Parts po = even_parts(own, pv.kv_heads, t, 0, h, gi);
     join_row<T, D>(pp, po, static_cast<T *>(out) + row * D);
-}
-
-// Whole units are written; block x joins the unit cut by the boundary between
-// CTA x and CTA x + 1, if that is the first boundary inside it.  One warp per
-// row, blockIdx.y over blocks of rows.
-constexpr int kCutRows = 16;
-template <typename T, int D>
-__global__ void __launch_bounds__(128) k_join_cut(const PagedView pv, const LineArgs a, const JoinSource s) {
-    pdl_launch_dependents();
-    pdl_wait();
-    const uint32_t W = (uint32_t)s.cum[s.owners];
-    const uint32_t per = tiles_per_cta(W, (uint32_t)s.grid, (uint32_t)s.min_tiles);
-    const uint64_t wb = (uint64_t)per * (blockIdx.x + 1);
-    if (wb >= W) return;
-    const uint32_t w = (uint32_t)wb;
-    // the owner of tile w: the last whose first tile is not behind it (owners without units come before)
-    const int lane = threadIdx.x & 31;
-    int lo = 0, hi = s.owners;
-    while (hi - lo > 1) {
-        const int step = (hi - lo + 31) >> 5, i = lo + (lane + 1) * step;
-        const int c = __popc(__ballot_sync(0xffffffffu, i < hi && (uint32_t)s.cum[i] <= w));
-        lo += c * step;
-        hi = min(hi, lo + step);
-    }
-    Cursor c{};
-    c.base = (uint32_t)s.cum[lo];
-    cursor_owner(c, pv, a, lo);
-    if (c.wh == 0 || w - c.base >= (uint32_t)pv.kv_heads * c.wh) return;   // starts that are not in order
-    const Piece p = unit_at(c, s.geo, w - c.base);
-    const uint32_t w0 = w - (uint32_t)p.tb;
-    if (p.tb == 0 || (uint64_t)(w0 / per + 1) * per != wb) return;
-    Parts pa{}, none{};
-    pa.s = none.s = &s;
-    pa.i0 = (int)(w0 / per);
-    pa.n = (int)((w0 + (uint32_t)p.tiles - 1) / per) - pa.i0 + 1;
-    const int G = s.geo.G, gb = s.geo.hc > 1 ? min(s.rows, G - p.hc * s.rows) : G, tok0 = p.tt * s.geo.tq;
-    const int nrows = min(s.geo.tq, c.ow.nt - tok0) * gb;
-    for (int r = blockIdx.y * kCutRows + (threadIdx.x >> 5); r < min(nrows, ((int)blockIdx.y + 1) * kCutRows); r += 4) {
-        const int tl = r / gb, gi = p.hc * s.rows + r - tl * gb;
-        pa.row = slot_row(s, tl, gi);
-        join_row<T, D>(pa, none, static_cast<T *>(a.out) + ((int64_t)(c.ow.t0 + tok0 + tl) * a.hq + p.h * G + gi) * D);
-    }
 }
 
 // ---------------------------------------------------------------- host side
@@ -694,8 +727,8 @@ int plan_attn(const cbq_paged_cache *c, const cbq_paged_batch *b, int64_t tokens
     p->own.mode = extend ? kFull : kOwn;
     p->own.direct = !p->prefix;
     p->own_tile = tile && extend && own_rows > 32;
-    int e = p->own_tile ? cbq_host::tile_plan(p->pv, p->d, p->G, kFull, own_rows > 128, 0, &p->own)
-                        : stream_plan(p->pv, p->dtype, p->d, p->G, own_rows, 0, &p->own);
+    int e = p->own_tile ? cbq_host::tile_plan(p->pv, p->d, p->G, kFull, own_rows > 128, cbq_host::kCountBytes, &p->own)
+                        : stream_plan(p->pv, p->dtype, p->d, p->G, own_rows, cbq_host::kCountBytes, &p->own);
     if (e != CBQ_OK) return e;
     p->bytes = p->own.end;
     if (p->prefix) {
@@ -718,6 +751,7 @@ LineArgs line_args(const cbq_host::LinePlan &lp, LineArgs a, uint8_t *ws) {
     a.slots = lp.slots;
     a.min_tiles = lp.min_tiles;
     a.direct = lp.direct;
+    a.count = reinterpret_cast<uint32_t *>(ws);
     a.cum = reinterpret_cast<uint64_t *>(ws + lp.cum_off);
     a.part = reinterpret_cast<float *>(ws + lp.part_off);
     return a;
@@ -733,16 +767,9 @@ int run_line(const cbq_paged_cache *c, const AttnPlan &p, const cbq_host::LinePl
 
 template <typename T, int D>
 int join_launch(const AttnPlan &p, const LineArgs &own, const JoinSource &so, const JoinSource &sp, cudaStream_t s) {
-    if (p.prefix) {
-        const int64_t blocks = ((int64_t)p.pv.tokens * own.hq + 3) / 4;
-        CBQ_CUDA_TRY(cbq_host::launch_pdl(k_join_rows<T, D>, dim3((unsigned)blocks), dim3(128), 0, s, p.pv, so, sp,
-                                          own.hq, own.out));
-    } else if (p.own.grid > 1) {
-        const int rows = p.own.geo.hc > 1 ? p.own.rows : p.own.geo.tq * p.G;
-        CBQ_CUDA_TRY(cbq_host::launch_pdl(k_join_cut<T, D>,
-                                          dim3((unsigned)(p.own.grid - 1), (unsigned)((rows + kCutRows - 1) / kCutRows)),
-                                          dim3(128), 0, s, p.pv, own, so));
-    }
+    const int64_t blocks = ((int64_t)p.pv.tokens * own.hq + 3) / 4;
+    CBQ_CUDA_TRY(cbq_host::launch_pdl(k_join_rows<T, D>, dim3((unsigned)blocks), dim3(128), 0, s, p.pv, so, sp, own.hq,
+                                      own.out));
     return CBQ_OK;
 }
 
@@ -769,16 +796,16 @@ int paged_attn(const cbq_paged_cache *c, const cbq_paged_batch *b, int64_t token
     auto source = [&](const cbq_host::LinePlan &lp) {
         return JoinSource{reinterpret_cast<const float *>(w + lp.part_off),
                           reinterpret_cast<const uint64_t *>(w + lp.cum_off), lp.slots, lp.owners, lp.grid, lp.min_tiles,
-                          lp.rows, lp.tile_rows, lp.mode, lp.direct, lp.geo};
+                          lp.rows, lp.tile_rows, lp.geo};
     };
-    JoinSource so = source(p.own), sp{};
     if (p.prefix) {
-        sp = source(p.pre);
         if ((rc = run_line(c, p, p.pre, p.pre_tile, line_args(p.pre, a, w), s)) != CBQ_OK) return rc;
         a.wait_first = 0;                              // the prefix launch passed its wait before this one can start
     }
     const LineArgs own = line_args(p.own, a, w);
     if ((rc = run_line(c, p, p.own, p.own_tile, own, s)) != CBQ_OK) return rc;
+    if (!p.prefix) return CBQ_OK;
+    const JoinSource so = source(p.own), sp = source(p.pre);
     if (p.dtype == CBQ_F32)
         return p.d == 64 ? join_launch<float, 64>(p, own, so, sp, s)
                          : (p.d == 128 ? join_launch<float, 128>(p, own, so, sp, s)

@@ -43,7 +43,9 @@ struct LineArgs {
     float sc;                          // scale * log2(e)
     void *out;
     float *part;                       // slots of [rows * D + 2 * rows] fp32: o (unnormalised), m, l
-    uint64_t *cum;                     // [owners + 1] units << 32 | tiles before each owner
+    uint64_t *cum;                     // [owners + 1] units << 32 | tiles before each owner (not direct)
+    uint32_t *count;                   // direct: arrivals at the unit cut at a CTA's end, by CTA (tile kernel: by CTA
+                                       // and warp); 0 between calls
     int64_t slots;                     // slots of `part` (starts that are not in order could name more)
     int owners, mode;
     int min_tiles;                     // a CTA's part has at least so many tiles
@@ -158,6 +160,9 @@ __device__ __forceinline__ OwnerTiles owner_tiles(const Owner &w, const LineGeo 
     return t;
 }
 
+struct Piece {
+    int h, tt, hc, tiles, tb, te;      // a unit of the cursor's owner, its tiles, the piece [tb, te) of them
+};
 // Position on the line.
 struct Cursor {
     uint32_t w;                        // next tile
@@ -167,9 +172,7 @@ struct Cursor {
     int o;
     Owner ow;
     OwnerTiles tl;
-};
-struct Piece {
-    int h, tt, hc, tiles, tb, te;      // a unit of the cursor's owner, its tiles, the piece [tb, te) of them
+    Piece p;                           // the piece before w (tiles 0: none yet)
 };
 
 __device__ __forceinline__ void cursor_owner(Cursor &c, const PagedView &pv, const LineArgs &a, int o) {
@@ -205,17 +208,33 @@ __device__ __forceinline__ Piece unit_at(const Cursor &c, const LineGeo &g, uint
 // The next piece of [.., w1); false at the end.  Leaves c.w behind it.
 __device__ __forceinline__ bool next_piece(Cursor &c, const PagedView &pv, const LineArgs &a, uint32_t w1, Piece &p) {
     if (c.w >= w1) return false;
-    while (true) {
-        const uint32_t n = (uint32_t)pv.kv_heads * c.wh;
-        if (c.w < c.base + n) break;
+    bool step = c.p.tiles > 0;                         // the unit after the last one, if its owner has one
+    while (c.w >= c.base + (uint32_t)pv.kv_heads * c.wh) {
         if (c.o + 1 >= a.owners) return false;
-        c.base += n;
+        c.base += (uint32_t)pv.kv_heads * c.wh;
         c.ubase += (uint32_t)(pv.kv_heads * c.tl.tt * a.geo.hc);
         cursor_owner(c, pv, a, c.o + 1);
+        step = false;
     }
-    p = unit_at(c, a.geo, c.w - c.base);
+    if (step) {
+        p = c.p;
+        if (++p.hc == a.geo.hc) {
+            p.hc = 0;
+            if (++p.tt == c.tl.tt) {
+                p.tt = 0;
+                ++p.h;
+            }
+            p.tiles = (int)c.tl.of(p.tt);
+        }
+        p.tb = 0;
+    } else if (c.w == c.base) {
+        p = Piece{0, 0, 0, (int)c.tl.of(0), 0, 0};
+    } else {
+        p = unit_at(c, a.geo, c.w - c.base);
+    }
     p.te = (int)min((uint32_t)p.tiles, p.tb + (w1 - c.w));
     c.w += (uint32_t)(p.te - p.tb);
+    c.p = p;
     return true;
 }
 
@@ -233,20 +252,20 @@ __host__ __device__ __forceinline__ uint32_t tiles_per_cta(uint32_t W, uint32_t 
 }
 
 // Of this CTA: its part [c.w, w1) of the line and the owner it begins in;
-// false: nothing to do.  CTA 0 leaves the sums before each owner in a.cum.
-// All NT threads call it.
+// false: nothing to do.  Unless direct, CTA 0 leaves the sums before each owner
+// in a.cum.  All NT threads call it.
 template <int NT>
-__device__ __forceinline__ bool plan_line(const PagedView &pv, const LineArgs &a, Cursor &c, uint32_t &w1) {
+__device__ __forceinline__ bool plan_line(const PagedView &pv, const LineArgs &a, Cursor &c, uint32_t &w1, uint32_t &per) {
     constexpr int NW = NT / 32;
     __shared__ uint64_t red[NW];
     __shared__ uint64_t found_base;
     __shared__ int found;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const bool writer = blockIdx.x == 0;
+    const bool writer = blockIdx.x == 0 && !a.direct;
     auto weight = [&](int o) -> uint64_t {
         if (o >= a.owners) return 0;
         const Owner w = owner_of(pv, a.mode, o);
-        if (writer && (a.mode == kPrefix ? pv.plens[o] > pv.pcap : pv.lens[o] > pv.cap))
+        if (blockIdx.x == 0 && (a.mode == kPrefix ? pv.plens[o] > pv.pcap : pv.lens[o] > pv.cap))
             report(pv.status, CBQ_FLAG_CORRUPT, (uint32_t)o);
         const OwnerTiles t = owner_tiles(w, a.geo, a.mode);
         const uint32_t n = (uint32_t)(pv.kv_heads * a.geo.hc);
@@ -264,7 +283,7 @@ __device__ __forceinline__ bool plan_line(const PagedView &pv, const LineArgs &a
 #pragma unroll
     for (int i = 0; i < NW; ++i) total += red[i];
     const uint32_t W = (uint32_t)total;
-    const uint32_t per = tiles_per_cta(W, gridDim.x, (uint32_t)a.min_tiles);
+    per = tiles_per_cta(W, gridDim.x, (uint32_t)a.min_tiles);
     const uint32_t w0 = (uint32_t)min((uint64_t)per * blockIdx.x, (uint64_t)W);
     w1 = min(w0 + per, W);
     if (writer && tid == 0) a.cum[a.owners] = total;
@@ -306,6 +325,21 @@ __device__ __forceinline__ bool plan_line(const PagedView &pv, const LineArgs &a
     return true;
 }
 
+// A cut unit (direct): the CTA its first piece is in, and how many it spans.
+struct Cut {
+    int i0, n;
+    __device__ __forceinline__ const float *slot(const LineArgs &a, int k, int64_t floats) const {
+        return a.part + (2 * (int64_t)(i0 + k) + (k == 0 ? 1 : 0)) * floats;
+    }
+};
+__device__ __forceinline__ Cut cut_of(const Cursor &c, const Piece &p, uint32_t per) {
+    const uint32_t w0 = c.w - (uint32_t)p.te;          // the unit's first tile (the cursor stands behind the piece)
+    Cut x;
+    x.i0 = (int)(w0 / per);
+    x.n = (int)((w0 + (uint32_t)p.tiles - 1) / per) - x.i0 + 1;
+    return x;
+}
+
 __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -335,6 +369,11 @@ struct LinePlan {
     int64_t slots, cum_off, part_off, end;
 };
 
+// The workspace begins with the arrival counters of direct lines: a fixed
+// place, so calls of any shape may share a workspace.
+constexpr int kCounts = 4096;
+constexpr int64_t kCountBytes = kCounts * 4;
+
 // Room of a planned line in the workspace from byte `off` on; false: more
 // tiles than 32 bits count.
 inline bool line_room(const cbq::PagedView &pv, int d, int64_t off, LinePlan *p) {
@@ -342,7 +381,7 @@ inline bool line_room(const cbq::PagedView &pv, int d, int64_t off, LinePlan *p)
     const int64_t tt = p->mode == cbq::kOwn ? pv.seqs : pv.tokens / p->geo.tq + p->owners;
     const int64_t units = tt * p->geo.hc * pv.kv_heads;
     const int64_t keys = p->mode == cbq::kOwn ? pv.cap : (p->mode == cbq::kPrefix ? pv.pcap : (int64_t)pv.cap + pv.pcap);
-    if (units * ((keys + 32) / p->geo.keys + 2) > 0x7fffffffll) return false;
+    if (units * ((keys + 32) / p->geo.keys + 2) > 0x7fffffffll || p->grid > kCounts) return false;
     p->slots = p->direct ? 2 * (int64_t)p->grid : units + p->grid;
     p->cum_off = off;
     p->part_off = align_up(off + (p->owners + 1) * 8, 256);

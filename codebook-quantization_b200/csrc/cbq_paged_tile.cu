@@ -143,6 +143,74 @@ __device__ __forceinline__ TileAt tile_at(const Owner &w, int t) {
     return x;
 }
 
+// A warp joins its 32 rows of a cut unit: lane l holds row `row`'s weights,
+// eight rows at a time take their parts with the row's 512 (256) bytes side by
+// side over the lanes.
+template <int D, int NQ>
+__device__ __forceinline__ void join_block(const LineArgs &a, const Cut &cut, int row, bool live, int64_t orow) {
+    constexpr int RR = NQ * kBlk, E = D / 32;
+    constexpr int64_t SL = (int64_t)RR * (D + 2);
+    const int lane = threadIdx.x & 31, row0 = row - lane;
+    float M = -INFINITY, L = 0.f;
+    if (live) {
+        for (int k = 0; k < cut.n; ++k) M = fmaxf(M, __ldcg(cut.slot(a, k, SL) + RR * D + row));
+        for (int k = 0; k < cut.n; ++k) {
+            const float *b = cut.slot(a, k, SL) + RR * D + row;
+            const float m = __ldcg(b);
+            if (m != -INFINITY) L = fmaf(__ldcg(b + RR), ex2(m - M), L);
+        }
+    }
+    const float inv = L == 0.f ? 0.f : 1.f / L;
+    const unsigned who = __ballot_sync(0xffffffffu, live);
+    __nv_bfloat16 *out = static_cast<__nv_bfloat16 *>(a.out);
+    for (int j0 = 0; j0 < 32; j0 += 8) {
+        if (!(who >> j0 & 0xffu)) continue;
+        float y[8][E];
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+#pragma unroll
+            for (int e = 0; e < E; ++e) y[j][e] = 0.f;
+        for (int k = 0; k < cut.n; ++k) {
+            const float *s = cut.slot(a, k, SL);
+            float f = 0.f;
+            if (live) {
+                const float m = __ldcg(s + RR * D + row);
+                f = m == -INFINITY ? 0.f : ex2(m - M) * inv;
+            }
+            float v[8][E];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float *b = s + (int64_t)(row0 + j0 + j) * D + lane * E;
+                if (who >> (j0 + j) & 1u) {
+                    if constexpr (E == 4) {
+                        const float4 x = __ldcg(reinterpret_cast<const float4 *>(b));
+                        v[j][0] = x.x; v[j][1] = x.y; v[j][2] = x.z; v[j][3] = x.w;
+                    } else {
+                        const float2 x = __ldcg(reinterpret_cast<const float2 *>(b));
+                        v[j][0] = x.x; v[j][1] = x.y;
+                    }
+                } else {
+#pragma unroll
+                    for (int e = 0; e < E; ++e) v[j][e] = 0.f;
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float fj = __shfl_sync(0xffffffffu, f, j0 + j);
+#pragma unroll
+                for (int e = 0; e < E; ++e) y[j][e] = fmaf(v[j][e], fj, y[j][e]);
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const int64_t at = __shfl_sync(0xffffffffu, orow, j0 + j) * D + lane * E;
+            if (!(who >> (j0 + j) & 1u)) continue;
+            if constexpr (E == 4) st4(out + at, y[j][0], y[j][1], y[j][2], y[j][3]);
+            else *reinterpret_cast<uint32_t *>(out + at) = pack_bf16(y[j][0], y[j][1]);
+        }
+    }
+}
+
 template <int D, int NQ>
 __global__ void __launch_bounds__(TileCfg<D, NQ>::kThreads, TileCfg<D, NQ>::kCtas)
     k_paged_tile(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const PagedView pv,
@@ -183,8 +251,8 @@ __global__ void __launch_bounds__(TileCfg<D, NQ>::kThreads, TileCfg<D, NQ>::kCta
     tc_after();
     const uint32_t tmem = bars->tmem;
     Cursor c{};
-    uint32_t w1 = 0;
-    const bool any = plan_line<Cfg::kThreads>(pv, a, c, w1);
+    uint32_t w1 = 0, per = 1;
+    const bool any = plan_line<Cfg::kThreads>(pv, a, c, w1, per);
 
     const int tb = kBlk / a.geo.G;                     // tokens of a row block
     Piece p{};
@@ -231,6 +299,7 @@ __global__ void __launch_bounds__(TileCfg<D, NQ>::kThreads, TileCfg<D, NQ>::kCta
             const int olim = a.mode == kPrefix ? 0 : own_limit(c.ow, tok);
             // the piece's place and output, before the cursor moves on
             const bool whole = a.direct && p.tb == 0 && p.te == p.tiles;
+            const Cut cut = cut_of(c, p, per);
             const int64_t slot = slot_of(c, p, a, (int)blockIdx.x);
             const int64_t orow = (int64_t)(c.ow.t0 + tok) * a.hq + p.h * a.geo.G + rg;
             float m = -INFINITY, l = 0.f;
@@ -332,6 +401,22 @@ __global__ void __launch_bounds__(TileCfg<D, NQ>::kThreads, TileCfg<D, NQ>::kCta
                 // joined with parts of either kernel: the maximum in units of log2
                 ps[NQ * kBlk * D + q * kBlk + r] = m == -INFINITY ? m : m * sc;
                 ps[NQ * kBlk * D + NQ * kBlk + q * kBlk + r] = l;
+            }
+            if (a.direct && !whole) {
+                // the warp that arrives last at its 32 rows of a cut unit joins
+                // their parts (a count for each warp: no barrier that a warp whose
+                // wait gave up could leave the others at)
+                __threadfence();
+                __syncwarp();
+                uint32_t *cnt = a.count + cut.i0 * 8 + warp;
+                uint32_t before = 0;
+                if (lane == 0) before = atomicAdd(cnt, 1u);
+                before = __shfl_sync(0xffffffffu, before, 0);
+                if (before == (uint32_t)(cut.n - 1)) {
+                    __threadfence();
+                    join_block<D, NQ>(a, cut, q * kBlk + r, live, orow);
+                    if (lane == 0) *cnt = 0u;
+                }
             }
             __syncwarp();
             tc_before();                               // O's reads before the next unit's first product
@@ -542,9 +627,9 @@ int tile_plan(const cbq::PagedView &pv, int d, int G, int mode, bool two, int64_
     p->geo.hc = 1;
     p->geo.keys = kBlk;
     p->geo.join = 0;
-    p->min_tiles = 2;
+    p->min_tiles = 2;                  // a part costs its CTA about as much as a tile
     p->grid = n * sm_count();
-    return line_room(pv, d, off, p) ? CBQ_OK : CBQ_ERR_UNSUPPORTED;
+    return p->grid * 8 <= kCounts && line_room(pv, d, off, p) ? CBQ_OK : CBQ_ERR_UNSUPPORTED;
 }
 
 int tile_launch(const cbq_paged_cache *c, const cbq::PagedView &pv, const LinePlan &p, cbq::LineArgs a, cudaStream_t s) {

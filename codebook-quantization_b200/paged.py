@@ -27,6 +27,10 @@ from . import _lib
 
 __all__ = ["PagedKVCache", "PagedBatch"]
 
+# Zero-filled scratch of the attention calls, one growing buffer per stream: calls
+# on one stream do not overlap, and each leaves its arrival counters zero.
+_WORKSPACES = {}
+
 _CODES = {torch.float32: _lib.CBQ_F32, torch.bfloat16: _lib.CBQ_BF16}
 
 
@@ -176,7 +180,8 @@ class PagedKVCache:
               out.device == self.device, f"out: contiguous [{tokens}, {heads}, {self.head_dim}] of the cache's dtype")
 
     def workspace_bytes(self, batch: PagedBatch, tokens: int, heads: int, extend: bool) -> int:
-        """Bytes of scratch one attention call needs."""
+        """Bytes of the zero-filled scratch one attention call needs; a
+        ``workspace=`` tensor may serve calls of any shape that do not overlap."""
         key = (self._key, tokens, heads, extend)
         n = batch._ws.get(key)
         if n is None:
@@ -192,14 +197,23 @@ class PagedKVCache:
             out = torch.empty((tokens, heads, d), dtype=self.dtype, device=self.device)
         else:
             self._out(out, tokens, heads)
+        stream = torch.cuda.current_stream(self.device).cuda_stream
         if workspace is None:
-            # from torch's caching allocator: safe on any stream, and inside a captured graph
-            workspace = torch.empty(self.workspace_bytes(batch, tokens, heads, extend), dtype=torch.uint8,
-                                    device=self.device)
+            workspace = self._scratch(stream, self.workspace_bytes(batch, tokens, heads, extend))
         _lib.call(name, self._addr, batch._addr, tokens, q.data_ptr(), stride, heads,
-                  d ** -0.5 if scale is None else scale, out.data_ptr(), workspace.data_ptr(), workspace.numel(),
-                  torch.cuda.current_stream(self.device).cuda_stream)
+                  d ** -0.5 if scale is None else scale, out.data_ptr(), workspace.data_ptr(), workspace.numel(), stream)
         return out
+
+    def _scratch(self, stream: int, need: int) -> torch.Tensor:
+        """Zero-filled scratch for calls on ``stream``; inside a graph capture a
+        buffer of the graph's own, which its replays clear."""
+        if torch.cuda.is_current_stream_capturing():
+            return torch.zeros(need, dtype=torch.uint8, device=self.device)
+        key = (self.device.index, stream)
+        ws = _WORKSPACES.get(key)
+        if ws is None or ws.numel() < need:
+            ws = _WORKSPACES[key] = torch.zeros(need + need // 2, dtype=torch.uint8, device=self.device)
+        return ws
 
     def attend_decode(self, batch: PagedBatch, q: torch.Tensor, scale: Optional[float] = None,
                       out: Optional[torch.Tensor] = None, workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
