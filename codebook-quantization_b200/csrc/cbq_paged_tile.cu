@@ -15,7 +15,8 @@
 //
 // Warp roles: NQ softmax warpgroups (one row block each), a TMA warp (one
 // cp.async.bulk.tensor per page, or part of one, and 64 dimensions; K and V
-// tiles alternate in a ring of 128-key slots), an MMA warp.  With NQ = 2 the
+// tiles alternate in a ring of 128-key slots), an MMA warp, a warp that walks
+// the line ahead of them and leaves its pieces in shared memory.  With NQ = 2 the
 // MMA warp's order is P0 V, Q0 K', P1 V, Q1 K': each softmax works while the
 // tensor core does the other row block's products.
 // Work is the tile line of cbq_paged_line.cuh, one persistent CTA per part.
@@ -40,22 +41,37 @@ template <int D, int NQ> struct TileCfg {
     static constexpr int kTileB = kHalves * kHalfB;
     static constexpr int kSlots = NQ == 2 ? (D == 128 ? 5 : 8) : (D == 128 ? 2 : 4);   // K / V tiles in flight
     static constexpr int kSoft = NQ * 128;
-    static constexpr int kThreads = kSoft + 64;
+    static constexpr int kThreads = kSoft + 128;                       // + a warpgroup for the TMA and the MMA warp
+    // registers: the launch's share is split unevenly, kSoft * kSoftRegs + 128 * kRestRegs <= 65536 / kCtas
+    static constexpr int kSoftRegs = NQ == 2 ? 208 : 200;
+    static constexpr int kRestRegs = NQ == 2 ? 88 : 56;
     static constexpr int kCtas = NQ == 2 ? 1 : 2;                       // per SM: TMEM has 512 columns
     static constexpr int kCols = NQ == 2 ? 512 : 256;
-    static constexpr int kSmem = 1024 + (NQ + kSlots) * kTileB + 512;
+    static constexpr int kSmem = 1024 + (NQ + kSlots) * kTileB + 768;
     static __host__ __device__ constexpr uint32_t sCol(int b) { return (uint32_t)b * 128u; }
     static __host__ __device__ constexpr uint32_t oCol(int b) { return (uint32_t)NQ * 128u + (uint32_t)b * 128u; }
 };
 
+// A piece of the line as the roles need it, written by the scheduling warp.
+struct Work {
+    int o, t0, nt, plen, olen, group;  // owner
+    int h, tok, tb, te;                // kv head, first token in the owner, key tiles
+    int whole, live;                   // a whole unit of a direct line; 0: the line's end
+    Cut cut;
+    int64_t slot;
+};
+constexpr int kWorks = 3;              // the piece in hand, the next one, one ahead
+
 struct Bars {
     uint64_t q_full[2], s_full[2], p_full[2], o_full[2];
     uint64_t kv_full[8], kv_empty[8];
+    uint64_t w_full[kWorks], w_empty[kWorks];
     uint64_t drain;
     uint32_t tmem;
     int abort_flag;
+    Work work[kWorks];
 };
-static_assert(sizeof(Bars) <= 512, "barriers outgrow their region");
+static_assert(sizeof(Bars) <= 768, "barriers outgrow their region");
 
 // ---------------------------------------------------------------- PTX helpers
 __device__ __forceinline__ uint64_t desc_k(uint32_t addr) {
@@ -134,12 +150,12 @@ struct TileAt {
     bool pre;
     int key0, have;                    // rows of the tile that exist (0..128)
 };
-__device__ __forceinline__ TileAt tile_at(const Owner &w, int t) {
-    const int np = (w.plen + kBlk - 1) / kBlk;
+__device__ __forceinline__ TileAt tile_at(int plen, int olen, int t) {
+    const int np = (plen + kBlk - 1) / kBlk;
     TileAt x;
     x.pre = t < np;
     x.key0 = (x.pre ? t : t - np) * kBlk;
-    x.have = clampi((x.pre ? w.plen : w.olen) - x.key0, 0, kBlk);
+    x.have = clampi((x.pre ? plen : olen) - x.key0, 0, kBlk);
     return x;
 }
 
@@ -211,6 +227,9 @@ __device__ __forceinline__ void join_block(const LineArgs &a, const Cut &cut, in
     }
 }
 
+template <int N> __device__ __forceinline__ void regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N> __device__ __forceinline__ void regs_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+
 template <int D, int NQ>
 __global__ void __launch_bounds__(TileCfg<D, NQ>::kThreads, TileCfg<D, NQ>::kCtas)
     k_paged_tile(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const PagedView pv,
@@ -222,7 +241,7 @@ __global__ void __launch_bounds__(TileCfg<D, NQ>::kThreads, TileCfg<D, NQ>::kCta
     uint8_t *sQ = smem, *sKV = smem + NQ * kTileB;
     Bars *bars = reinterpret_cast<Bars *>(sKV + kSlots * kTileB);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    constexpr int kTmaWarp = Cfg::kSoft / 32, kMmaWarp = kTmaWarp + 1;
+    constexpr int kTmaWarp = Cfg::kSoft / 32, kMmaWarp = kTmaWarp + 1, kWorkWarp = kTmaWarp + 2;
 
     if (tid == 0) {
         for (int q = 0; q < NQ; ++q) {
@@ -234,6 +253,10 @@ __global__ void __launch_bounds__(TileCfg<D, NQ>::kThreads, TileCfg<D, NQ>::kCta
         for (int s = 0; s < kSlots; ++s) {
             mbar_init(&bars->kv_full[s], 1);
             mbar_init(&bars->kv_empty[s], 1);
+        }
+        for (int i = 0; i < kWorks; ++i) {
+            mbar_init(&bars->w_full[i], 1);
+            mbar_init(&bars->w_empty[i], kWorkWarp);  // one arrival of every other warp
         }
         mbar_init(&bars->drain, 1);
         bars->abort_flag = 0;
@@ -254,8 +277,18 @@ __global__ void __launch_bounds__(TileCfg<D, NQ>::kThreads, TileCfg<D, NQ>::kCta
     uint32_t w1 = 0, per = 1;
     const bool any = plan_line<Cfg::kThreads>(pv, a, c, w1, per);
 
+    // The i-th piece (0 where the line ends or a wait gave up); done(i) gives its place back.
+    auto work = [&](uint32_t i) -> const Work * {
+        if (!warp_wait(&bars->w_full[i % kWorks], (i / kWorks) & 1, bars, pv.status)) return nullptr;
+        const Work *w = &bars->work[i % kWorks];
+        return w->live ? w : nullptr;
+    };
+    auto done = [&](uint32_t i) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars->w_empty[i % kWorks]);
+    };
     const int tb = kBlk / a.geo.G;                     // tokens of a row block
-    Piece p{};
+    if (warp < kTmaWarp) regs_up<Cfg::kSoftRegs>(); else regs_down<Cfg::kRestRegs>();
     if (!any) {
         // nothing of the line for this CTA
     } else if (warp < kTmaWarp) {
@@ -267,18 +300,18 @@ __global__ void __launch_bounds__(TileCfg<D, NQ>::kThreads, TileCfg<D, NQ>::kCta
         // a negative scale turns Q's sign at its load, zero its value: sc > 0 below
         const float sc = a.sc == 0.f ? 1.f : fabsf(a.sc);
         const uint32_t sign = a.sc < 0.f ? 0x80008000u : 0u, keep = a.sc == 0.f ? 0u : 0xffffffffu;
-        // the block's rows of the unit at cursor c into shared memory (128-byte swizzle)
-        auto load_q = [&]() {
+        // the block's rows of a piece into shared memory (128-byte swizzle)
+        auto load_q = [&](const Work *w) {
             uint8_t *dst = sQ + q * kTileB;
-            const int tok0 = p.tt * a.geo.tq + q * tb, left = min(tb, c.ow.nt - tok0);
+            const int tok0 = w->tok + q * tb, left = min(tb, w->nt - tok0), t0 = w->t0 + tok0, h0 = w->h * a.geo.G;
             constexpr int CH = D / 8;
 #pragma unroll 4
             for (int e = r; e < kBlk * CH; e += 128) {
                 const int row = e / CH, ch = e - row * CH, tk = row / a.geo.G;
                 uint4 v = make_uint4(0u, 0u, 0u, 0u);
                 if (tk < left) {
-                    const __nv_bfloat16 *src = static_cast<const __nv_bfloat16 *>(a.q) + (int64_t)(c.ow.t0 + tok0 + tk) * a.qs +
-                                               (int64_t)(p.h * a.geo.G + row - tk * a.geo.G) * D + ch * 8;
+                    const __nv_bfloat16 *src = static_cast<const __nv_bfloat16 *>(a.q) + (int64_t)(t0 + tk) * a.qs +
+                                               (int64_t)(h0 + row - tk * a.geo.G) * D + ch * 8;
                     v = *reinterpret_cast<const uint4 *>(src);
                     v.x = (v.x ^ sign) & keep;
                     v.y = (v.y ^ sign) & keep;
@@ -290,20 +323,16 @@ __global__ void __launch_bounds__(TileCfg<D, NQ>::kThreads, TileCfg<D, NQ>::kCta
             fence_proxy_async_smem();
             mbar_arrive(&bars->q_full[q]);
         };
-        bool go = next_piece(c, pv, a, w1, p);
-        if (go) load_q();
-        uint32_t ns = 0;                               // tiles seen (phases of s_full and o_full)
-        while (go) {
-            const int tok = p.tt * a.geo.tq + q * tb + rt;
-            const bool live = rt < tb && tok < c.ow.nt;
-            const int olim = a.mode == kPrefix ? 0 : own_limit(c.ow, tok);
-            // the piece's place and output, before the cursor moves on
-            const bool whole = a.direct && p.tb == 0 && p.te == p.tiles;
-            const Cut cut = cut_of(c, p, per);
-            const int64_t slot = slot_of(c, p, a, (int)blockIdx.x);
-            const int64_t orow = (int64_t)(c.ow.t0 + tok) * a.hq + p.h * a.geo.G + rg;
+        uint32_t nw = 0, ns = 0;                       // pieces; tiles seen (phases of s_full and o_full)
+        const Work *w = work(0);
+        if (w) load_q(w);
+        bool go = true;
+        while (w) {
+            const int tok = w->tok + q * tb + rt;
+            const bool live = rt < tb && tok < w->nt;
+            const int plen = w->plen, olen = w->olen, t0 = w->tb, t1 = w->te;
+            const int olim = a.mode == kPrefix ? 0 : clampi(olen - w->nt + tok + 1, 0, olen);
             float m = -INFINITY, l = 0.f;
-            const int t0 = p.tb, t1 = p.te;
             for (int t = t0; t < t1; ++t, ++ns) {
                 if (!warp_wait(&bars->s_full[q], ns & 1, bars, pv.status)) { go = false; break; }
                 tc_after();
@@ -311,7 +340,7 @@ __global__ void __launch_bounds__(TileCfg<D, NQ>::kThreads, TileCfg<D, NQ>::kCta
 #pragma unroll
                 for (int i = 0; i < 4; ++i) tld32(tS + i * 32, s + i * 32);
                 tld_wait();
-                const TileAt x = tile_at(c.ow, t);
+                const TileAt x = tile_at(plen, olen, t);
                 const int vis = x.pre ? x.have : min(x.have, olim - x.key0);   // visible keys of the tile
                 if (__any_sync(0xffffffffu, vis < kBlk)) {
 #pragma unroll
@@ -366,13 +395,14 @@ __global__ void __launch_bounds__(TileCfg<D, NQ>::kThreads, TileCfg<D, NQ>::kCta
             }
             if (!go) break;
             // the last S has been read, so every product with this Q is done
-            const bool more = next_piece(c, pv, a, w1, p);
-            if (more) load_q();
+            const Work *wn = work(nw + 1);
+            if (wn) load_q(wn);
             if (!warp_wait(&bars->o_full[q], (ns - 1) & 1, bars, pv.status)) { go = false; break; }
             tc_after();
             const float inv = l == 0.f ? 0.f : 1.f / l;
-            float *ps = a.part + slot * (int64_t)(NQ * kBlk * (D + 2));
-            const bool fits = slot < a.slots;
+            float *ps = a.part + w->slot * (int64_t)(NQ * kBlk * (D + 2));
+            const bool fits = w->slot < a.slots, whole = w->whole;
+            const int64_t orow = (int64_t)(w->t0 + tok) * a.hq + w->h * a.geo.G + rg;
 #pragma unroll 1
             for (int i = 0; i < D; i += 32) {
                 uint32_t o[32];
@@ -408,6 +438,7 @@ __global__ void __launch_bounds__(TileCfg<D, NQ>::kThreads, TileCfg<D, NQ>::kCta
                 // wait gave up could leave the others at)
                 __threadfence();
                 __syncwarp();
+                const Cut cut = w->cut;
                 uint32_t *cnt = a.count + cut.i0 * 8 + warp;
                 uint32_t before = 0;
                 if (lane == 0) before = atomicAdd(cnt, 1u);
@@ -420,26 +451,31 @@ __global__ void __launch_bounds__(TileCfg<D, NQ>::kThreads, TileCfg<D, NQ>::kCta
             }
             __syncwarp();
             tc_before();                               // O's reads before the next unit's first product
-            go = more;
+            done(nw);
+            ++nw;
+            w = wn;
         }
     } else if (warp == kTmaWarp) {
         // ------------------------------------------------------------- K and V tiles
-        uint32_t n = 0;                                // tiles issued (K and V)
+        uint32_t n = 0, nw = 0;                        // tiles issued (K and V), pieces
         bool go = true;
         const int ps = 1 << pv.ps_shift, box = min(ps, kBlk);
-        while (go && next_piece(c, pv, a, w1, p)) {
-            for (int t = p.tb; t < p.te && go; ++t) {
-                const TileAt x = tile_at(c.ow, t);
+        while (go) {
+            const Work *w = work(nw);
+            if (!w) break;
+            const int plen = w->plen, olen = w->olen, h = w->h, o = w->o, t1 = w->te;
+            const int32_t *ptab = pv.ptable + w->group * pv.ptable_stride, *otab = pv.table + o * pv.table_stride;
+            for (int t = w->tb; t < t1 && go; ++t) {
+                const TileAt x = tile_at(plen, olen, t);
                 const int nbox = (x.have + box - 1) / box;
                 // lane: one box of rows and 64 dimensions
                 const int bx = lane / Cfg::kHalves, hf = lane - bx * Cfg::kHalves;
                 const int key = x.key0 + bx * box;
                 int page = 0;
                 if (bx < nbox) {
-                    const int32_t *tab = x.pre ? pv.ptable + c.ow.group * pv.ptable_stride : pv.table + c.o * pv.table_stride;
-                    page = __ldg(tab + (key >> pv.ps_shift));
+                    page = __ldg((x.pre ? ptab : otab) + (key >> pv.ps_shift));
                     if (page < 0 || page >= pv.pages) {
-                        if (hf == 0) report(pv.status, CBQ_FLAG_CORRUPT, (uint32_t)c.o);
+                        if (hf == 0) report(pv.status, CBQ_FLAG_CORRUPT, (uint32_t)o);
                         page = pv.pages;               // outside the map: the copy fills with zeros
                     }
                 }
@@ -454,19 +490,20 @@ __global__ void __launch_bounds__(TileCfg<D, NQ>::kThreads, TileCfg<D, NQ>::kCta
                     __syncwarp();
                     if (bx < nbox)
                         tma_4d(smem_u32(sKV + s * kTileB + hf * kHalfB + bx * box * 128), kv ? &vmap : &kmap, hf * 64,
-                               key & (ps - 1), p.h, page, &bars->kv_full[s]);
+                               key & (ps - 1), h, page, &bars->kv_full[s]);
                 }
             }
+            done(nw++);
         }
         // no copy may still be landing when the CTA ends
         for (uint32_t s = 0; s < kSlots && s < n; ++s) {
             const uint32_t last = n - 1 - (n - 1 - s) % kSlots;
             mbar_wait_bounded(&bars->kv_full[s], (last / kSlots) & 1);
         }
-    } else {
+    } else if (warp == kMmaWarp) {
         // ------------------------------------------------------------------ products
         constexpr uint32_t idS = idesc(128, 128, 0), idO = idesc(128, D, 1);
-        uint32_t n = 0, np = 0, nq = 0;                // ring tiles used, p_full phases, pieces
+        uint32_t n = 0, np = 0, nw = 0;                // ring tiles used, p_full phases, pieces
         bool go = true;
         auto slot = [&](uint32_t i) { return smem_u32(sKV + (i % kSlots) * kTileB); };
         auto wait_kv = [&](uint32_t i) {
@@ -499,12 +536,17 @@ __global__ void __launch_bounds__(TileCfg<D, NQ>::kThreads, TileCfg<D, NQ>::kCta
             if (lane == 0) mma_commit(&bars->kv_empty[i % kSlots]);
             __syncwarp();
         };
-        while (go && next_piece(c, pv, a, w1, p)) {
+        while (go) {
+            const Work *w = work(nw);
+            if (!w) {
+                go = !*(volatile int *)&bars->abort_flag;
+                break;
+            }
             // ring: K of tile t at n + 2 t, V at n + 2 t + 1
-            const int nt = p.te - p.tb;
+            const int plen = w->plen, olen = w->olen, tb0 = w->tb, nt = w->te - tb0;
             go = wait_kv(n);
             for (int q = 0; q < NQ && go; ++q) {
-                go = warp_wait(&bars->q_full[q], nq & 1, bars, pv.status);
+                go = warp_wait(&bars->q_full[q], nw & 1, bars, pv.status);
                 tc_after();
                 if (go) scores(q, n);
             }
@@ -513,7 +555,7 @@ __global__ void __launch_bounds__(TileCfg<D, NQ>::kThreads, TileCfg<D, NQ>::kCta
             for (int t = 0; t < nt; ++t, ++np) {
                 const uint32_t iv = n + 2 * t + 1;
                 if (!(go = wait_kv(iv))) break;
-                const TileAt x = tile_at(c.ow, p.tb + t);
+                const TileAt x = tile_at(plen, olen, tb0 + t);
                 if (x.have < kBlk) {
                     // rows that do not exist (rest of a page, pages not copied) must not meet a weight of 0
                     for (int e = x.have * 8 + lane; e < kBlk * 8; e += 32)
@@ -538,13 +580,36 @@ __global__ void __launch_bounds__(TileCfg<D, NQ>::kThreads, TileCfg<D, NQ>::kCta
                 release(iv);
                 if (next) release(iv + 1);
             }
+            if (!go) break;
             n += 2 * nt;
-            ++nq;
+            done(nw++);
         }
         if (!go) {                                     // gave up: products in flight end first
             if (lane == 0) mma_commit(&bars->drain);
             __syncwarp();
             mbar_wait_bounded(&bars->drain, 0);
+        }
+    } else if (warp == kWorkWarp) {
+        // -------------------------------------------------------------- the line ahead
+        Piece p{};
+        bool more = true;
+        for (uint32_t i = 0; more; ++i) {
+            if (i >= kWorks && !warp_wait(&bars->w_empty[i % kWorks], (i / kWorks - 1) & 1, bars, pv.status)) break;
+            more = next_piece(c, pv, a, w1, p);
+            if (lane == 0) {
+                Work *w = &bars->work[i % kWorks];
+                w->live = more;
+                if (more) {
+                    w->o = c.o; w->t0 = c.ow.t0; w->nt = c.ow.nt; w->plen = c.ow.plen; w->olen = c.ow.olen;
+                    w->group = max(c.ow.group, 0);
+                    w->h = p.h; w->tok = p.tt * a.geo.tq; w->tb = p.tb; w->te = p.te;
+                    w->whole = a.direct && p.tb == 0 && p.te == p.tiles;
+                    w->cut = cut_of(c, p, per);
+                    w->slot = slot_of(c, p, a, (int)blockIdx.x);
+                }
+                mbar_arrive(&bars->w_full[i % kWorks]);
+            }
+            __syncwarp();
         }
     }
     tc_before();
