@@ -134,9 +134,14 @@ __device__ __forceinline__ void tst32(uint32_t a, const uint32_t *v) {
 }
 __device__ __forceinline__ void tst_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// Bounded wait of a whole warp; false (for all its lanes) once the CTA has given up.
+// Bounded wait of a whole warp; false (for all its lanes) once the CTA has
+// given up.  The waits of the pipeline end within microseconds: they suspend on
+// the barrier and only then look at the clock, whose read is slow.
 __device__ __forceinline__ bool warp_wait(uint64_t *bar, uint32_t parity, Bars *b, uint32_t *status) {
-    bool ok = !*(volatile int *)&b->abort_flag && mbar_wait_bounded(bar, parity);
+    bool ok = mbar_try_wait(bar, parity);
+#pragma unroll 1
+    for (int i = 0; i < 4 && !ok; ++i) ok = mbar_try_wait_sleep(bar, parity, 20000u);
+    if (!ok) ok = !*(volatile int *)&b->abort_flag && mbar_wait_bounded(bar, parity);
     ok = __all_sync(0xffffffffu, ok);
     if (!ok && (threadIdx.x & 31) == 0 && !*(volatile int *)&b->abort_flag) {
         *(volatile int *)&b->abort_flag = 1;
@@ -300,25 +305,27 @@ __global__ void __launch_bounds__(TileCfg<D, NQ>::kThreads, TileCfg<D, NQ>::kCta
         // a negative scale turns Q's sign at its load, zero its value: sc > 0 below
         const float sc = a.sc == 0.f ? 1.f : fabsf(a.sc);
         const uint32_t sign = a.sc < 0.f ? 0x80008000u : 0u, keep = a.sc == 0.f ? 0u : 0xffffffffu;
+        const uint32_t ginv = (65536u + a.geo.G - 1) / a.geo.G;       // x / G = x * ginv >> 16 for x < 128
         // the block's rows of a piece into shared memory (128-byte swizzle)
         auto load_q = [&](const Work *w) {
             uint8_t *dst = sQ + q * kTileB;
             const int tok0 = w->tok + q * tb, left = min(tb, w->nt - tok0), t0 = w->t0 + tok0, h0 = w->h * a.geo.G;
             constexpr int CH = D / 8;
-#pragma unroll 4
-            for (int e = r; e < kBlk * CH; e += 128) {
-                const int row = e / CH, ch = e - row * CH, tk = row / a.geo.G;
-                uint4 v = make_uint4(0u, 0u, 0u, 0u);
-                if (tk < left) {
-                    const __nv_bfloat16 *src = static_cast<const __nv_bfloat16 *>(a.q) + (int64_t)(t0 + tk) * a.qs +
-                                               (int64_t)(h0 + row - tk * a.geo.G) * D + ch * 8;
-                    v = *reinterpret_cast<const uint4 *>(src);
-                    v.x = (v.x ^ sign) & keep;
-                    v.y = (v.y ^ sign) & keep;
-                    v.z = (v.z ^ sign) & keep;
-                    v.w = (v.w ^ sign) & keep;
-                }
-                *reinterpret_cast<uint4 *>(dst + (ch >> 3) * kHalfB + row * 128 + (((ch & 7) ^ (row & 7)) << 4)) = v;
+            uint4 v[CH];                               // all loads first
+#pragma unroll
+            for (int i = 0; i < CH; ++i) {
+                const int e = i * 128 + r, row = e / CH, ch = e - row * CH, tk = (int)((uint32_t)row * ginv >> 16);
+                v[i] = make_uint4(0u, 0u, 0u, 0u);
+                if (tk < left)
+                    v[i] = *reinterpret_cast<const uint4 *>(static_cast<const __nv_bfloat16 *>(a.q) +
+                                                            (int64_t)(t0 + tk) * a.qs +
+                                                            (int64_t)(h0 + row - tk * a.geo.G) * D + ch * 8);
+            }
+#pragma unroll
+            for (int i = 0; i < CH; ++i) {
+                const int e = i * 128 + r, row = e / CH, ch = e - row * CH;
+                *reinterpret_cast<uint4 *>(dst + (ch >> 3) * kHalfB + row * 128 + (((ch & 7) ^ (row & 7)) << 4)) =
+                    make_uint4((v[i].x ^ sign) & keep, (v[i].y ^ sign) & keep, (v[i].z ^ sign) & keep, (v[i].w ^ sign) & keep);
             }
             fence_proxy_async_smem();
             mbar_arrive(&bars->q_full[q]);
