@@ -74,30 +74,36 @@ struct Bars {
 static_assert(sizeof(Bars) <= 768, "barriers outgrow their region");
 
 // ---------------------------------------------------------------- PTX helpers
-__device__ __forceinline__ uint64_t desc_k(uint32_t addr) {
-    // K-major operand, 128-byte swizzle: rows of 128 bytes, 8-row groups 1024 bytes apart
-    return (uint64_t)((addr >> 4) & 0x3FFFu) | ((uint64_t)1 << 16) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) |
-           ((uint64_t)2 << 61);
-}
-__device__ __forceinline__ uint64_t desc_mn(uint32_t addr, uint32_t block_bytes) {
-    // MN-major operand (rows are K), 128-byte swizzle: 64-wide column blocks block_bytes apart, 8-row groups 1024 bytes apart
-    return (uint64_t)((addr >> 4) & 0x3FFFu) | ((uint64_t)(block_bytes >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
-           ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
-}
+// Shared-memory operand descriptors, 128-byte swizzle, 8-row groups 1024 bytes
+// apart.  The low word holds the address (in 16-byte units; stepping through an
+// operand adds to it) and the leading offset: unused for a K-major operand, the
+// distance of the 64-wide column blocks for an MN-major one (rows are K).
+constexpr uint32_t kDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t desc_lo(uint32_t addr, uint32_t lead) { return (addr >> 4) | (lead >> 4) << 16; }
 // kind::f16: D fp32, A and B bf16, A K-major, B K-major or (bt) MN-major.
 __host__ __device__ constexpr uint32_t idesc(int M, int N, int bt) {
     return (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)bt << 16) | ((uint32_t)(N >> 3) << 17) |
            ((uint32_t)(M >> 4) << 24);
 }
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t acc) {
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t id, uint32_t acc) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(id), "r"(acc));
+        "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "mov.b64 da, {%1, %5};\n\tmov.b64 db, {%2, %5};\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n\t}" ::"r"(d), "r"(a), "r"(b), "r"(id), "r"(acc),
+        "r"(kDescHi));
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t id, uint32_t acc) {
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t id, uint32_t acc) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(id), "r"(acc));
+        "{\n\t.reg .pred p;\n\t.reg .b64 db;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "mov.b64 db, {%2, %5};\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, p;\n\t}" ::"r"(d), "r"(a), "r"(b), "r"(id), "r"(acc),
+        "r"(kDescHi));
+}
+// One lane of the warp; the code under it stays uniform to the compiler.
+__device__ __forceinline__ bool elect() {
+    uint32_t e;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(e));
+    return e != 0;
 }
 __device__ __forceinline__ void mma_commit(uint64_t *bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
@@ -277,7 +283,7 @@ __global__ void __launch_bounds__(TileCfg<D, NQ>::kThreads, TileCfg<D, NQ>::kCta
     tc_before();
     __syncthreads();
     tc_after();
-    const uint32_t tmem = bars->tmem;
+    const uint32_t tmem = __shfl_sync(0xffffffffu, bars->tmem, 0);
     Cursor c{};
     uint32_t w1 = 0, per = 1;
     const bool any = plan_line<Cfg::kThreads>(pv, a, c, w1, per);
@@ -512,35 +518,34 @@ __global__ void __launch_bounds__(TileCfg<D, NQ>::kThreads, TileCfg<D, NQ>::kCta
         constexpr uint32_t idS = idesc(128, 128, 0), idO = idesc(128, D, 1);
         uint32_t n = 0, np = 0, nw = 0;                // ring tiles used, p_full phases, pieces
         bool go = true;
-        auto slot = [&](uint32_t i) { return smem_u32(sKV + (i % kSlots) * kTileB); };
+        const uint32_t kv0 = desc_lo(smem_u32(sKV), kHalfB), q0 = desc_lo(smem_u32(sQ), kHalfB);
         auto wait_kv = [&](uint32_t i) {
             return warp_wait(&bars->kv_full[i % kSlots], (i / kSlots) & 1, bars, pv.status);
         };
         auto scores = [&](int q, uint32_t ik) {
-            if (lane == 0) {
-                const uint32_t qa = smem_u32(sQ + q * kTileB), ka = slot(ik);
+            const uint32_t qa = q0 + q * (kTileB >> 4), ka = kv0 + (ik % kSlots) * (kTileB >> 4);
+            if (elect()) {
 #pragma unroll
                 for (int kk = 0; kk < D / 16; ++kk) {
-                    const uint32_t off = (kk >> 2) * kHalfB + (kk & 3) * 32;
-                    mma_ss(tmem + Cfg::sCol(q), desc_k(qa + off), desc_k(ka + off), idS, kk > 0);
+                    const uint32_t off = ((kk >> 2) * kHalfB + (kk & 3) * 32) >> 4;
+                    mma_ss(tmem + Cfg::sCol(q), qa + off, ka + off, idS, kk > 0);
                 }
                 mma_commit(&bars->s_full[q]);
             }
             __syncwarp();
         };
         auto values = [&](int q, uint32_t iv, bool first) {
-            if (lane == 0) {
-                const uint32_t va = slot(iv);
+            const uint32_t va = kv0 + (iv % kSlots) * (kTileB >> 4);
+            if (elect()) {
 #pragma unroll
                 for (int kk = 0; kk < kBlk / 16; ++kk)
-                    mma_ts(tmem + Cfg::oCol(q), tmem + Cfg::sCol(q) + kk * 8, desc_mn(va + kk * 2048, kHalfB), idO,
-                           !first || kk > 0);
+                    mma_ts(tmem + Cfg::oCol(q), tmem + Cfg::sCol(q) + kk * 8, va + kk * (2048 >> 4), idO, !first || kk > 0);
                 mma_commit(&bars->o_full[q]);
             }
             __syncwarp();
         };
         auto release = [&](uint32_t i) {
-            if (lane == 0) mma_commit(&bars->kv_empty[i % kSlots]);
+            if (elect()) mma_commit(&bars->kv_empty[i % kSlots]);
             __syncwarp();
         };
         while (go) {
@@ -550,7 +555,7 @@ __global__ void __launch_bounds__(TileCfg<D, NQ>::kThreads, TileCfg<D, NQ>::kCta
                 break;
             }
             // ring: K of tile t at n + 2 t, V at n + 2 t + 1
-            const int plen = w->plen, olen = w->olen, tb0 = w->tb, nt = w->te - tb0;
+            const int plen = w->plen, olen = w->olen, tb0 = w->tb, nt = __shfl_sync(0xffffffffu, w->te - tb0, 0);
             go = wait_kv(n);
             for (int q = 0; q < NQ && go; ++q) {
                 go = warp_wait(&bars->q_full[q], nw & 1, bars, pv.status);
@@ -574,6 +579,7 @@ __global__ void __launch_bounds__(TileCfg<D, NQ>::kThreads, TileCfg<D, NQ>::kCta
                     __syncwarp();
                 }
                 const bool next = t + 1 < nt;
+#pragma unroll
                 for (int q = 0; q < NQ; ++q) {
                     if (!(go = warp_wait(&bars->p_full[q], np & 1, bars, pv.status))) break;
                     tc_after();
@@ -592,7 +598,7 @@ __global__ void __launch_bounds__(TileCfg<D, NQ>::kThreads, TileCfg<D, NQ>::kCta
             done(nw++);
         }
         if (!go) {                                     // gave up: products in flight end first
-            if (lane == 0) mma_commit(&bars->drain);
+            if (elect()) mma_commit(&bars->drain);
             __syncwarp();
             mbar_wait_bounded(&bars->drain, 0);
         }
