@@ -3,9 +3,9 @@
 // (extend), and the shared prefix of a group of sequences (decode).
 //
 // A unit's query rows (whole tokens, the G heads of a kv head side by side) lie
-// in NQ blocks of 128.  Per key tile of 128 keys and row block:
+// in NQ blocks of 128.  Per key tile and row block:
 //   S = Q K^T          tcgen05.mma, Q and K in shared memory, S fp32 in TMEM
-//   P = 2^(sc S - m)   one thread per row, S from TMEM, P (bf16) over S's columns
+//   P = 2^(sc S - m)   one thread per row, S from TMEM, P (bf16) to TMEM
 //   O += P V           tcgen05.mma with P from TMEM, O fp32 in TMEM
 // The running maximum m of a row is only moved when a tile exceeds it by more
 // than 2^kGrow: until then the weights are taken relative to the old one (they
@@ -13,12 +13,17 @@
 // times per unit instead of once per tile.  The result does not depend on m
 // beyond rounding: o = (sum 2^(x - m) v) / (sum 2^(x - m)).
 //
-// Warp roles: NQ softmax warpgroups (one row block each), a TMA warp (one
-// cp.async.bulk.tensor per page, or part of one, and 64 dimensions; K and V
-// tiles alternate in a ring of 128-key slots), an MMA warp, a warp that walks
-// the line ahead of them and leaves its pieces in shared memory.  With NQ = 2 the
-// MMA warp's order is P0 V, Q0 K', P1 V, Q1 K': each softmax works while the
-// tensor core does the other row block's products.
+// A softmax reads S into registers at once, so the next tile's S can be computed
+// while it works; P has columns of its own for that.  TMEM's 512 columns hold,
+// per row block, S (one column per key), P (half) and O (one per dimension): at
+// head_dim 128 that leaves room for 80 keys a tile, at 64 for 128.  With P over
+// S's columns and 128 keys a tile the products of a tile waited for its softmax
+// and the other way round: 943 TFLOP/s at 8192 tokens where this form has RATE.
+//
+// Warp roles: NQ softmax warpgroups (one row block each), a warp for each block's
+// products, a TMA warp (one cp.async.bulk.tensor for 16 rows and 64 dimensions;
+// K and V tiles alternate in a ring), a warp that walks the line ahead of them
+// and leaves its pieces in shared memory.
 // Work is the tile line of cbq_paged_line.cuh, one persistent CTA per part.
 // Every mbarrier wait is bounded; a wait that gives up sets CBQ_FLAG_TIMEOUT,
 // all roles stop at their next wait, and TMEM is released on the way out.
@@ -32,24 +37,28 @@ namespace {
 
 using namespace cbq;
 
-constexpr int kBlk = 128;              // rows of a block, keys of a tile
+constexpr int kBlk = 128;              // rows of a block
+constexpr int kBox = 16;               // rows of a copy; page_size is a multiple
 constexpr float kGrow = 8.f;           // log2 growth of a row's maximum that moves its reference
 
 template <int D, int NQ> struct TileCfg {
+    static constexpr int KT = D == 128 ? 80 : 128;                     // keys of a tile
     static constexpr int kHalves = D / 64;                             // 128-byte wide column blocks
-    static constexpr int kHalfB = kBlk * 128;                           // one of them: 16 KB
-    static constexpr int kTileB = kHalves * kHalfB;
-    static constexpr int kSlots = NQ == 2 ? (D == 128 ? 5 : 8) : (D == 128 ? 2 : 4);   // K / V tiles in flight
+    static constexpr int kQHalfB = kBlk * 128, kQB = kHalves * kQHalfB; // a row block of Q
+    static constexpr int kHalfB = KT * 128, kTileB = kHalves * kHalfB;  // a K or V tile
+    static constexpr int kSlots = NQ == 2 ? 8 : (D == 128 ? 3 : 4);     // K / V tiles in flight
     static constexpr int kSoft = NQ * 128;
-    static constexpr int kThreads = kSoft + 128;                       // + a warpgroup for the TMA and the MMA warp
+    static constexpr int kThreads = kSoft + 128;                       // + a warpgroup for the other roles
     // registers: the launch's share is split unevenly, kSoft * kSoftRegs + 128 * kRestRegs <= 65536 / kCtas
     static constexpr int kSoftRegs = NQ == 2 ? 208 : 200;
     static constexpr int kRestRegs = NQ == 2 ? 88 : 56;
     static constexpr int kCtas = NQ == 2 ? 1 : 2;                       // per SM: TMEM has 512 columns
     static constexpr int kCols = NQ == 2 ? 512 : 256;
-    static constexpr int kSmem = 1024 + (NQ + kSlots) * kTileB + 768;
-    static __host__ __device__ constexpr uint32_t sCol(int b) { return (uint32_t)b * 128u; }
-    static __host__ __device__ constexpr uint32_t oCol(int b) { return (uint32_t)NQ * 128u + (uint32_t)b * 128u; }
+    static constexpr int kSmem = 1024 + NQ * kQB + kSlots * kTileB + 768;
+    static __host__ __device__ constexpr uint32_t sCol(int b) { return (uint32_t)(b * (KT + KT / 2)); }
+    static __host__ __device__ constexpr uint32_t pCol(int b) { return sCol(b) + KT; }
+    static __host__ __device__ constexpr uint32_t oCol(int b) { return (uint32_t)(kCols - (NQ - b) * D); }
+    static_assert(NQ * (KT + KT / 2 + D) <= kCols, "TMEM columns");
 };
 
 // A piece of the line as the roles need it, written by the scheduling warp.
@@ -63,10 +72,10 @@ struct Work {
 constexpr int kWorks = 3;              // the piece in hand, the next one, one ahead
 
 struct Bars {
-    uint64_t q_full[2], s_full[2], p_full[2], o_full[2];
+    uint64_t q_full[2], s_full[2], s_free[2], p_full[2], o_full[2];
     uint64_t kv_full[8], kv_empty[8];
     uint64_t w_full[kWorks], w_empty[kWorks];
-    uint64_t drain;
+    uint64_t drain[2];
     uint32_t tmem;
     int abort_flag;
     Work work[kWorks];
@@ -127,12 +136,23 @@ __device__ __forceinline__ void tld32(uint32_t a, uint32_t *v) {
           "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
         : "r"(a));
 }
+__device__ __forceinline__ void tld16(uint32_t a, uint32_t *v) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
+          "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+        : "r"(a));
+}
 __device__ __forceinline__ void tld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tst16(uint32_t a, const uint32_t *v) {
     asm volatile(
         "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(a),
         "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
         "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]) : "memory");
+}
+__device__ __forceinline__ void tst8(uint32_t a, const uint32_t *v) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(a), "r"(v[0]), "r"(v[1]),
+                 "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]) : "memory");
 }
 __device__ __forceinline__ void tst32(uint32_t a, const uint32_t *v) {
     tst16(a, v);
@@ -156,17 +176,44 @@ __device__ __forceinline__ bool warp_wait(uint64_t *bar, uint32_t parity, Bars *
     return ok;
 }
 
-// A key tile: 128 rows of the prefix or of the own rows from row key0 of it.
+// Pairs of fp32 in one register pair: one instruction for both.
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float2 unpair(uint64_t v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+
+// A key tile: KT rows of the prefix or of the own rows from row key0 of it.
 struct TileAt {
     bool pre;
-    int key0, have;                    // rows of the tile that exist (0..128)
+    int key0, have;                    // rows of the tile that exist (0..KT)
 };
-__device__ __forceinline__ TileAt tile_at(int plen, int olen, int t) {
-    const int np = (plen + kBlk - 1) / kBlk;
+template <int KT> __device__ __forceinline__ TileAt tile_at(int plen, int olen, int t) {
+    const int np = (plen + KT - 1) / KT;
     TileAt x;
     x.pre = t < np;
-    x.key0 = (x.pre ? t : t - np) * kBlk;
-    x.have = clampi((x.pre ? plen : olen) - x.key0, 0, kBlk);
+    x.key0 = (x.pre ? t : t - np) * KT;
+    x.have = clampi((x.pre ? plen : olen) - x.key0, 0, KT);
     return x;
 }
 
@@ -246,30 +293,31 @@ __global__ void __launch_bounds__(TileCfg<D, NQ>::kThreads, TileCfg<D, NQ>::kCta
     k_paged_tile(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const PagedView pv,
                  const LineArgs a) {
     using Cfg = TileCfg<D, NQ>;
-    constexpr int kSlots = Cfg::kSlots, kTileB = Cfg::kTileB, kHalfB = Cfg::kHalfB;
+    constexpr int kSlots = Cfg::kSlots, kTileB = Cfg::kTileB, kHalfB = Cfg::kHalfB, KT = Cfg::KT;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-    uint8_t *sQ = smem, *sKV = smem + NQ * kTileB;
+    uint8_t *sQ = smem, *sKV = smem + NQ * Cfg::kQB;
     Bars *bars = reinterpret_cast<Bars *>(sKV + kSlots * kTileB);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    constexpr int kTmaWarp = Cfg::kSoft / 32, kMmaWarp = kTmaWarp + 1, kWorkWarp = kTmaWarp + 2;
+    constexpr int kTmaWarp = Cfg::kSoft / 32, kWorkWarp = kTmaWarp + 1, kMmaWarp = kTmaWarp + 2;   // kMmaWarp + block
 
     if (tid == 0) {
         for (int q = 0; q < NQ; ++q) {
             mbar_init(&bars->q_full[q], 128);
             mbar_init(&bars->s_full[q], 1);
+            mbar_init(&bars->s_free[q], 128);
             mbar_init(&bars->p_full[q], 128);
             mbar_init(&bars->o_full[q], 1);
         }
         for (int s = 0; s < kSlots; ++s) {
             mbar_init(&bars->kv_full[s], 1);
-            mbar_init(&bars->kv_empty[s], 1);
+            mbar_init(&bars->kv_empty[s], NQ);
         }
         for (int i = 0; i < kWorks; ++i) {
             mbar_init(&bars->w_full[i], 1);
-            mbar_init(&bars->w_empty[i], kWorkWarp);  // one arrival of every other warp
+            mbar_init(&bars->w_empty[i], kTmaWarp + 1 + NQ);   // one arrival of every warp that reads it
         }
-        mbar_init(&bars->drain, 1);
+        for (int q = 0; q < NQ; ++q) mbar_init(&bars->drain[q], 1);
         bars->abort_flag = 0;
         mbar_fence_init();
     }
@@ -306,7 +354,7 @@ __global__ void __launch_bounds__(TileCfg<D, NQ>::kThreads, TileCfg<D, NQ>::kCta
         // ------------------------------------------- softmax and output: thread = row
         const int q = warp >> 2, r = tid & 127;
         const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
-        const uint32_t tS = lanes + Cfg::sCol(q), tO = lanes + Cfg::oCol(q);
+        const uint32_t tS = lanes + Cfg::sCol(q), tP = lanes + Cfg::pCol(q), tO = lanes + Cfg::oCol(q);
         const int rt = r / a.geo.G, rg = r - rt * a.geo.G;            // the row's token in the block, head in the group
         // a negative scale turns Q's sign at its load, zero its value: sc > 0 below
         const float sc = a.sc == 0.f ? 1.f : fabsf(a.sc);
@@ -314,7 +362,7 @@ __global__ void __launch_bounds__(TileCfg<D, NQ>::kThreads, TileCfg<D, NQ>::kCta
         const uint32_t ginv = (65536u + a.geo.G - 1) / a.geo.G;       // x / G = x * ginv >> 16 for x < 128
         // the block's rows of a piece into shared memory (128-byte swizzle)
         auto load_q = [&](const Work *w) {
-            uint8_t *dst = sQ + q * kTileB;
+            uint8_t *dst = sQ + q * Cfg::kQB;
             const int tok0 = w->tok + q * tb, left = min(tb, w->nt - tok0), t0 = w->t0 + tok0, h0 = w->h * a.geo.G;
             constexpr int CH = D / 8;
             uint4 v[CH];                               // all loads first
@@ -330,13 +378,13 @@ __global__ void __launch_bounds__(TileCfg<D, NQ>::kThreads, TileCfg<D, NQ>::kCta
 #pragma unroll
             for (int i = 0; i < CH; ++i) {
                 const int e = i * 128 + r, row = e / CH, ch = e - row * CH;
-                *reinterpret_cast<uint4 *>(dst + (ch >> 3) * kHalfB + row * 128 + (((ch & 7) ^ (row & 7)) << 4)) =
+                *reinterpret_cast<uint4 *>(dst + (ch >> 3) * Cfg::kQHalfB + row * 128 + (((ch & 7) ^ (row & 7)) << 4)) =
                     make_uint4((v[i].x ^ sign) & keep, (v[i].y ^ sign) & keep, (v[i].z ^ sign) & keep, (v[i].w ^ sign) & keep);
             }
             fence_proxy_async_smem();
             mbar_arrive(&bars->q_full[q]);
         };
-        uint32_t nw = 0, ns = 0;                       // pieces; tiles seen (phases of s_full and o_full)
+        uint32_t nw = 0, ns = 0;                       // pieces; tiles seen (phases of s_full, p_full and o_full)
         const Work *w = work(0);
         if (w) load_q(w);
         bool go = true;
@@ -349,31 +397,50 @@ __global__ void __launch_bounds__(TileCfg<D, NQ>::kThreads, TileCfg<D, NQ>::kCta
             for (int t = t0; t < t1; ++t, ++ns) {
                 if (!warp_wait(&bars->s_full[q], ns & 1, bars, pv.status)) { go = false; break; }
                 tc_after();
-                uint32_t s[128];
+                uint32_t s[KT];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) tld32(tS + i * 32, s + i * 32);
+                for (int i = 0; i + 32 <= KT; i += 32) tld32(tS + i, s + i);
+                if constexpr (KT % 32) tld16(tS + KT / 32 * 32, s + KT / 32 * 32);
                 tld_wait();
-                const TileAt x = tile_at(plen, olen, t);
+                tc_before();
+                mbar_arrive(&bars->s_free[q]);         // the next tile's S may come
+                const TileAt x = tile_at<KT>(plen, olen, t);
                 const int vis = x.pre ? x.have : min(x.have, olim - x.key0);   // visible keys of the tile
-                if (__any_sync(0xffffffffu, vis < kBlk)) {
+                if (__any_sync(0xffffffffu, vis < KT)) {
 #pragma unroll
-                    for (int j = 0; j < 128; ++j)
+                    for (int j = 0; j < KT; ++j)
                         if (j >= vis) s[j] = 0xff800000u;                      // -inf
                 }
-                float mx[4] = {__uint_as_float(s[0]), __uint_as_float(s[1]), __uint_as_float(s[2]), __uint_as_float(s[3])};
+                float mx[4];
 #pragma unroll
-                for (int j = 4; j < 128; j += 4)
+                for (int e = 0; e < 4; ++e) mx[e] = fmaxf(__uint_as_float(s[e]), __uint_as_float(s[e + 4]));
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) mx[e] = fmaxf(mx[e], __uint_as_float(s[j + e]));
+                for (int j = 8; j < KT; j += 8)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        mx[e] = max3(mx[e], __uint_as_float(s[j + e]), __uint_as_float(s[j + e + 4]));
                 const float mn = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
                 const bool grow = (mn - m) * sc > kGrow;                       // false where both are -inf
-                if (__any_sync(0xffffffffu, grow)) {
-                    const float f = grow ? ex2((m - mn) * sc) : 1.f;           // 0 from -inf
-                    if (grow) m = mn;
-                    l *= f;
-                    if (t > t0) {
-                        // O holds the tiles before: wait for the last of them, scale it
-                        if (!warp_wait(&bars->o_full[q], (ns - 1) & 1, bars, pv.status)) { go = false; break; }
+                const float f = grow ? ex2((m - mn) * sc) : 1.f;               // 0 from -inf
+                if (grow) m = mn;
+                const float mb = m == -INFINITY ? 0.f : m * sc;
+                const uint64_t sc2 = pair(sc, sc), mb2 = pair(-mb, -mb);
+                uint64_t ls[2] = {0ull, 0ull};
+                uint32_t pk[KT / 2];
+#pragma unroll
+                for (int j = 0; j < KT / 2; ++j) {
+                    float2 e = unpair(fma2(pair(__uint_as_float(s[2 * j]), __uint_as_float(s[2 * j + 1])), sc2, mb2));
+                    e.x = ex2(e.x);
+                    e.y = ex2(e.y);
+                    ls[j & 1] = add2(ls[j & 1], pair(e.x, e.y));
+                    pk[j] = pack_bf16(e.x, e.y);
+                }
+                const float2 lp = unpair(add2(ls[0], ls[1]));
+                l = l * f + (lp.x + lp.y);
+                if (t > t0) {
+                    // the products with the last P are done: P may be written, O scaled
+                    if (!warp_wait(&bars->o_full[q], (ns - 1) & 1, bars, pv.status)) { go = false; break; }
+                    if (__any_sync(0xffffffffu, grow)) {
                         tc_after();
 #pragma unroll 1
                         for (int i = 0; i < D; i += 32) {
@@ -386,22 +453,9 @@ __global__ void __launch_bounds__(TileCfg<D, NQ>::kThreads, TileCfg<D, NQ>::kCta
                         }
                     }
                 }
-                const float mb = m == -INFINITY ? 0.f : m * sc;
-                float ls[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    uint32_t pk[16];
-#pragma unroll
-                    for (int j = 0; j < 16; ++j) {
-                        const float p0 = ex2(fmaf(__uint_as_float(s[i * 32 + 2 * j]), sc, -mb));
-                        const float p1 = ex2(fmaf(__uint_as_float(s[i * 32 + 2 * j + 1]), sc, -mb));
-                        ls[(2 * j) & 3] += p0;
-                        ls[(2 * j + 1) & 3] += p1;
-                        pk[j] = pack_bf16(p0, p1);
-                    }
-                    tst16(tS + i * 16, pk);
-                }
-                l += (ls[0] + ls[1]) + (ls[2] + ls[3]);
+                for (int i = 0; i + 16 <= KT / 2; i += 16) tst16(tP + i, pk + i);
+                if constexpr (KT / 2 % 16) tst8(tP + KT / 32 * 16, pk + KT / 32 * 16);
                 tst_wait();
                 tc_before();
                 mbar_arrive(&bars->p_full[q]);
@@ -472,18 +526,18 @@ __global__ void __launch_bounds__(TileCfg<D, NQ>::kThreads, TileCfg<D, NQ>::kCta
         // ------------------------------------------------------------- K and V tiles
         uint32_t n = 0, nw = 0;                        // tiles issued (K and V), pieces
         bool go = true;
-        const int ps = 1 << pv.ps_shift, box = min(ps, kBlk);
+        const int ps = 1 << pv.ps_shift;
         while (go) {
             const Work *w = work(nw);
             if (!w) break;
             const int plen = w->plen, olen = w->olen, h = w->h, o = w->o, t1 = w->te;
             const int32_t *ptab = pv.ptable + w->group * pv.ptable_stride, *otab = pv.table + o * pv.table_stride;
             for (int t = w->tb; t < t1 && go; ++t) {
-                const TileAt x = tile_at(plen, olen, t);
-                const int nbox = (x.have + box - 1) / box;
+                const TileAt x = tile_at<KT>(plen, olen, t);
+                const int nbox = (x.have + kBox - 1) / kBox;
                 // lane: one box of rows and 64 dimensions
                 const int bx = lane / Cfg::kHalves, hf = lane - bx * Cfg::kHalves;
-                const int key = x.key0 + bx * box;
+                const int key = x.key0 + bx * kBox;
                 int page = 0;
                 if (bx < nbox) {
                     page = __ldg((x.pre ? ptab : otab) + (key >> pv.ps_shift));
@@ -499,10 +553,10 @@ __global__ void __launch_bounds__(TileCfg<D, NQ>::kThreads, TileCfg<D, NQ>::kCta
                         go = false;
                         break;
                     }
-                    if (lane == 0) mbar_arrive_expect_tx(&bars->kv_full[s], (uint32_t)(nbox * box * D * 2));
+                    if (lane == 0) mbar_arrive_expect_tx(&bars->kv_full[s], (uint32_t)(nbox * kBox * D * 2));
                     __syncwarp();
                     if (bx < nbox)
-                        tma_4d(smem_u32(sKV + s * kTileB + hf * kHalfB + bx * box * 128), kv ? &vmap : &kmap, hf * 64,
+                        tma_4d(smem_u32(sKV + s * kTileB + hf * kHalfB + bx * kBox * 128), kv ? &vmap : &kmap, hf * 64,
                                key & (ps - 1), h, page, &bars->kv_full[s]);
                 }
             }
@@ -513,40 +567,33 @@ __global__ void __launch_bounds__(TileCfg<D, NQ>::kThreads, TileCfg<D, NQ>::kCta
             const uint32_t last = n - 1 - (n - 1 - s) % kSlots;
             mbar_wait_bounded(&bars->kv_full[s], (last / kSlots) & 1);
         }
-    } else if (warp == kMmaWarp) {
-        // ------------------------------------------------------------------ products
-        constexpr uint32_t idS = idesc(128, 128, 0), idO = idesc(128, D, 1);
-        uint32_t n = 0, np = 0, nw = 0;                // ring tiles used, p_full phases, pieces
+    } else if (warp >= kMmaWarp && warp < kMmaWarp + NQ) {
+        // ------------------------------------------------------------------ products of block q
+        const int q = warp - kMmaWarp;
+        constexpr uint32_t idS = idesc(128, KT, 0), idO = idesc(128, D, 1);
+        uint32_t n = 0, ns = 0, nw = 0;                // ring tiles used, tiles of S, pieces
         bool go = true;
-        const uint32_t kv0 = desc_lo(smem_u32(sKV), kHalfB), q0 = desc_lo(smem_u32(sQ), kHalfB);
+        const uint32_t kv0 = desc_lo(smem_u32(sKV), kHalfB), q0 = desc_lo(smem_u32(sQ + q * Cfg::kQB), kHalfB);
+        const uint32_t tS = tmem + Cfg::sCol(q), tP = tmem + Cfg::pCol(q), tO = tmem + Cfg::oCol(q);
         auto wait_kv = [&](uint32_t i) {
             return warp_wait(&bars->kv_full[i % kSlots], (i / kSlots) & 1, bars, pv.status);
         };
-        auto scores = [&](int q, uint32_t ik) {
-            const uint32_t qa = q0 + q * (kTileB >> 4), ka = kv0 + (ik % kSlots) * (kTileB >> 4);
+        // S of the tile whose K is the ring's i-th, once the S before it has been read
+        auto scores = [&](uint32_t i) {
+            if (!wait_kv(i) || (ns && !warp_wait(&bars->s_free[q], (ns - 1) & 1, bars, pv.status))) return false;
+            tc_after();
+            const uint32_t ka = kv0 + (i % kSlots) * (kTileB >> 4);
             if (elect()) {
 #pragma unroll
-                for (int kk = 0; kk < D / 16; ++kk) {
-                    const uint32_t off = ((kk >> 2) * kHalfB + (kk & 3) * 32) >> 4;
-                    mma_ss(tmem + Cfg::sCol(q), qa + off, ka + off, idS, kk > 0);
-                }
+                for (int kk = 0; kk < D / 16; ++kk)
+                    mma_ss(tS, q0 + (((kk >> 2) * Cfg::kQHalfB + (kk & 3) * 32) >> 4),
+                           ka + (((kk >> 2) * kHalfB + (kk & 3) * 32) >> 4), idS, kk > 0);
                 mma_commit(&bars->s_full[q]);
+                mma_commit(&bars->kv_empty[i % kSlots]);
             }
             __syncwarp();
-        };
-        auto values = [&](int q, uint32_t iv, bool first) {
-            const uint32_t va = kv0 + (iv % kSlots) * (kTileB >> 4);
-            if (elect()) {
-#pragma unroll
-                for (int kk = 0; kk < kBlk / 16; ++kk)
-                    mma_ts(tmem + Cfg::oCol(q), tmem + Cfg::sCol(q) + kk * 8, va + kk * (2048 >> 4), idO, !first || kk > 0);
-                mma_commit(&bars->o_full[q]);
-            }
-            __syncwarp();
-        };
-        auto release = [&](uint32_t i) {
-            if (elect()) mma_commit(&bars->kv_empty[i % kSlots]);
-            __syncwarp();
+            ++ns;
+            return true;
         };
         while (go) {
             const Work *w = work(nw);
@@ -556,21 +603,16 @@ __global__ void __launch_bounds__(TileCfg<D, NQ>::kThreads, TileCfg<D, NQ>::kCta
             }
             // ring: K of tile t at n + 2 t, V at n + 2 t + 1
             const int plen = w->plen, olen = w->olen, tb0 = w->tb, nt = __shfl_sync(0xffffffffu, w->te - tb0, 0);
-            go = wait_kv(n);
-            for (int q = 0; q < NQ && go; ++q) {
-                go = warp_wait(&bars->q_full[q], nw & 1, bars, pv.status);
-                tc_after();
-                if (go) scores(q, n);
-            }
-            if (!go) break;
-            release(n);
-            for (int t = 0; t < nt; ++t, ++np) {
+            go = warp_wait(&bars->q_full[q], nw & 1, bars, pv.status) && scores(n);
+            for (int t = 0; t < nt && go; ++t) {
                 const uint32_t iv = n + 2 * t + 1;
+                if (t + 1 < nt && !(go = scores(iv + 1))) break;
                 if (!(go = wait_kv(iv))) break;
-                const TileAt x = tile_at(plen, olen, tb0 + t);
-                if (x.have < kBlk) {
-                    // rows that do not exist (rest of a page, pages not copied) must not meet a weight of 0
-                    for (int e = x.have * 8 + lane; e < kBlk * 8; e += 32)
+                const TileAt x = tile_at<KT>(plen, olen, tb0 + t);
+                if (x.have < KT) {
+                    // rows that do not exist (rest of a page, pages not copied) must not meet a weight
+                    // of 0; both blocks' warps clear them, each before its own product
+                    for (int e = x.have * 8 + lane; e < KT * 8; e += 32)
 #pragma unroll
                         for (int hf = 0; hf < Cfg::kHalves; ++hf)
                             *reinterpret_cast<uint4 *>(sKV + (iv % kSlots) * kTileB + hf * kHalfB + e * 16) =
@@ -578,29 +620,26 @@ __global__ void __launch_bounds__(TileCfg<D, NQ>::kThreads, TileCfg<D, NQ>::kCta
                     fence_proxy_async_smem();
                     __syncwarp();
                 }
-                const bool next = t + 1 < nt;
+                if (!(go = warp_wait(&bars->p_full[q], (ns - (t + 1 < nt ? 2 : 1)) & 1, bars, pv.status))) break;
+                tc_after();
+                const uint32_t va = kv0 + (iv % kSlots) * (kTileB >> 4);
+                if (elect()) {
 #pragma unroll
-                for (int q = 0; q < NQ; ++q) {
-                    if (!(go = warp_wait(&bars->p_full[q], np & 1, bars, pv.status))) break;
-                    tc_after();
-                    values(q, iv, t == 0);
-                    if (next) {
-                        if (q == 0 && !(go = wait_kv(iv + 1))) break;
-                        scores(q, iv + 1);
-                    }
+                    for (int kk = 0; kk < KT / 16; ++kk)
+                        mma_ts(tO, tP + kk * 8, va + kk * (2048 >> 4), idO, t > 0 || kk > 0);
+                    mma_commit(&bars->o_full[q]);
+                    mma_commit(&bars->kv_empty[iv % kSlots]);
                 }
-                if (!go) break;
-                release(iv);
-                if (next) release(iv + 1);
+                __syncwarp();
             }
             if (!go) break;
             n += 2 * nt;
             done(nw++);
         }
         if (!go) {                                     // gave up: products in flight end first
-            if (elect()) mma_commit(&bars->drain);
+            if (elect()) mma_commit(&bars->drain[q]);
             __syncwarp();
-            mbar_wait_bounded(&bars->drain, 0);
+            mbar_wait_bounded(&bars->drain[q], 0);
         }
     } else if (warp == kWorkWarp) {
         // -------------------------------------------------------------- the line ahead
@@ -651,7 +690,7 @@ EncodeFn encoder() {
     return fn;
 }
 
-// The pool as {dimension, row, head, page}; a box is a page's rows (at most 128) by 64 dimensions.
+// The pool as {dimension, row, head, page}; a box is 16 rows by 64 dimensions.
 bool pool_map(const cbq_paged_cache *c, void *pool, CUtensorMap *map) {
     EncodeFn enc = encoder();
     if (!enc) return false;
@@ -659,7 +698,7 @@ bool pool_map(const cbq_paged_cache *c, void *pool, CUtensorMap *map) {
                                 (cuuint64_t)c->pages};
     const cuuint64_t strides[3] = {(cuuint64_t)c->row_stride * 2, (cuuint64_t)c->head_stride * 2,
                                    (cuuint64_t)c->page_stride * 2};
-    const cuuint32_t box[4] = {64, (cuuint32_t)std::min<int64_t>(c->page_size, kBlk), 1, 1}, es[4] = {1, 1, 1, 1};
+    const cuuint32_t box[4] = {64, kBox, 1, 1}, es[4] = {1, 1, 1, 1};
     return enc(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, pool, dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
                CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) ==
            CUDA_SUCCESS;
@@ -703,7 +742,7 @@ int tile_plan(const cbq::PagedView &pv, int d, int G, int mode, bool two, int64_
     p->geo.G = G;
     p->geo.tq = nq * (kBlk / G);
     p->geo.hc = 1;
-    p->geo.keys = kBlk;
+    p->geo.keys = d == 64 ? TileCfg<64, 1>::KT : TileCfg<128, 1>::KT;
     p->geo.join = 0;
     p->min_tiles = 2;                  // a part costs its CTA about as much as a tile
     p->grid = n * sm_count();
