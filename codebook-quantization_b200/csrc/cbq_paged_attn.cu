@@ -782,7 +782,7 @@ int paged_attn(const cbq_paged_cache *c, const cbq_paged_batch *b, int64_t token
     if (b->seqs == 0) return CBQ_ERR_ARG;
     const int64_t unit = c->dtype == CBQ_BF16 ? 8 : 4;
     if (!q || !out || !ws || ws_bytes < p.bytes || q_stride < q_heads * c->head_dim || q_stride % unit) return CBQ_ERR_ARG;
-    if ((reinterpret_cast<uintptr_t>(q) & 15) || (reinterpret_cast<uintptr_t>(out) & 15) ||
+    if ((reinterpret_cast<uintptr_t>(q) & 15) || (reinterpret_cast<uintptr_t>(out) & 31) ||
         (reinterpret_cast<uintptr_t>(ws) & 255))
         return CBQ_ERR_ARG;
     uint8_t *w = static_cast<uint8_t *>(ws);

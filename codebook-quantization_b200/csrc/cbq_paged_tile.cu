@@ -30,6 +30,7 @@
 #include <cuda.h>
 
 #include <mutex>
+#include <type_traits>
 
 #include "cbq_paged_line.cuh"
 
@@ -40,6 +41,8 @@ using namespace cbq;
 constexpr int kBlk = 128;              // rows of a block
 constexpr int kBox = 16;               // rows of a copy; page_size is a multiple
 constexpr float kGrow = 8.f;           // log2 growth of a row's maximum that moves its reference
+
+constexpr int kPoly = 0;               // of 16 weights, computed on the FMA pipe
 
 template <int D, int NQ> struct TileCfg {
     static constexpr int KT = D == 128 ? 80 : 128;                     // keys of a tile
@@ -72,7 +75,7 @@ struct Work {
 constexpr int kWorks = 3;              // the piece in hand, the next one, one ahead
 
 struct Bars {
-    uint64_t q_full[2], s_full[2], s_free[2], p_full[2], o_full[2];
+    uint64_t q_full[2], q_free[2], s_full[2], s_free[2], p_full[2], o_full[2];
     uint64_t kv_full[8], kv_empty[8];
     uint64_t w_full[kWorks], w_empty[kWorks];
     uint64_t drain[2];
@@ -120,6 +123,16 @@ __device__ __forceinline__ void mma_commit(uint64_t *bar) {
 }
 __device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tma_3d(uint32_t dst, const CUtensorMap *map, int c0, int c1, int c2, uint64_t *bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+        ::"r"(dst), "l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(smem_u32(bar)) : "memory");
+}
+// 32 bytes in one store: a whole sector of each lane's row
+__device__ __forceinline__ void st32b(void *p, const uint32_t *v) {
+    asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]),
+                 "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]) : "memory");
+}
 __device__ __forceinline__ void tma_4d(uint32_t dst, const CUtensorMap *map, int c0, int c1, int c2, int c3, uint64_t *bar) {
     asm volatile(
         "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
@@ -160,6 +173,13 @@ __device__ __forceinline__ void tst32(uint32_t a, const uint32_t *v) {
 }
 __device__ __forceinline__ void tst_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+__device__ __forceinline__ bool mbar_test(uint64_t *bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                 : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity) : "memory");
+    return ok != 0;
+}
+
 // Bounded wait of a whole warp; false (for all its lanes) once the CTA has
 // given up.  The waits of the pipeline end within microseconds: they suspend on
 // the barrier and only then look at the clock, whose read is slow.
@@ -176,26 +196,18 @@ __device__ __forceinline__ bool warp_wait(uint64_t *bar, uint32_t parity, Bars *
     return ok;
 }
 
-// Pairs of fp32 in one register pair: one instruction for both.
-__device__ __forceinline__ uint64_t pair(float a, float b) {
-    uint64_t r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-    return r;
-}
-__device__ __forceinline__ float2 unpair(uint64_t v) {
-    float2 r;
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
-    return r;
-}
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-    uint64_t r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-    return r;
-}
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-    uint64_t r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
+// 2^x, x <= kGrow, on the FMA pipe (the special-function pipe's 16
+// results a cycle and SM are as many as a tile's products take): x = n + f with
+// n the nearest integer (adding 1.5 * 2^23 leaves it in the low mantissa bits),
+// a cubic for 2^f on [-1/2, 1/2] fitted to the least relative error, n added to
+// the exponent.  Relative error 7.5e-5, a twenty-fifth of the rounding to bf16
+// that follows; the sum of the weights takes the same values.
+constexpr float kC0 = 0.99992806f, kC1 = 0.69326097f, kC2 = 0.24261114f, kC3 = 0.05517167f;
+__device__ __forceinline__ float ex2_fma(float x) {
+    x = fmaxf(x, -126.f);
+    const float t = x + 12582912.f, f = x - (t - 12582912.f);
+    const float y = fmaf(f, fmaf(f, fmaf(f, kC3, kC2), kC1), kC0);
+    return __uint_as_float(__float_as_uint(y) + (__float_as_uint(t) << 23));
 }
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float r;
@@ -208,8 +220,7 @@ struct TileAt {
     bool pre;
     int key0, have;                    // rows of the tile that exist (0..KT)
 };
-template <int KT> __device__ __forceinline__ TileAt tile_at(int plen, int olen, int t) {
-    const int np = (plen + KT - 1) / KT;
+template <int KT> __device__ __forceinline__ TileAt tile_at(int plen, int olen, int np, int t) {   // np: tiles of the prefix
     TileAt x;
     x.pre = t < np;
     x.key0 = (x.pre ? t : t - np) * KT;
@@ -217,71 +228,48 @@ template <int KT> __device__ __forceinline__ TileAt tile_at(int plen, int olen, 
     return x;
 }
 
-// A warp joins its 32 rows of a cut unit: lane l holds row `row`'s weights,
-// eight rows at a time take their parts with the row's 512 (256) bytes side by
-// side over the lanes.
+// 32 dimensions of a row of the output.
+__device__ __forceinline__ void store_row(__nv_bfloat16 *dst, const uint32_t *o, float f) {
+#pragma unroll
+    for (int j = 0; j < 32; j += 16) {
+        uint32_t w[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            w[e] = pack_bf16(__uint_as_float(o[j + 2 * e]) * f, __uint_as_float(o[j + 2 * e + 1]) * f);
+        st32b(dst + j, w);
+    }
+}
+
+// A warp joins its 32 rows of a cut unit (parts dimension by dimension), a
+// lane its row `row`.
 template <int D, int NQ>
-__device__ __forceinline__ void join_block(const LineArgs &a, const Cut &cut, int row, bool live, int64_t orow) {
-    constexpr int RR = NQ * kBlk, E = D / 32;
+__device__ __forceinline__ void join_block(const LineArgs &a, const Cut &cut, int row, bool live, __nv_bfloat16 *dst) {
+    constexpr int RR = NQ * kBlk;
     constexpr int64_t SL = (int64_t)RR * (D + 2);
-    const int lane = threadIdx.x & 31, row0 = row - lane;
     float M = -INFINITY, L = 0.f;
-    if (live) {
-        for (int k = 0; k < cut.n; ++k) M = fmaxf(M, __ldcg(cut.slot(a, k, SL) + RR * D + row));
-        for (int k = 0; k < cut.n; ++k) {
-            const float *b = cut.slot(a, k, SL) + RR * D + row;
-            const float m = __ldcg(b);
-            if (m != -INFINITY) L = fmaf(__ldcg(b + RR), ex2(m - M), L);
-        }
+    for (int k = 0; k < cut.n; ++k) M = fmaxf(M, __ldcg(cut.slot(a, k, SL) + RR * D + row));
+    for (int k = 0; k < cut.n; ++k) {
+        const float *b = cut.slot(a, k, SL) + RR * D + row;
+        const float m = __ldcg(b);
+        if (m != -INFINITY) L = fmaf(__ldcg(b + RR), ex2(m - M), L);
     }
     const float inv = L == 0.f ? 0.f : 1.f / L;
-    const unsigned who = __ballot_sync(0xffffffffu, live);
-    __nv_bfloat16 *out = static_cast<__nv_bfloat16 *>(a.out);
-    for (int j0 = 0; j0 < 32; j0 += 8) {
-        if (!(who >> j0 & 0xffu)) continue;
-        float y[8][E];
+#pragma unroll 1
+    for (int i = 0; i < D; i += 32) {
+        uint32_t y[32];
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-#pragma unroll
-            for (int e = 0; e < E; ++e) y[j][e] = 0.f;
+        for (int j = 0; j < 32; ++j) y[j] = 0u;
         for (int k = 0; k < cut.n; ++k) {
             const float *s = cut.slot(a, k, SL);
-            float f = 0.f;
-            if (live) {
-                const float m = __ldcg(s + RR * D + row);
-                f = m == -INFINITY ? 0.f : ex2(m - M) * inv;
-            }
-            float v[8][E];
+            const float m = __ldcg(s + RR * D + row), f = m == -INFINITY ? 0.f : ex2(m - M);
+            float v[32];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const float *b = s + (int64_t)(row0 + j0 + j) * D + lane * E;
-                if (who >> (j0 + j) & 1u) {
-                    if constexpr (E == 4) {
-                        const float4 x = __ldcg(reinterpret_cast<const float4 *>(b));
-                        v[j][0] = x.x; v[j][1] = x.y; v[j][2] = x.z; v[j][3] = x.w;
-                    } else {
-                        const float2 x = __ldcg(reinterpret_cast<const float2 *>(b));
-                        v[j][0] = x.x; v[j][1] = x.y;
-                    }
-                } else {
+            for (int j = 0; j < 32; ++j) v[j] = __ldcg(s + (int64_t)(i + j) * RR + row);
 #pragma unroll
-                    for (int e = 0; e < E; ++e) v[j][e] = 0.f;
-                }
-            }
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const float fj = __shfl_sync(0xffffffffu, f, j0 + j);
-#pragma unroll
-                for (int e = 0; e < E; ++e) y[j][e] = fmaf(v[j][e], fj, y[j][e]);
-            }
+            for (int j = 0; j < 32; ++j) y[j] = __float_as_uint(fmaf(v[j], f, __uint_as_float(y[j])));
         }
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const int64_t at = __shfl_sync(0xffffffffu, orow, j0 + j) * D + lane * E;
-            if (!(who >> (j0 + j) & 1u)) continue;
-            if constexpr (E == 4) st4(out + at, y[j][0], y[j][1], y[j][2], y[j][3]);
-            else *reinterpret_cast<uint32_t *>(out + at) = pack_bf16(y[j][0], y[j][1]);
-        }
+        if (live) store_row(dst + i, y, inv);
+        __syncwarp();
     }
 }
 
@@ -290,8 +278,8 @@ template <int N> __device__ __forceinline__ void regs_down() { asm volatile("set
 
 template <int D, int NQ>
 __global__ void __launch_bounds__(TileCfg<D, NQ>::kThreads, TileCfg<D, NQ>::kCtas)
-    k_paged_tile(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const PagedView pv,
-                 const LineArgs a) {
+    k_paged_tile(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
+                 const __grid_constant__ CUtensorMap qmap, const PagedView pv, const LineArgs a) {
     using Cfg = TileCfg<D, NQ>;
     constexpr int kSlots = Cfg::kSlots, kTileB = Cfg::kTileB, kHalfB = Cfg::kHalfB, KT = Cfg::KT;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -303,7 +291,8 @@ __global__ void __launch_bounds__(TileCfg<D, NQ>::kThreads, TileCfg<D, NQ>::kCta
 
     if (tid == 0) {
         for (int q = 0; q < NQ; ++q) {
-            mbar_init(&bars->q_full[q], 128);
+            mbar_init(&bars->q_full[q], 1);
+            mbar_init(&bars->q_free[q], 1);
             mbar_init(&bars->s_full[q], 1);
             mbar_init(&bars->s_free[q], 128);
             mbar_init(&bars->p_full[q], 128);
@@ -356,46 +345,23 @@ __global__ void __launch_bounds__(TileCfg<D, NQ>::kThreads, TileCfg<D, NQ>::kCta
         const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
         const uint32_t tS = lanes + Cfg::sCol(q), tP = lanes + Cfg::pCol(q), tO = lanes + Cfg::oCol(q);
         const int rt = r / a.geo.G, rg = r - rt * a.geo.G;            // the row's token in the block, head in the group
-        // a negative scale turns Q's sign at its load, zero its value: sc > 0 below
-        const float sc = a.sc == 0.f ? 1.f : fabsf(a.sc);
-        const uint32_t sign = a.sc < 0.f ? 0x80008000u : 0u, keep = a.sc == 0.f ? 0u : 0xffffffffu;
-        const uint32_t ginv = (65536u + a.geo.G - 1) / a.geo.G;       // x / G = x * ginv >> 16 for x < 128
-        // the block's rows of a piece into shared memory (128-byte swizzle)
-        auto load_q = [&](const Work *w) {
-            uint8_t *dst = sQ + q * Cfg::kQB;
-            const int tok0 = w->tok + q * tb, left = min(tb, w->nt - tok0), t0 = w->t0 + tok0, h0 = w->h * a.geo.G;
-            constexpr int CH = D / 8;
-            uint4 v[CH];                               // all loads first
-#pragma unroll
-            for (int i = 0; i < CH; ++i) {
-                const int e = i * 128 + r, row = e / CH, ch = e - row * CH, tk = (int)((uint32_t)row * ginv >> 16);
-                v[i] = make_uint4(0u, 0u, 0u, 0u);
-                if (tk < left)
-                    v[i] = *reinterpret_cast<const uint4 *>(static_cast<const __nv_bfloat16 *>(a.q) +
-                                                            (int64_t)(t0 + tk) * a.qs +
-                                                            (int64_t)(h0 + row - tk * a.geo.G) * D + ch * 8);
-            }
-#pragma unroll
-            for (int i = 0; i < CH; ++i) {
-                const int e = i * 128 + r, row = e / CH, ch = e - row * CH;
-                *reinterpret_cast<uint4 *>(dst + (ch >> 3) * Cfg::kQHalfB + row * 128 + (((ch & 7) ^ (row & 7)) << 4)) =
-                    make_uint4((v[i].x ^ sign) & keep, (v[i].y ^ sign) & keep, (v[i].z ^ sign) & keep, (v[i].w ^ sign) & keep);
-            }
-            fence_proxy_async_smem();
-            mbar_arrive(&bars->q_full[q]);
-        };
+        // a scale below 0 turns S's sign, a scale of 0 clears it: sc > 0 below
+        const float sc = a.sc == 0.f ? 1.f : fabsf(a.sc), turn = a.sc == 0.f ? 0.f : -1.f;
         uint32_t nw = 0, ns = 0;                       // pieces; tiles seen (phases of s_full, p_full and o_full)
         const Work *w = work(0);
-        if (w) load_q(w);
         bool go = true;
         while (w) {
             const int tok = w->tok + q * tb + rt;
             const bool live = rt < tb && tok < w->nt;
-            const int plen = w->plen, olen = w->olen, t0 = w->tb, t1 = w->te;
+            const int plen = w->plen, olen = w->olen, np = (plen + KT - 1) / KT, t0 = w->tb, t1 = w->te;
             const int olim = a.mode == kPrefix ? 0 : clampi(olen - w->nt + tok + 1, 0, olen);
             float m = -INFINITY, l = 0.f;
+            bool early = false;                        // S of the tile was there before the last one's end
             for (int t = t0; t < t1; ++t, ++ns) {
-                if (!warp_wait(&bars->s_full[q], ns & 1, bars, pv.status)) { go = false; break; }
+                if (!__all_sync(0xffffffffu, early) && !warp_wait(&bars->s_full[q], ns & 1, bars, pv.status)) {
+                    go = false;
+                    break;
+                }
                 tc_after();
                 uint32_t s[KT];
 #pragma unroll
@@ -404,9 +370,16 @@ __global__ void __launch_bounds__(TileCfg<D, NQ>::kThreads, TileCfg<D, NQ>::kCta
                 tld_wait();
                 tc_before();
                 mbar_arrive(&bars->s_free[q]);         // the next tile's S may come
-                const TileAt x = tile_at<KT>(plen, olen, t);
+                if (a.sc <= 0.f) {
+#pragma unroll
+                    for (int j = 0; j < KT; ++j) s[j] = __float_as_uint(__uint_as_float(s[j]) * turn);
+                }
+                const TileAt x = tile_at<KT>(plen, olen, np, t);
                 const int vis = x.pre ? x.have : min(x.have, olim - x.key0);   // visible keys of the tile
-                if (__any_sync(0xffffffffu, vis < KT)) {
+                const bool edge = __any_sync(0xffffffffu, vis < KT);
+                // whether the products with the last P are done: asked here, needed after the weights
+                bool o_done = t > t0 && mbar_test(&bars->o_full[q], (ns - 1) & 1);
+                if (edge) {
 #pragma unroll
                     for (int j = 0; j < KT; ++j)
                         if (j >= vis) s[j] = 0xff800000u;                      // -inf
@@ -424,22 +397,30 @@ __global__ void __launch_bounds__(TileCfg<D, NQ>::kThreads, TileCfg<D, NQ>::kCta
                 const float f = grow ? ex2((m - mn) * sc) : 1.f;               // 0 from -inf
                 if (grow) m = mn;
                 const float mb = m == -INFINITY ? 0.f : m * sc;
-                const uint64_t sc2 = pair(sc, sc), mb2 = pair(-mb, -mb);
-                uint64_t ls[2] = {0ull, 0ull};
+                float ls[4] = {0.f, 0.f, 0.f, 0.f};
                 uint32_t pk[KT / 2];
+                // kPoly of 16 weights by polynomial (not where keys are hidden: their weight has to be 0)
+                auto weights = [&](auto poly) {
 #pragma unroll
-                for (int j = 0; j < KT / 2; ++j) {
-                    float2 e = unpair(fma2(pair(__uint_as_float(s[2 * j]), __uint_as_float(s[2 * j + 1])), sc2, mb2));
-                    e.x = ex2(e.x);
-                    e.y = ex2(e.y);
-                    ls[j & 1] = add2(ls[j & 1], pair(e.x, e.y));
-                    pk[j] = pack_bf16(e.x, e.y);
-                }
-                const float2 lp = unpair(add2(ls[0], ls[1]));
-                l = l * f + (lp.x + lp.y);
+                    for (int j = 0; j < KT; j += 2) {
+                        float e[2];
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            const float x = fmaf(__uint_as_float(s[j + i]), sc, -mb);
+                            e[i] = decltype(poly)::value && ((j + i) * kPoly) % 16 < kPoly ? ex2_fma(x) : ex2(x);
+                            ls[(j + i) & 3] += e[i];
+                        }
+                        pk[j / 2] = pack_bf16(e[0], e[1]);
+                    }
+                };
+                if (edge) weights(std::false_type{}); else weights(std::true_type{});
+                l = l * f + ((ls[0] + ls[1]) + (ls[2] + ls[3]));
                 if (t > t0) {
                     // the products with the last P are done: P may be written, O scaled
-                    if (!warp_wait(&bars->o_full[q], (ns - 1) & 1, bars, pv.status)) { go = false; break; }
+                    if (!__all_sync(0xffffffffu, o_done) && !warp_wait(&bars->o_full[q], (ns - 1) & 1, bars, pv.status)) {
+                        go = false;
+                        break;
+                    }
                     if (__any_sync(0xffffffffu, grow)) {
                         tc_after();
 #pragma unroll 1
@@ -456,45 +437,41 @@ __global__ void __launch_bounds__(TileCfg<D, NQ>::kThreads, TileCfg<D, NQ>::kCta
 #pragma unroll
                 for (int i = 0; i + 16 <= KT / 2; i += 16) tst16(tP + i, pk + i);
                 if constexpr (KT / 2 % 16) tst8(tP + KT / 32 * 16, pk + KT / 32 * 16);
+                early = t + 1 < t1 && mbar_test(&bars->s_full[q], (ns + 1) & 1);
                 tst_wait();
                 tc_before();
                 mbar_arrive(&bars->p_full[q]);
             }
             if (!go) break;
-            // the last S has been read, so every product with this Q is done
-            const Work *wn = work(nw + 1);
-            if (wn) load_q(wn);
             if (!warp_wait(&bars->o_full[q], (ns - 1) & 1, bars, pv.status)) { go = false; break; }
             tc_after();
             const float inv = l == 0.f ? 0.f : 1.f / l;
-            float *ps = a.part + w->slot * (int64_t)(NQ * kBlk * (D + 2));
             const bool fits = w->slot < a.slots, whole = w->whole;
-            const int64_t orow = (int64_t)(w->t0 + tok) * a.hq + w->h * a.geo.G + rg;
+            constexpr int64_t SL = (int64_t)NQ * kBlk * (D + 2);
+            float *ps = a.part + w->slot * SL;
+            __nv_bfloat16 *dst = static_cast<__nv_bfloat16 *>(a.out) +
+                                 ((int64_t)(w->t0 + tok) * a.hq + w->h * a.geo.G + rg) * D;
 #pragma unroll 1
             for (int i = 0; i < D; i += 32) {
                 uint32_t o[32];
                 tld32(tO + i, o);
                 tld_wait();
-                if (!live) {
-                } else if (whole) {
-                    __nv_bfloat16 *dst = static_cast<__nv_bfloat16 *>(a.out) + orow * D + i;
+                if (whole) {
+                    if (live) store_row(dst + i, o, inv);
+                } else if (fits && a.direct) {
+                    // joined by the same rows of another CTA's warps: dimension by dimension, rows side by side
+                    float *b = ps + (int64_t)i * (NQ * kBlk) + q * kBlk + r;
 #pragma unroll
-                    for (int j = 0; j < 32; j += 8) {
-                        uint32_t w[4];
+                    for (int j = 0; j < 32; ++j) __stcg(b + j * (NQ * kBlk), __uint_as_float(o[j]));
+                } else if (fits && live) {
+                    float *b = ps + (int64_t)(q * kBlk + r) * D + i;
 #pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            w[e] = pack_bf16(__uint_as_float(o[j + 2 * e]) * inv, __uint_as_float(o[j + 2 * e + 1]) * inv);
-                        *reinterpret_cast<uint4 *>(dst + j) = make_uint4(w[0], w[1], w[2], w[3]);
-                    }
-                } else if (fits) {
-                    float *dst = ps + (int64_t)(q * kBlk + r) * D + i;
-#pragma unroll
-                    for (int j = 0; j < 32; j += 4)
-                        *reinterpret_cast<uint4 *>(dst + j) = make_uint4(o[j], o[j + 1], o[j + 2], o[j + 3]);
+                    for (int j = 0; j < 32; j += 8) st32b(b + j, o + j);
                 }
                 __syncwarp();                          // the next TMEM load is the whole warp's
             }
-            if (live && !whole && fits) {
+            tc_before();                               // O's reads before the next unit's first product
+            if (!whole && fits) {
                 // joined with parts of either kernel: the maximum in units of log2
                 ps[NQ * kBlk * D + q * kBlk + r] = m == -INFINITY ? m : m * sc;
                 ps[NQ * kBlk * D + NQ * kBlk + q * kBlk + r] = l;
@@ -512,15 +489,14 @@ __global__ void __launch_bounds__(TileCfg<D, NQ>::kThreads, TileCfg<D, NQ>::kCta
                 before = __shfl_sync(0xffffffffu, before, 0);
                 if (before == (uint32_t)(cut.n - 1)) {
                     __threadfence();
-                    join_block<D, NQ>(a, cut, q * kBlk + r, live, orow);
+                    join_block<D, NQ>(a, cut, q * kBlk + r, live, dst);
                     if (lane == 0) *cnt = 0u;
                 }
             }
             __syncwarp();
-            tc_before();                               // O's reads before the next unit's first product
             done(nw);
             ++nw;
-            w = wn;
+            w = work(nw);
         }
     } else if (warp == kTmaWarp) {
         // ------------------------------------------------------------- K and V tiles
@@ -530,10 +506,10 @@ __global__ void __launch_bounds__(TileCfg<D, NQ>::kThreads, TileCfg<D, NQ>::kCta
         while (go) {
             const Work *w = work(nw);
             if (!w) break;
-            const int plen = w->plen, olen = w->olen, h = w->h, o = w->o, t1 = w->te;
+            const int plen = w->plen, olen = w->olen, np = (plen + KT - 1) / KT, h = w->h, o = w->o, t1 = w->te;
             const int32_t *ptab = pv.ptable + w->group * pv.ptable_stride, *otab = pv.table + o * pv.table_stride;
             for (int t = w->tb; t < t1 && go; ++t) {
-                const TileAt x = tile_at<KT>(plen, olen, t);
+                const TileAt x = tile_at<KT>(plen, olen, np, t);
                 const int nbox = (x.have + kBox - 1) / kBox;
                 // lane: one box of rows and 64 dimensions
                 const int bx = lane / Cfg::kHalves, hf = lane - bx * Cfg::kHalves;
@@ -579,7 +555,7 @@ __global__ void __launch_bounds__(TileCfg<D, NQ>::kThreads, TileCfg<D, NQ>::kCta
             return warp_wait(&bars->kv_full[i % kSlots], (i / kSlots) & 1, bars, pv.status);
         };
         // S of the tile whose K is the ring's i-th, once the S before it has been read
-        auto scores = [&](uint32_t i) {
+        auto scores = [&](uint32_t i, bool last) {
             if (!wait_kv(i) || (ns && !warp_wait(&bars->s_free[q], (ns - 1) & 1, bars, pv.status))) return false;
             tc_after();
             const uint32_t ka = kv0 + (i % kSlots) * (kTileB >> 4);
@@ -590,6 +566,7 @@ __global__ void __launch_bounds__(TileCfg<D, NQ>::kThreads, TileCfg<D, NQ>::kCta
                            ka + (((kk >> 2) * kHalfB + (kk & 3) * 32) >> 4), idS, kk > 0);
                 mma_commit(&bars->s_full[q]);
                 mma_commit(&bars->kv_empty[i % kSlots]);
+                if (last) mma_commit(&bars->q_free[q]);
             }
             __syncwarp();
             ++ns;
@@ -602,13 +579,13 @@ __global__ void __launch_bounds__(TileCfg<D, NQ>::kThreads, TileCfg<D, NQ>::kCta
                 break;
             }
             // ring: K of tile t at n + 2 t, V at n + 2 t + 1
-            const int plen = w->plen, olen = w->olen, tb0 = w->tb, nt = __shfl_sync(0xffffffffu, w->te - tb0, 0);
-            go = warp_wait(&bars->q_full[q], nw & 1, bars, pv.status) && scores(n);
+            const int plen = w->plen, olen = w->olen, np = (plen + KT - 1) / KT, tb0 = w->tb, nt = __shfl_sync(0xffffffffu, w->te - tb0, 0);
+            go = warp_wait(&bars->q_full[q], nw & 1, bars, pv.status) && scores(n, nt == 1);
             for (int t = 0; t < nt && go; ++t) {
                 const uint32_t iv = n + 2 * t + 1;
-                if (t + 1 < nt && !(go = scores(iv + 1))) break;
+                if (t + 1 < nt && !(go = scores(iv + 1, t + 2 == nt))) break;
                 if (!(go = wait_kv(iv))) break;
-                const TileAt x = tile_at<KT>(plen, olen, tb0 + t);
+                const TileAt x = tile_at<KT>(plen, olen, np, tb0 + t);
                 if (x.have < KT) {
                     // rows that do not exist (rest of a page, pages not copied) must not meet a weight
                     // of 0; both blocks' warps clear them, each before its own product
@@ -644,6 +621,7 @@ __global__ void __launch_bounds__(TileCfg<D, NQ>::kThreads, TileCfg<D, NQ>::kCta
     } else if (warp == kWorkWarp) {
         // -------------------------------------------------------------- the line ahead
         Piece p{};
+        uint32_t nq = 0;                               // pieces whose Q is on its way
         bool more = true;
         for (uint32_t i = 0; more; ++i) {
             if (i >= kWorks && !warp_wait(&bars->w_empty[i % kWorks], (i / kWorks - 1) & 1, bars, pv.status)) break;
@@ -662,7 +640,21 @@ __global__ void __launch_bounds__(TileCfg<D, NQ>::kThreads, TileCfg<D, NQ>::kCta
                 mbar_arrive(&bars->w_full[i % kWorks]);
             }
             __syncwarp();
+            // Q of the piece, once the products with the last one are done; rows past the
+            // tensor's end come as zeros, rows of other tokens are not used
+            for (int q = 0; q < NQ && more; ++q) {
+                if (i && !(more = warp_wait(&bars->q_free[q], (i - 1) & 1, bars, pv.status))) break;
+                if (lane == 0) mbar_arrive_expect_tx(&bars->q_full[q], (uint32_t)(tb * a.geo.G * D * 2));
+                __syncwarp();
+                if (lane < Cfg::kHalves)
+                    tma_3d(smem_u32(sQ + q * Cfg::kQB + lane * Cfg::kQHalfB), &qmap, lane * 64, p.h * a.geo.G,
+                           c.ow.t0 + p.tt * a.geo.tq + q * tb, &bars->q_full[q]);
+                __syncwarp();
+                nq = i + 1;
+            }
         }
+        // no copy may still be landing when the CTA ends
+        for (int q = 0; q < NQ && nq; ++q) mbar_wait_bounded(&bars->q_full[q], (nq - 1) & 1);
     }
     tc_before();
     __syncthreads();
@@ -704,17 +696,29 @@ bool pool_map(const cbq_paged_cache *c, void *pool, CUtensorMap *map) {
            CUDA_SUCCESS;
 }
 
+// The queries as {dimension, head, token}; a box is the G heads of a row block's tokens by 64 dimensions.
+bool query_map(const cbq_paged_cache *c, const cbq::PagedView &pv, const LineArgs &a, CUtensorMap *map) {
+    EncodeFn enc = encoder();
+    if (!enc) return false;
+    const cuuint64_t dims[3] = {(cuuint64_t)c->head_dim, (cuuint64_t)a.hq, (cuuint64_t)pv.tokens};
+    const cuuint64_t strides[2] = {(cuuint64_t)c->head_dim * 2, (cuuint64_t)a.qs * 2};
+    const cuuint32_t box[3] = {64, (cuuint32_t)a.geo.G, (cuuint32_t)(kBlk / a.geo.G)}, es[3] = {1, 1, 1};
+    return enc(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void *>(a.q), dims, strides, box, es,
+               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <int D, int NQ> int grid_of(int *ctas) {
     using Cfg = TileCfg<D, NQ>;
     return cbq_host::resident_ctas(reinterpret_cast<const void *>(k_paged_tile<D, NQ>), Cfg::kThreads, Cfg::kSmem, ctas);
 }
 
 template <int D, int NQ>
-int launch_tile(const CUtensorMap &km, const CUtensorMap &vm, const PagedView &pv, const LineArgs &a, int grid,
+int launch_tile(const CUtensorMap &km, const CUtensorMap &vm, const CUtensorMap &qm, const PagedView &pv, const LineArgs &a, int grid,
                 cudaStream_t s) {
     using Cfg = TileCfg<D, NQ>;
     CBQ_CUDA_TRY(cbq_host::launch_pdl(k_paged_tile<D, NQ>, dim3((unsigned)grid), dim3(Cfg::kThreads), (size_t)Cfg::kSmem, s,
-                                      km, vm, pv, a));
+                                      km, vm, qm, pv, a));
     return CBQ_OK;
 }
 
@@ -750,12 +754,12 @@ int tile_plan(const cbq::PagedView &pv, int d, int G, int mode, bool two, int64_
 }
 
 int tile_launch(const cbq_paged_cache *c, const cbq::PagedView &pv, const LinePlan &p, cbq::LineArgs a, cudaStream_t s) {
-    CUtensorMap km, vm;
-    if (!pool_map(c, c->k_dev, &km) || !pool_map(c, c->v_dev, &vm)) return CBQ_ERR_UNSUPPORTED;
+    CUtensorMap km, vm, qm;
+    if (!pool_map(c, c->k_dev, &km) || !pool_map(c, c->v_dev, &vm) || !query_map(c, pv, a, &qm)) return CBQ_ERR_UNSUPPORTED;
     const bool two = p.rows > kBlk;
     if (c->head_dim == 64)
-        return two ? launch_tile<64, 2>(km, vm, pv, a, p.grid, s) : launch_tile<64, 1>(km, vm, pv, a, p.grid, s);
-    return two ? launch_tile<128, 2>(km, vm, pv, a, p.grid, s) : launch_tile<128, 1>(km, vm, pv, a, p.grid, s);
+        return two ? launch_tile<64, 2>(km, vm, qm, pv, a, p.grid, s) : launch_tile<64, 1>(km, vm, qm, pv, a, p.grid, s);
+    return two ? launch_tile<128, 2>(km, vm, qm, pv, a, p.grid, s) : launch_tile<128, 1>(km, vm, qm, pv, a, p.grid, s);
 }
 
 }  // namespace cbq_host

@@ -604,7 +604,7 @@ int64_t cbq_paged_attn_workspace_bytes(const cbq_paged_cache *cache, const cbq_p
 /* Attention of one new token per sequence (tokens == seqs, cu_tokens_dev is
  * not read): q [seqs, Hq, d] (token stride q_stride) over the sequence's
  * prefix and its own kv_lens[s] rows, softmax(q k^T * scale) v -> out
- * [seqs, Hq, d] contiguous; query head h reads kv head h / (Hq / Hkv).  A
+ * [seqs, Hq, d] contiguous, 32-byte aligned (workspace 256); query head h reads kv head h / (Hq / Hkv).  A
  * group's prefix is read once for all its sequences.  A sequence with nothing
  * to read gives zeros.  Rows outside the lengths are never used, whatever they
  * hold.  Scores, softmax and sums in fp32; bf16: products of bf16 on the
