@@ -21,7 +21,7 @@
 // and the other way round: 943 TFLOP/s at 8192 tokens where this form has RATE.
 //
 // Warp roles: NQ softmax warpgroups (one row block each), a warp for each block's
-// products, a TMA warp (one cp.async.bulk.tensor for 16 rows and 64 dimensions;
+// products, a TMA warp (one cp.async.bulk.tensor for 16 rows;
 // K and V tiles alternate in a ring), a warp that walks the line ahead of them
 // and leaves its pieces in shared memory.
 // Work is the tile line of cbq_paged_line.cuh, one persistent CTA per part.
@@ -47,8 +47,9 @@ constexpr int kPoly = 0;               // of 16 weights, computed on the FMA pip
 template <int D, int NQ> struct TileCfg {
     static constexpr int KT = D == 128 ? 80 : 128;                     // keys of a tile
     static constexpr int kHalves = D / 64;                             // 128-byte wide column blocks
-    static constexpr int kQHalfB = kBlk * 128, kQB = kHalves * kQHalfB; // a row block of Q
-    static constexpr int kHalfB = KT * 128, kTileB = kHalves * kHalfB;  // a K or V tile
+    static constexpr int kQHalfB = kBlk * 128, kQB = kHalves * kQHalfB; // a row block of Q: column block by column block
+    static constexpr int kGroupB = kHalves * 1024;                      // 8 rows of K or V, column block by column block
+    static constexpr int kTileB = KT / 8 * kGroupB;                     // a K or V tile
     static constexpr int kSlots = NQ == 2 ? 8 : (D == 128 ? 3 : 4);     // K / V tiles in flight
     static constexpr int kSoft = NQ * 128;
     static constexpr int kThreads = kSoft + 128;                       // + a warpgroup for the other roles
@@ -86,30 +87,32 @@ struct Bars {
 static_assert(sizeof(Bars) <= 768, "barriers outgrow their region");
 
 // ---------------------------------------------------------------- PTX helpers
-// Shared-memory operand descriptors, 128-byte swizzle, 8-row groups 1024 bytes
-// apart.  The low word holds the address (in 16-byte units; stepping through an
-// operand adds to it) and the leading offset: unused for a K-major operand, the
-// distance of the 64-wide column blocks for an MN-major one (rows are K).
-constexpr uint32_t kDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);
+// Shared-memory operand descriptors, 128-byte swizzle.  The low word holds the
+// address (in 16-byte units; stepping through an operand adds to it) and the
+// leading offset: unused for a K-major operand, the distance of the 64-wide
+// column blocks for an MN-major one (rows are K).  The high word: the distance
+// of 8-row groups.
 __device__ __forceinline__ uint32_t desc_lo(uint32_t addr, uint32_t lead) { return (addr >> 4) | (lead >> 4) << 16; }
+__host__ __device__ constexpr uint32_t desc_hi(uint32_t group) { return (group >> 4) | (1u << 14) | (2u << 29); }
 // kind::f16: D fp32, A and B bf16, A K-major, B K-major or (bt) MN-major.
 __host__ __device__ constexpr uint32_t idesc(int M, int N, int bt) {
     return (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)bt << 16) | ((uint32_t)(N >> 3) << 17) |
            ((uint32_t)(M >> 4) << 24);
 }
-__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t id, uint32_t acc) {
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a, uint32_t ahi, uint32_t b, uint32_t bhi, uint32_t id,
+                                       uint32_t acc) {
     asm volatile(
         "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "mov.b64 da, {%1, %5};\n\tmov.b64 db, {%2, %5};\n\t"
+        "mov.b64 da, {%1, %5};\n\tmov.b64 db, {%2, %6};\n\t"
         "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n\t}" ::"r"(d), "r"(a), "r"(b), "r"(id), "r"(acc),
-        "r"(kDescHi));
+        "r"(ahi), "r"(bhi));
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t id, uint32_t acc) {
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t bhi, uint32_t id, uint32_t acc) {
     asm volatile(
         "{\n\t.reg .pred p;\n\t.reg .b64 db;\n\tsetp.ne.b32 p, %4, 0;\n\t"
         "mov.b64 db, {%2, %5};\n\t"
         "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, p;\n\t}" ::"r"(d), "r"(a), "r"(b), "r"(id), "r"(acc),
-        "r"(kDescHi));
+        "r"(bhi));
 }
 // One lane of the warp; the code under it stays uniform to the compiler.
 __device__ __forceinline__ bool elect() {
@@ -133,10 +136,10 @@ __device__ __forceinline__ void st32b(void *p, const uint32_t *v) {
     asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]),
                  "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]) : "memory");
 }
-__device__ __forceinline__ void tma_4d(uint32_t dst, const CUtensorMap *map, int c0, int c1, int c2, int c3, uint64_t *bar) {
+__device__ __forceinline__ void tma_5d(uint32_t dst, const CUtensorMap *map, int c3, int c4, uint64_t *bar) {
     asm volatile(
-        "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
-        ::"r"(dst), "l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(smem_u32(bar)) : "memory");
+        "cp.async.bulk.tensor.5d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %2, %2, %3, %4}], [%5];"
+        ::"r"(dst), "l"(map), "r"(0), "r"(c3), "r"(c4), "r"(smem_u32(bar)) : "memory");
 }
 // 32 columns of this thread's TMEM lane, without waiting for them.
 __device__ __forceinline__ void tld32(uint32_t a, uint32_t *v) {
@@ -281,7 +284,7 @@ __global__ void __launch_bounds__(TileCfg<D, NQ>::kThreads, TileCfg<D, NQ>::kCta
     k_paged_tile(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
                  const __grid_constant__ CUtensorMap qmap, const PagedView pv, const LineArgs a) {
     using Cfg = TileCfg<D, NQ>;
-    constexpr int kSlots = Cfg::kSlots, kTileB = Cfg::kTileB, kHalfB = Cfg::kHalfB, KT = Cfg::KT;
+    constexpr int kSlots = Cfg::kSlots, kTileB = Cfg::kTileB, KT = Cfg::KT;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     uint8_t *sQ = smem, *sKV = smem + NQ * Cfg::kQB;
@@ -502,25 +505,22 @@ __global__ void __launch_bounds__(TileCfg<D, NQ>::kThreads, TileCfg<D, NQ>::kCta
         // ------------------------------------------------------------- K and V tiles
         uint32_t n = 0, nw = 0;                        // tiles issued (K and V), pieces
         bool go = true;
-        const int ps = 1 << pv.ps_shift;
+        const int ps = 1 << pv.ps_shift, ratio = (int)(pv.page_stride / pv.head_stride);
+        const int none = (pv.pages - 1) * ratio + pv.kv_heads;
         while (go) {
             const Work *w = work(nw);
             if (!w) break;
-            const int plen = w->plen, olen = w->olen, np = (plen + KT - 1) / KT, h = w->h, o = w->o, t1 = w->te;
+            const int plen = w->plen, olen = w->olen, np = (plen + KT - 1) / KT, o = w->o, t1 = w->te, h = w->h;
             const int32_t *ptab = pv.ptable + w->group * pv.ptable_stride, *otab = pv.table + o * pv.table_stride;
             for (int t = w->tb; t < t1 && go; ++t) {
                 const TileAt x = tile_at<KT>(plen, olen, np, t);
-                const int nbox = (x.have + kBox - 1) / kBox;
-                // lane: one box of rows and 64 dimensions
-                const int bx = lane / Cfg::kHalves, hf = lane - bx * Cfg::kHalves;
-                const int key = x.key0 + bx * kBox;
-                int page = 0;
-                if (bx < nbox) {
-                    page = __ldg((x.pre ? ptab : otab) + (key >> pv.ps_shift));
-                    if (page < 0 || page >= pv.pages) {
-                        if (hf == 0) report(pv.status, CBQ_FLAG_CORRUPT, (uint32_t)o);
-                        page = pv.pages;               // outside the map: the copy fills with zeros
-                    }
+                const int nbox = __shfl_sync(0xffffffffu, (x.have + kBox - 1) / kBox, 0);
+                // lane b: the tile's b-th 16 rows, as a coordinate of (page, head); outside the map: zeros
+                int at = none;
+                if (lane < nbox) {
+                    const int page = __ldg((x.pre ? ptab : otab) + ((x.key0 + lane * kBox) >> pv.ps_shift));
+                    if (page >= 0 && page < pv.pages) at = page * ratio + h;
+                    else report(pv.status, CBQ_FLAG_CORRUPT, (uint32_t)o);
                 }
 #pragma unroll
                 for (int kv = 0; kv < 2; ++kv, ++n) {
@@ -529,11 +529,17 @@ __global__ void __launch_bounds__(TileCfg<D, NQ>::kThreads, TileCfg<D, NQ>::kCta
                         go = false;
                         break;
                     }
-                    if (lane == 0) mbar_arrive_expect_tx(&bars->kv_full[s], (uint32_t)(nbox * kBox * D * 2));
+                    const uint32_t dst = smem_u32(sKV) + s * kTileB;
+                    uint64_t *full = &bars->kv_full[s];
+                    if (elect()) mbar_arrive_expect_tx(full, (uint32_t)(nbox * kBox * D * 2));
                     __syncwarp();
-                    if (bx < nbox)
-                        tma_4d(smem_u32(sKV + s * kTileB + hf * kHalfB + bx * kBox * 128), kv ? &vmap : &kmap, hf * 64,
-                               key & (ps - 1), h, page, &bars->kv_full[s]);
+#pragma unroll
+                    for (int b = 0; b < KT / kBox; ++b) {
+                        if (b >= nbox) break;
+                        const int pg = __shfl_sync(0xffffffffu, at, b), grp = ((x.key0 + b * kBox) & (ps - 1)) >> 3;
+                        if (elect()) tma_5d(dst + b * 2 * Cfg::kGroupB, kv ? &vmap : &kmap, grp, pg, full);
+                        __syncwarp();
+                    }
                 }
             }
             done(nw++);
@@ -549,7 +555,8 @@ __global__ void __launch_bounds__(TileCfg<D, NQ>::kThreads, TileCfg<D, NQ>::kCta
         constexpr uint32_t idS = idesc(128, KT, 0), idO = idesc(128, D, 1);
         uint32_t n = 0, ns = 0, nw = 0;                // ring tiles used, tiles of S, pieces
         bool go = true;
-        const uint32_t kv0 = desc_lo(smem_u32(sKV), kHalfB), q0 = desc_lo(smem_u32(sQ + q * Cfg::kQB), kHalfB);
+        const uint32_t kv0 = desc_lo(smem_u32(sKV), 1024), q0 = desc_lo(smem_u32(sQ + q * Cfg::kQB), 0);
+        constexpr uint32_t hiQ = desc_hi(1024), hiKV = desc_hi(Cfg::kGroupB);
         const uint32_t tS = tmem + Cfg::sCol(q), tP = tmem + Cfg::pCol(q), tO = tmem + Cfg::oCol(q);
         auto wait_kv = [&](uint32_t i) {
             return warp_wait(&bars->kv_full[i % kSlots], (i / kSlots) & 1, bars, pv.status);
@@ -562,8 +569,8 @@ __global__ void __launch_bounds__(TileCfg<D, NQ>::kThreads, TileCfg<D, NQ>::kCta
             if (elect()) {
 #pragma unroll
                 for (int kk = 0; kk < D / 16; ++kk)
-                    mma_ss(tS, q0 + (((kk >> 2) * Cfg::kQHalfB + (kk & 3) * 32) >> 4),
-                           ka + (((kk >> 2) * kHalfB + (kk & 3) * 32) >> 4), idS, kk > 0);
+                    mma_ss(tS, q0 + (((kk >> 2) * Cfg::kQHalfB + (kk & 3) * 32) >> 4), hiQ,
+                           ka + (((kk >> 2) * 1024 + (kk & 3) * 32) >> 4), hiKV, idS, kk > 0);
                 mma_commit(&bars->s_full[q]);
                 mma_commit(&bars->kv_empty[i % kSlots]);
                 if (last) mma_commit(&bars->q_free[q]);
@@ -589,11 +596,12 @@ __global__ void __launch_bounds__(TileCfg<D, NQ>::kThreads, TileCfg<D, NQ>::kCta
                 if (x.have < KT) {
                     // rows that do not exist (rest of a page, pages not copied) must not meet a weight
                     // of 0; both blocks' warps clear them, each before its own product
-                    for (int e = x.have * 8 + lane; e < KT * 8; e += 32)
+                    for (int e = x.have * 8 + lane; e < KT * 8; e += 32) {
+                        uint8_t *row = sKV + (iv % kSlots) * kTileB + (e >> 6) * Cfg::kGroupB + (e & 63) * 16;
 #pragma unroll
                         for (int hf = 0; hf < Cfg::kHalves; ++hf)
-                            *reinterpret_cast<uint4 *>(sKV + (iv % kSlots) * kTileB + hf * kHalfB + e * 16) =
-                                make_uint4(0u, 0u, 0u, 0u);
+                            *reinterpret_cast<uint4 *>(row + hf * 1024) = make_uint4(0u, 0u, 0u, 0u);
+                    }
                     fence_proxy_async_smem();
                     __syncwarp();
                 }
@@ -603,7 +611,7 @@ __global__ void __launch_bounds__(TileCfg<D, NQ>::kThreads, TileCfg<D, NQ>::kCta
                 if (elect()) {
 #pragma unroll
                     for (int kk = 0; kk < KT / 16; ++kk)
-                        mma_ts(tO, tP + kk * 8, va + kk * (2048 >> 4), idO, t > 0 || kk > 0);
+                        mma_ts(tO, tP + kk * 8, va + kk * (2 * Cfg::kGroupB >> 4), hiKV, idO, t > 0 || kk > 0);
                     mma_commit(&bars->o_full[q]);
                     mma_commit(&bars->kv_empty[iv % kSlots]);
                 }
@@ -682,16 +690,21 @@ EncodeFn encoder() {
     return fn;
 }
 
-// The pool as {dimension, row, head, page}; a box is 16 rows by 64 dimensions.
+// The pool as {64 dimensions, 8 rows, column blocks, row groups, (page, head)};
+// a box is 16 rows of a page and head, in shared memory 8 rows by 8 rows and
+// within them column block by column block, which both products' descriptors
+// can step through: 4 KB a copy at head_dim 128 (a copy costs the SM's copy
+// engine 46 cycles and 18 a KB).
 bool pool_map(const cbq_paged_cache *c, void *pool, CUtensorMap *map) {
     EncodeFn enc = encoder();
     if (!enc) return false;
-    const cuuint64_t dims[4] = {(cuuint64_t)c->head_dim, (cuuint64_t)c->page_size, (cuuint64_t)c->kv_heads,
-                                (cuuint64_t)c->pages};
-    const cuuint64_t strides[3] = {(cuuint64_t)c->row_stride * 2, (cuuint64_t)c->head_stride * 2,
-                                   (cuuint64_t)c->page_stride * 2};
-    const cuuint32_t box[4] = {64, kBox, 1, 1}, es[4] = {1, 1, 1, 1};
-    return enc(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, pool, dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+    const cuuint64_t ratio = (cuuint64_t)(c->page_stride / c->head_stride);
+    const cuuint64_t dims[5] = {64, 8, (cuuint64_t)c->head_dim / 64, (cuuint64_t)c->page_size / 8,
+                                (cuuint64_t)(c->pages - 1) * ratio + (cuuint64_t)c->kv_heads};
+    const cuuint64_t strides[4] = {(cuuint64_t)c->row_stride * 2, 128, (cuuint64_t)c->row_stride * 16,
+                                   (cuuint64_t)c->head_stride * 2};
+    const cuuint32_t box[5] = {64, 8, (cuuint32_t)c->head_dim / 64, kBox / 8, 1}, es[5] = {1, 1, 1, 1, 1};
+    return enc(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 5, pool, dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
                CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) ==
            CUDA_SUCCESS;
 }
@@ -727,11 +740,13 @@ int launch_tile(const CUtensorMap &km, const CUtensorMap &vm, const CUtensorMap 
 namespace cbq_host {
 
 bool tile_takes(const cbq_paged_cache *c) {
-    // strides that a tensor map holds: positive, below 2^40 bytes
-    const int64_t top = (int64_t)1 << 39;
-    return c->dtype == CBQ_BF16 && (c->head_dim == 64 || c->head_dim == 128) && c->pages > 0 && c->row_stride > 0 &&
-           c->head_stride > 0 && c->page_stride > 0 && c->row_stride < top && c->head_stride < top && c->page_stride < top &&
-           encoder() != nullptr;
+    // what the pools' tensor maps hold: pages a whole number of heads apart, strides below 2^40 bytes,
+    // (page, head) counted in 32 bits
+    const int64_t top = (int64_t)1 << 35;
+    return c->dtype == CBQ_BF16 && (c->head_dim == 64 || c->head_dim == 128) && c->pages > 0 && c->head_stride > 0 &&
+           c->head_stride < top && c->row_stride < top && c->page_stride % c->head_stride == 0 && c->page_stride > 0 &&
+           c->pages < (int64_t)1 << 30 &&
+           c->page_stride / c->head_stride < ((int64_t)1 << 31) / (c->pages + 1) - c->kv_heads && encoder() != nullptr;
 }
 
 int tile_plan(const cbq::PagedView &pv, int d, int G, int mode, bool two, int64_t off, LinePlan *p) {
