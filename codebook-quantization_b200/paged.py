@@ -31,7 +31,25 @@ __all__ = ["PagedKVCache", "PagedBatch"]
 # on one stream do not overlap, and each leaves its arrival counters zero.
 _WORKSPACES = {}
 
+_F32 = torch.float32
+_FUNCTIONS = {}
+
 _CODES = {torch.float32: _lib.CBQ_F32, torch.bfloat16: _lib.CBQ_BF16}
+
+
+def _run(name: str, *args) -> None:
+    """A libcbq call, its function looked up once (these calls are short)."""
+    f = _FUNCTIONS.get(name)
+    if f is None:
+        f = _FUNCTIONS[name] = getattr(_lib.lib(), name)
+    rc = f(*args)
+    if rc != _lib.CBQ_OK:
+        raise _lib.CbqError(name, rc)
+
+
+# torch.cuda.current_stream builds a Stream object; the raw handle is all that is passed on
+_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
+_capturing = torch.cuda.is_current_stream_capturing
 
 
 def _need(ok: bool, what: str) -> None:
@@ -135,19 +153,20 @@ class PagedKVCache:
         self._desc = ct.create_string_buffer(raw, len(raw))
         self._addr = ct.addressof(self._desc)
         self._key = (tuple(k_pages.shape), self.dtype)
+        self._index = k_pages.get_device()
 
-    def _rows(self, t: torch.Tensor, name: str, heads: Optional[int]) -> int:
+    def _rows(self, t: torch.Tensor, name: str, heads: int) -> int:
         """Checks [tokens, heads, head_dim] of the cache's dtype, heads and
         head_dim contiguous; the stride from token to token."""
-        if t.dim() != 3 or t.shape[2] != self.head_dim or (heads is not None and t.shape[1] != heads):
-            raise ValueError(f"{name}: [tokens, {'heads' if heads is None else heads}, {self.head_dim}] expected, "
-                             f"got {tuple(t.shape)}")
-        if t.dtype != self.dtype or t.device != self.device:
-            raise ValueError(f"{name}: {t.dtype} on {t.device}, the cache is {self.dtype} on {self.device}")
+        n, h, d = t.shape
         st = t.stride()
-        if st[2] != 1 or (st[1] != self.head_dim and t.shape[1] != 1):
+        if d != self.head_dim or h != heads:
+            raise ValueError(f"{name}: [tokens, {heads}, {self.head_dim}] expected, got {tuple(t.shape)}")
+        if t.dtype is not self.dtype or t.get_device() != self._index:
+            raise ValueError(f"{name}: {t.dtype} on {t.device}, the cache is {self.dtype} on {self.device}")
+        if st[2] != 1 or (st[1] != d and h != 1):
             raise ValueError(f"{name}: the heads of a token must be contiguous")
-        return st[0] if t.shape[0] > 1 else t.shape[1] * self.head_dim
+        return st[0] if n > 1 else h * d
 
     def append_rope(self, batch: PagedBatch, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: torch.Tensor,
                     sin: torch.Tensor, eps: float = 1e-6, q_weight: Optional[torch.Tensor] = None,
@@ -157,22 +176,25 @@ class PagedKVCache:
         q.  ``eps`` < 0: no RMSNorm; weights fp32 [d] or None (ones); cos / sin
         fp32 [positions, d] (``qwen3_decode.rope_tables``)."""
         tokens, heads, d = q.shape
-        qs, ks, vs = self._rows(q, "q", None), self._rows(k, "k", self.kv_heads), self._rows(v, "v", self.kv_heads)
-        _need(k.shape[0] == tokens and v.shape[0] == tokens, "q, k and v must have the same tokens")
-        _need(cos.shape == sin.shape and cos.dim() == 2 and cos.shape[1] == d and cos.dtype == torch.float32 and
-              sin.dtype == torch.float32 and cos.is_contiguous() and sin.is_contiguous(),
-              f"cos and sin: contiguous float32 [positions, {d}] expected")
-        for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
-            _need(w is None or (w.dtype == torch.float32 and w.shape == (d,) and w.is_contiguous()),
-                  f"{name}: contiguous float32 [{d}] expected")
+        qs, ks, vs = self._rows(q, "q", heads), self._rows(k, "k", self.kv_heads), self._rows(v, "v", self.kv_heads)
+        if k.shape[0] != tokens or v.shape[0] != tokens:
+            raise ValueError("q, k and v must have the same tokens")
+        length = cos.shape[0]
+        for t in (cos, sin):
+            if t.shape != (length, d) or t.dtype is not _F32 or not t.is_contiguous() or t.get_device() != self._index:
+                raise ValueError(f"cos and sin: contiguous float32 [positions, {d}] on {self.device} expected")
+        for w in (q_weight, k_weight):
+            if w is not None and (w.shape != (d,) or w.dtype is not _F32 or not w.is_contiguous() or
+                                  w.get_device() != self._index):
+                raise ValueError(f"q_weight and k_weight: contiguous float32 [{d}] on {self.device} expected")
         if out is None:
-            out = torch.empty((tokens, heads, d), dtype=self.dtype, device=self.device)
+            out = q.new_empty((tokens, heads, d))
         else:
             self._out(out, tokens, heads)
-        _lib.call("cbq_paged_append_rope", self._addr, batch._addr, tokens, q.data_ptr(), qs, k.data_ptr(),
-                  ks, v.data_ptr(), vs, heads, eps, None if q_weight is None else q_weight.data_ptr(),
-                  None if k_weight is None else k_weight.data_ptr(), cos.data_ptr(), sin.data_ptr(), cos.shape[0],
-                  out.data_ptr(), torch.cuda.current_stream(self.device).cuda_stream)
+        _run("cbq_paged_append_rope", self._addr, batch._addr, tokens, q.data_ptr(), qs, k.data_ptr(),
+             ks, v.data_ptr(), vs, heads, eps, None if q_weight is None else q_weight.data_ptr(),
+             None if k_weight is None else k_weight.data_ptr(), cos.data_ptr(), sin.data_ptr(), length, out.data_ptr(),
+             _stream(self._index))
         return out
 
     def _out(self, out: torch.Tensor, tokens: int, heads: int) -> None:
@@ -192,24 +214,24 @@ class PagedKVCache:
     def _attend(self, name: str, extend: bool, batch: PagedBatch, q: torch.Tensor, scale: Optional[float],
                 out: Optional[torch.Tensor], workspace: Optional[torch.Tensor]) -> torch.Tensor:
         tokens, heads, d = q.shape
-        stride = self._rows(q, "q", None)
+        stride = self._rows(q, "q", heads)
         if out is None:
-            out = torch.empty((tokens, heads, d), dtype=self.dtype, device=self.device)
+            out = q.new_empty((tokens, heads, d))
         else:
             self._out(out, tokens, heads)
-        stream = torch.cuda.current_stream(self.device).cuda_stream
+        stream = _stream(self._index)
         if workspace is None:
             workspace = self._scratch(stream, self.workspace_bytes(batch, tokens, heads, extend))
-        _lib.call(name, self._addr, batch._addr, tokens, q.data_ptr(), stride, heads,
-                  d ** -0.5 if scale is None else scale, out.data_ptr(), workspace.data_ptr(), workspace.numel(), stream)
+        _run(name, self._addr, batch._addr, tokens, q.data_ptr(), stride, heads, d ** -0.5 if scale is None else scale,
+             out.data_ptr(), workspace.data_ptr(), workspace.numel(), stream)
         return out
 
     def _scratch(self, stream: int, need: int) -> torch.Tensor:
         """Zero-filled scratch for calls on ``stream``; inside a graph capture a
         buffer of the graph's own, which its replays clear."""
-        if torch.cuda.is_current_stream_capturing():
+        if _capturing():
             return torch.zeros(need, dtype=torch.uint8, device=self.device)
-        key = (self.device.index, stream)
+        key = (self._index, stream)
         ws = _WORKSPACES.get(key)
         if ws is None or ws.numel() < need:
             ws = _WORKSPACES[key] = torch.zeros(need + need // 2, dtype=torch.uint8, device=self.device)
