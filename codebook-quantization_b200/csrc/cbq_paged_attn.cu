@@ -57,7 +57,7 @@ template <typename T, int D, int NB> struct StreamCfg {
     static constexpr int kRowB = D * (int)sizeof(T);
     static constexpr int kHalf = kKeys * kRowB;                         // K (or V) of a stage
     static constexpr int kStage = 2 * kHalf;
-    static constexpr int S = D == 64 && !kF32 ? 4 : (D == 256 && !kF32 && NB > 1 ? 2 : 3);   // stages in flight per warp
+    static constexpr int S = kF32 ? (D == 64 ? 2 : 3) : (D == 64 ? 4 : (D == 256 && NB > 1 ? 2 : 3));   // ring stages of a warp
     static constexpr int kPitch = D + 4;                                // merge rows, padded against bank conflicts
     static constexpr int kMerge = NW * R * (kPitch + 2) * 4;
     static constexpr int kQ = kF32 ? R * D * 4 : 0;
@@ -522,7 +522,7 @@ struct JoinSource {
     const float *part;
     const uint64_t *cum;
     int64_t slots;
-    int owners, grid, min_tiles, rows, tile_rows;
+    int owners, grid, min_tiles, rows, tile_rows, mode;
     LineGeo geo;
 };
 
@@ -607,18 +607,19 @@ __device__ __forceinline__ void join_row(const Parts &pa, const Parts &pb, T *ds
     }
 }
 
-// Decode over a shared prefix: every unit left parts, all units of an owner
-// have the same tiles.  Parts of the row of token `tl` of owner o, head (h, gi).
-__device__ __forceinline__ Parts even_parts(const JoinSource &s, int kv_heads, int o, int tl, int h, int gi) {
+// Where every unit left parts: those of the row of owner o's token tl, head (h, gi).
+__device__ __forceinline__ Parts parts_of(const JoinSource &s, const PagedView &pv, int o, const Owner &w, int tl, int h,
+                                          int gi) {
     Parts p{};
     p.s = &s;
-    const uint64_t c0 = s.cum[o], c1 = s.cum[o + 1], all = s.cum[s.owners];
-    const uint32_t nu = (uint32_t)(c1 >> 32) - (uint32_t)(c0 >> 32), n = (uint32_t)c1 - (uint32_t)c0;
-    const int per_h = (int)(nu / (uint32_t)kv_heads), tts = per_h / s.geo.hc, tt = tl / s.geo.tq;
-    if (n == 0 || tl < 0 || tt >= tts) return p;
-    const uint32_t per = tiles_per_cta((uint32_t)all, (uint32_t)s.grid, (uint32_t)s.min_tiles), tiles = n / nu;
-    const int hc = s.geo.hc > 1 ? gi / s.rows : 0;
-    const uint32_t u = (uint32_t)(h * per_h + tt * s.geo.hc + hc), w0 = (uint32_t)c0 + u * tiles;
+    const uint64_t c0 = s.cum[o], all = s.cum[s.owners];
+    const OwnerTiles t = owner_tiles(w, s.geo, s.mode);
+    const int tt = tl / s.geo.tq;
+    if (tl < 0 || tt >= t.tt) return p;
+    const uint32_t per = tiles_per_cta((uint32_t)all, (uint32_t)s.grid, (uint32_t)s.min_tiles), tiles = t.of(tt);
+    const int nhc = s.geo.hc, hc = nhc > 1 ? gi / s.rows : 0;
+    const uint32_t u = (uint32_t)((h * t.tt + tt) * nhc + hc);
+    const uint32_t w0 = (uint32_t)c0 + ((uint32_t)h * t.all() + t.before(tt)) * (uint32_t)nhc + (uint32_t)hc * tiles;
     const int i0 = (int)(w0 / per);
     p.slot0 = (int64_t)(c0 >> 32) + u + i0;
     p.n = (int)((w0 + tiles - 1) / per) - i0 + 1;
@@ -636,9 +637,15 @@ __global__ void __launch_bounds__(128) k_join_rows(const PagedView pv, const Joi
     const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
     if (row >= (int64_t)pv.tokens * hq) return;
     const int t = (int)(row / hq), x = (int)(row - (int64_t)t * hq), h = x / own.geo.G, gi = x - h * own.geo.G;
-    const int g = warp_upper(pv.gs, pv.groups, t);
-    const Parts pp = even_parts(pre, pv.kv_heads, g, t - pv.gs[g], h, gi);
-    const Parts po = even_parts(own, pv.kv_heads, t, 0, h, gi);
+    const int o = own.mode == kFull && pv.cu ? warp_upper(pv.cu, pv.seqs, t) : t;
+    const Owner w = owner_of(pv, own.mode, o);
+    const Parts po = parts_of(own, pv, o, w, t - w.t0, h, gi);
+    Parts pp{};
+    if (pre.part) {
+        const int g = warp_upper(pv.gs, pv.groups, t);
+        const Owner wg = owner_of(pv, kPrefix, g);
+        pp = parts_of(pre, pv, g, wg, t - wg.t0, h, gi);
+    }
     join_row<T, D>(pp, po, static_cast<T *>(out) + row * D);
 }
 
@@ -683,12 +690,14 @@ int row_blocks(int64_t rows) { return rows <= 8 ? 1 : (rows <= 16 ? 2 : 4); }
 
 // Plan of a k_paged_stream launch whose owners have about `rows` query rows
 // per kv head: as few blocks of 8 as hold them, at most 32.
-int stream_plan(const PagedView &pv, int dtype, int d, int G, int64_t rows, int64_t off, cbq_host::LinePlan *p) {
+int stream_plan(const PagedView &pv, int dtype, int d, int G, int64_t rows, int limit, int64_t off,
+                cbq_host::LinePlan *p) {
     int rc = CBQ_OK;
 #define CBQ_CALL(T, DD, NN) rc = stream_grid<T, DD, NN>(p)
     CBQ_STREAM_DISPATCH(dtype, d, row_blocks(rows), CBQ_CALL)
 #undef CBQ_CALL
     if (rc != CBQ_OK) return rc;
+    p->grid = std::min(p->grid, limit);
     p->tile_rows = 0;
     p->geo.G = G;
     p->geo.tq = std::max(1, p->rows / G);
@@ -697,6 +706,8 @@ int stream_plan(const PagedView &pv, int dtype, int d, int G, int64_t rows, int6
     p->min_tiles = 1;
     return cbq_host::line_room(pv, d, off, p) ? CBQ_OK : CBQ_ERR_UNSUPPORTED;
 }
+
+constexpr int kStreamRows = 16;       // query rows per kv head up to which k_paged_stream is the faster kernel
 
 struct AttnPlan {
     PagedView pv;
@@ -725,19 +736,31 @@ int plan_attn(const cbq_paged_cache *c, const cbq_paged_batch *b, int64_t tokens
     // query rows that share a kv head's keys, on the mean of the owners
     const int64_t own_rows = extend ? (tokens * p->G + b->seqs - 1) / b->seqs : p->G;
     p->own.mode = extend ? kFull : kOwn;
+    p->own_tile = tile && extend && own_rows > kStreamRows;
+    const int sms = cbq_host::sm_count();
+    int64_t group_rows = 0;
+    if (p->prefix) {
+        group_rows = ((int64_t)b->seqs + b->groups - 1) / b->groups * p->G;
+        p->pre_tile = tile && group_rows > kStreamRows;
+    }
+    // a tile kernel of one row block and the own rows' kernel run side by side, one CTA of each on an SM
+    const int limit = p->pre_tile && group_rows <= 128 ? sms : 1 << 30;
     p->own.direct = !p->prefix;
-    p->own_tile = tile && extend && own_rows > 32;
-    int e = p->own_tile ? cbq_host::tile_plan(p->pv, p->d, p->G, kFull, own_rows > 128, cbq_host::kCountBytes, &p->own)
-                        : stream_plan(p->pv, p->dtype, p->d, p->G, own_rows, cbq_host::kCountBytes, &p->own);
+    if (p->own_tile) {
+        // few units: each is cut into many parts, which k_join_rows joins with a warp for every row
+        const bool two = own_rows > 128;
+        const int64_t units = (tokens * p->G / (two ? 256 : 128) + b->seqs) * c->kv_heads;
+        if (2 * units < (two ? sms : 2 * sms)) p->own.direct = 0;
+    }
+    int e = p->own_tile ? cbq_host::tile_plan(p->pv, p->d, p->G, kFull, own_rows > 128, limit, cbq_host::kCountBytes, &p->own)
+                        : stream_plan(p->pv, p->dtype, p->d, p->G, own_rows, limit, cbq_host::kCountBytes, &p->own);
     if (e != CBQ_OK) return e;
     p->bytes = p->own.end;
     if (p->prefix) {
-        const int64_t rows = ((int64_t)b->seqs + b->groups - 1) / b->groups * p->G;
         p->pre.mode = kPrefix;
         p->pre.direct = 0;
-        p->pre_tile = tile && rows > 32;
-        e = p->pre_tile ? cbq_host::tile_plan(p->pv, p->d, p->G, kPrefix, rows > 128, p->bytes, &p->pre)
-                        : stream_plan(p->pv, p->dtype, p->d, p->G, rows, p->bytes, &p->pre);
+        e = p->pre_tile ? cbq_host::tile_plan(p->pv, p->d, p->G, kPrefix, group_rows > 128, limit, p->bytes, &p->pre)
+                        : stream_plan(p->pv, p->dtype, p->d, p->G, group_rows, limit, p->bytes, &p->pre);
         if (e != CBQ_OK) return e;
         p->bytes = p->pre.end;
     }
@@ -796,7 +819,7 @@ int paged_attn(const cbq_paged_cache *c, const cbq_paged_batch *b, int64_t token
     auto source = [&](const cbq_host::LinePlan &lp) {
         return JoinSource{reinterpret_cast<const float *>(w + lp.part_off),
                           reinterpret_cast<const uint64_t *>(w + lp.cum_off), lp.slots, lp.owners, lp.grid, lp.min_tiles,
-                          lp.rows, lp.tile_rows, lp.geo};
+                          lp.rows, lp.tile_rows, lp.mode, lp.geo};
     };
     if (p.prefix) {
         if ((rc = run_line(c, p, p.pre, p.pre_tile, line_args(p.pre, a, w), s)) != CBQ_OK) return rc;
@@ -804,8 +827,8 @@ int paged_attn(const cbq_paged_cache *c, const cbq_paged_batch *b, int64_t token
     }
     const LineArgs own = line_args(p.own, a, w);
     if ((rc = run_line(c, p, p.own, p.own_tile, own, s)) != CBQ_OK) return rc;
-    if (!p.prefix) return CBQ_OK;
-    const JoinSource so = source(p.own), sp = source(p.pre);
+    if (p.own.direct) return CBQ_OK;
+    const JoinSource so = source(p.own), sp = p.prefix ? source(p.pre) : JoinSource{};
     if (p.dtype == CBQ_F32)
         return p.d == 64 ? join_launch<float, 64>(p, own, so, sp, s)
                          : (p.d == 128 ? join_launch<float, 128>(p, own, so, sp, s)

@@ -396,7 +396,7 @@ int resident_ctas(const void *kern, int threads, int smem, int *out);
 // The tensor-core kernel for many query rows (cbq_paged_tile.cu): whether it
 // takes the shape, its plan, and its launch.
 bool tile_takes(const cbq_paged_cache *c);
-int tile_plan(const cbq::PagedView &pv, int d, int G, int mode, bool two, int64_t off, LinePlan *p);
+int tile_plan(const cbq::PagedView &pv, int d, int G, int mode, bool two, int limit, int64_t off, LinePlan *p);
 int tile_launch(const cbq_paged_cache *c, const cbq::PagedView &pv, const LinePlan &p, cbq::LineArgs a, cudaStream_t s);
 
 }  // namespace cbq_host

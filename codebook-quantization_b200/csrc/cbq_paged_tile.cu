@@ -359,11 +359,20 @@ __global__ void __launch_bounds__(TileCfg<D, NQ>::kThreads, TileCfg<D, NQ>::kCta
             const int plen = w->plen, olen = w->olen, np = (plen + KT - 1) / KT, t0 = w->tb, t1 = w->te;
             const int olim = a.mode == kPrefix ? 0 : clampi(olen - w->nt + tok + 1, 0, olen);
             float m = -INFINITY, l = 0.f;
+            const bool idle = !__any_sync(0xffffffffu, live);       // a warp whose rows hold no query only keeps step
             bool early = false;                        // S of the tile was there before the last one's end
             for (int t = t0; t < t1; ++t, ++ns) {
                 if (!__all_sync(0xffffffffu, early) && !warp_wait(&bars->s_full[q], ns & 1, bars, pv.status)) {
                     go = false;
                     break;
+                }
+                if (idle) {
+                    mbar_arrive(&bars->s_free[q]);
+                    // not a P ahead of the others: its arrival would count for theirs
+                    if (t > t0 && !warp_wait(&bars->o_full[q], (ns - 1) & 1, bars, pv.status)) { go = false; break; }
+                    mbar_arrive(&bars->p_full[q]);
+                    early = false;
+                    continue;
                 }
                 tc_after();
                 uint32_t s[KT];
@@ -455,7 +464,7 @@ __global__ void __launch_bounds__(TileCfg<D, NQ>::kThreads, TileCfg<D, NQ>::kCta
             __nv_bfloat16 *dst = static_cast<__nv_bfloat16 *>(a.out) +
                                  ((int64_t)(w->t0 + tok) * a.hq + w->h * a.geo.G + rg) * D;
 #pragma unroll 1
-            for (int i = 0; i < D; i += 32) {
+            for (int i = 0; i < D && !idle; i += 32) {
                 uint32_t o[32];
                 tld32(tO + i, o);
                 tld_wait();
@@ -474,12 +483,12 @@ __global__ void __launch_bounds__(TileCfg<D, NQ>::kThreads, TileCfg<D, NQ>::kCta
                 __syncwarp();                          // the next TMEM load is the whole warp's
             }
             tc_before();                               // O's reads before the next unit's first product
-            if (!whole && fits) {
+            if (!whole && fits && !idle) {
                 // joined with parts of either kernel: the maximum in units of log2
                 ps[NQ * kBlk * D + q * kBlk + r] = m == -INFINITY ? m : m * sc;
                 ps[NQ * kBlk * D + NQ * kBlk + q * kBlk + r] = l;
             }
-            if (a.direct && !whole) {
+            if (a.direct && !whole && !idle) {
                 // the warp that arrives last at its 32 rows of a cut unit joins
                 // their parts (a count for each warp: no barrier that a warp whose
                 // wait gave up could leave the others at)
@@ -749,7 +758,7 @@ bool tile_takes(const cbq_paged_cache *c) {
            c->page_stride / c->head_stride < ((int64_t)1 << 31) / (c->pages + 1) - c->kv_heads && encoder() != nullptr;
 }
 
-int tile_plan(const cbq::PagedView &pv, int d, int G, int mode, bool two, int64_t off, LinePlan *p) {
+int tile_plan(const cbq::PagedView &pv, int d, int G, int mode, bool two, int limit, int64_t off, LinePlan *p) {
     int n = 0;
     const int rc = d == 64 ? (two ? grid_of<64, 2>(&n) : grid_of<64, 1>(&n))
                            : (two ? grid_of<128, 2>(&n) : grid_of<128, 1>(&n));
@@ -764,7 +773,7 @@ int tile_plan(const cbq::PagedView &pv, int d, int G, int mode, bool two, int64_
     p->geo.keys = d == 64 ? TileCfg<64, 1>::KT : TileCfg<128, 1>::KT;
     p->geo.join = 0;
     p->min_tiles = 2;                  // a part costs its CTA about as much as a tile
-    p->grid = n * sm_count();
+    p->grid = std::min(n * sm_count(), limit);
     return p->grid * 8 <= kCounts && line_room(pv, d, off, p) ? CBQ_OK : CBQ_ERR_UNSUPPORTED;
 }
 
