@@ -690,14 +690,12 @@ int row_blocks(int64_t rows) { return rows <= 8 ? 1 : (rows <= 16 ? 2 : 4); }
 
 // Plan of a k_paged_stream launch whose owners have about `rows` query rows
 // per kv head: as few blocks of 8 as hold them, at most 32.
-int stream_plan(const PagedView &pv, int dtype, int d, int G, int64_t rows, int limit, int64_t off,
-                cbq_host::LinePlan *p) {
+int stream_plan(const PagedView &pv, int dtype, int d, int G, int64_t rows, int64_t off, cbq_host::LinePlan *p) {
     int rc = CBQ_OK;
 #define CBQ_CALL(T, DD, NN) rc = stream_grid<T, DD, NN>(p)
     CBQ_STREAM_DISPATCH(dtype, d, row_blocks(rows), CBQ_CALL)
 #undef CBQ_CALL
     if (rc != CBQ_OK) return rc;
-    p->grid = std::min(p->grid, limit);
     p->tile_rows = 0;
     p->geo.G = G;
     p->geo.tq = std::max(1, p->rows / G);
@@ -743,24 +741,22 @@ int plan_attn(const cbq_paged_cache *c, const cbq_paged_batch *b, int64_t tokens
         group_rows = ((int64_t)b->seqs + b->groups - 1) / b->groups * p->G;
         p->pre_tile = tile && group_rows > kStreamRows;
     }
-    // a tile kernel of one row block and the own rows' kernel run side by side, one CTA of each on an SM
-    const int limit = p->pre_tile && group_rows <= 128 ? sms : 1 << 30;
     p->own.direct = !p->prefix;
     if (p->own_tile) {
         // few units: each is cut into many parts, which k_join_rows joins with a warp for every row
         const bool two = own_rows > 128;
         const int64_t units = (tokens * p->G / (two ? 256 : 128) + b->seqs) * c->kv_heads;
-        if (2 * units < (two ? sms : 2 * sms)) p->own.direct = 0;
+        if (2 * units < sms) p->own.direct = 0;
     }
-    int e = p->own_tile ? cbq_host::tile_plan(p->pv, p->d, p->G, kFull, own_rows > 128, limit, cbq_host::kCountBytes, &p->own)
-                        : stream_plan(p->pv, p->dtype, p->d, p->G, own_rows, limit, cbq_host::kCountBytes, &p->own);
+    int e = p->own_tile ? cbq_host::tile_plan(p->pv, p->d, p->G, kFull, own_rows > 128, cbq_host::kCountBytes, &p->own)
+                        : stream_plan(p->pv, p->dtype, p->d, p->G, own_rows, cbq_host::kCountBytes, &p->own);
     if (e != CBQ_OK) return e;
     p->bytes = p->own.end;
     if (p->prefix) {
         p->pre.mode = kPrefix;
         p->pre.direct = 0;
-        e = p->pre_tile ? cbq_host::tile_plan(p->pv, p->d, p->G, kPrefix, group_rows > 128, limit, p->bytes, &p->pre)
-                        : stream_plan(p->pv, p->dtype, p->d, p->G, group_rows, limit, p->bytes, &p->pre);
+        e = p->pre_tile ? cbq_host::tile_plan(p->pv, p->d, p->G, kPrefix, group_rows > 128, p->bytes, &p->pre)
+                        : stream_plan(p->pv, p->dtype, p->d, p->G, group_rows, p->bytes, &p->pre);
         if (e != CBQ_OK) return e;
         p->bytes = p->pre.end;
     }

@@ -257,31 +257,48 @@ __host__ __device__ __forceinline__ uint32_t tiles_per_cta(uint32_t W, uint32_t 
 template <int NT>
 __device__ __forceinline__ bool plan_line(const PagedView &pv, const LineArgs &a, Cursor &c, uint32_t &w1, uint32_t &per) {
     constexpr int NW = NT / 32;
-    __shared__ uint64_t red[NW];
-    __shared__ uint64_t found_base;
-    __shared__ int found;
+    __shared__ uint64_t red[2 * NW];
+    __shared__ Cursor at;                              // written by the thread whose owner holds w0
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const bool writer = blockIdx.x == 0 && !a.direct;
+    const uint32_t per_unit = (uint32_t)(pv.kv_heads * a.geo.hc);
+    Owner w{};
+    OwnerTiles tl{};
     auto weight = [&](int o) -> uint64_t {
         if (o >= a.owners) return 0;
-        const Owner w = owner_of(pv, a.mode, o);
+        w = owner_of(pv, a.mode, o);
         if (blockIdx.x == 0 && (a.mode == kPrefix ? pv.plens[o] > pv.pcap : pv.lens[o] > pv.cap))
             report(pv.status, CBQ_FLAG_CORRUPT, (uint32_t)o);
-        const OwnerTiles t = owner_tiles(w, a.geo, a.mode);
-        const uint32_t n = (uint32_t)(pv.kv_heads * a.geo.hc);
-        return (uint64_t)(n * (uint32_t)t.tt) << 32 | n * t.all();
+        tl = owner_tiles(w, a.geo, a.mode);
+        return (uint64_t)(per_unit * (uint32_t)tl.tt) << 32 | per_unit * tl.all();
     };
-    const uint64_t first = weight(tid);
-    uint64_t sum = first;
-    for (int o = tid + NT; o < a.owners; o += NT) sum += weight(o);
+    // owners beyond the first NT: their sum first, the first NT below in one scan
+    uint64_t rest = 0;
+    for (int o = tid + NT; o < a.owners; o += NT) rest += weight(o);
+    uint64_t x = weight(tid);
+    uint64_t inc = x;
 #pragma unroll
-    for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-    if (lane == 0) red[warp] = sum;
-    if (tid == 0) found = -1;
+    for (int d = 1; d < 32; d <<= 1) {
+        const uint64_t y = __shfl_up_sync(0xffffffffu, inc, d);
+        if (lane >= d) inc += y;
+    }
+    if (a.owners > NT)
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) rest += __shfl_xor_sync(0xffffffffu, rest, d);
+    if (lane == 31) {
+        red[warp] = inc;
+        red[NW + warp] = rest;
+    }
+    if (tid == 0) at.o = -1;
     __syncthreads();
-    uint64_t total = 0;
+    uint64_t before = 0, all = 0, total = 0;
 #pragma unroll
-    for (int i = 0; i < NW; ++i) total += red[i];
+    for (int i = 0; i < NW; ++i) {
+        if (i < warp) before += red[i];
+        all += red[i];
+        total += red[NW + i];
+    }
+    total += all;
     const uint32_t W = (uint32_t)total;
     per = tiles_per_cta(W, gridDim.x, (uint32_t)a.min_tiles);
     const uint32_t w0 = (uint32_t)min((uint64_t)per * blockIdx.x, (uint64_t)W);
@@ -289,39 +306,45 @@ __device__ __forceinline__ bool plan_line(const PagedView &pv, const LineArgs &a
     if (writer && tid == 0) a.cum[a.owners] = total;
     if (w0 >= w1 && !writer) return false;
     uint64_t run = 0;
-    for (int o0 = 0; o0 < a.owners; o0 += NT) {
+    for (int o0 = 0;; ) {
         const int o = o0 + tid;
-        const uint64_t x = o0 == 0 ? first : weight(o);
-        uint64_t inc = x;
+        const uint64_t ex = run + before + inc - x;
+        if (o < a.owners) {
+            if (writer) a.cum[o] = ex;
+            if ((uint32_t)ex <= w0 && w0 < (uint32_t)ex + (uint32_t)x) {
+                at.w = w0;
+                at.base = (uint32_t)ex;
+                at.ubase = (uint32_t)(ex >> 32);
+                at.wh = tl.all() * (uint32_t)a.geo.hc;
+                at.o = o;
+                at.ow = w;
+                at.tl = tl;
+                at.p.tiles = 0;
+            }
+        }
+        run += all;
+        o0 += NT;
+        if (o0 >= a.owners || (!writer && (uint32_t)run > w0)) break;   // all seen, or the owner was among these
+        x = weight(o0 + tid);
+        inc = x;
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) {
             const uint64_t y = __shfl_up_sync(0xffffffffu, inc, d);
             if (lane >= d) inc += y;
         }
-        __syncthreads();                              // red[] of the previous use
+        __syncthreads();                              // red[] of the previous block of owners
         if (lane == 31) red[warp] = inc;
         __syncthreads();
-        uint64_t before = run, all = 0;
+        before = all = 0;
 #pragma unroll
         for (int i = 0; i < NW; ++i) {
             if (i < warp) before += red[i];
             all += red[i];
         }
-        const uint64_t ex = before + inc - x;
-        if (writer && o < a.owners) a.cum[o] = ex;
-        if (o < a.owners && (uint32_t)ex <= w0 && w0 < (uint32_t)ex + (uint32_t)x) {
-            found = o;
-            found_base = ex;
-        }
-        run += all;
-        if (!writer && (uint32_t)run > w0) break;      // the owner is in this block of owners
     }
     __syncthreads();
-    if (w0 >= w1 || found < 0) return false;
-    c.w = w0;
-    c.base = (uint32_t)found_base;
-    c.ubase = (uint32_t)(found_base >> 32);
-    cursor_owner(c, pv, a, found);
+    if (w0 >= w1 || at.o < 0) return false;
+    c = at;
     return true;
 }
 
@@ -396,7 +419,7 @@ int resident_ctas(const void *kern, int threads, int smem, int *out);
 // The tensor-core kernel for many query rows (cbq_paged_tile.cu): whether it
 // takes the shape, its plan, and its launch.
 bool tile_takes(const cbq_paged_cache *c);
-int tile_plan(const cbq::PagedView &pv, int d, int G, int mode, bool two, int limit, int64_t off, LinePlan *p);
+int tile_plan(const cbq::PagedView &pv, int d, int G, int mode, bool two, int64_t off, LinePlan *p);
 int tile_launch(const cbq_paged_cache *c, const cbq::PagedView &pv, const LinePlan &p, cbq::LineArgs a, cudaStream_t s);
 
 }  // namespace cbq_host

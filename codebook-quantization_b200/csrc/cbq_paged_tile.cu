@@ -50,13 +50,13 @@ template <int D, int NQ> struct TileCfg {
     static constexpr int kQHalfB = kBlk * 128, kQB = kHalves * kQHalfB; // a row block of Q: column block by column block
     static constexpr int kGroupB = kHalves * 1024;                      // 8 rows of K or V, column block by column block
     static constexpr int kTileB = KT / 8 * kGroupB;                     // a K or V tile
-    static constexpr int kSlots = NQ == 2 ? 8 : (D == 128 ? 3 : 4);     // K / V tiles in flight
+    static constexpr int kSlots = 8;                                   // K / V tiles in flight
     static constexpr int kSoft = NQ * 128;
     static constexpr int kThreads = kSoft + 128;                       // + a warpgroup for the other roles
-    // registers: the launch's share is split unevenly, kSoft * kSoftRegs + 128 * kRestRegs <= 65536 / kCtas
-    static constexpr int kSoftRegs = NQ == 2 ? 208 : 200;
-    static constexpr int kRestRegs = NQ == 2 ? 88 : 56;
-    static constexpr int kCtas = NQ == 2 ? 1 : 2;                       // per SM: TMEM has 512 columns
+    // registers: NQ = 2 splits the launch's 168 a thread unevenly (NQ = 1 has enough: one CTA on an SM,
+    // whose shared memory goes to the ring)
+    static constexpr int kSoftRegs = 208, kRestRegs = 88;
+    static_assert(NQ == 1 || kSoft * kSoftRegs + 128 * kRestRegs <= kThreads * 168, "registers of the launch");
     static constexpr int kCols = NQ == 2 ? 512 : 256;
     static constexpr int kSmem = 1024 + NQ * kQB + kSlots * kTileB + 768;
     static __host__ __device__ constexpr uint32_t sCol(int b) { return (uint32_t)(b * (KT + KT / 2)); }
@@ -280,7 +280,7 @@ template <int N> __device__ __forceinline__ void regs_up() { asm volatile("setma
 template <int N> __device__ __forceinline__ void regs_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 
 template <int D, int NQ>
-__global__ void __launch_bounds__(TileCfg<D, NQ>::kThreads, TileCfg<D, NQ>::kCtas)
+__global__ void __launch_bounds__(TileCfg<D, NQ>::kThreads, 1)
     k_paged_tile(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
                  const __grid_constant__ CUtensorMap qmap, const PagedView pv, const LineArgs a) {
     using Cfg = TileCfg<D, NQ>;
@@ -339,7 +339,9 @@ __global__ void __launch_bounds__(TileCfg<D, NQ>::kThreads, TileCfg<D, NQ>::kCta
         if (lane == 0) mbar_arrive(&bars->w_empty[i % kWorks]);
     };
     const int tb = kBlk / a.geo.G;                     // tokens of a row block
-    if (warp < kTmaWarp) regs_up<Cfg::kSoftRegs>(); else regs_down<Cfg::kRestRegs>();
+    if constexpr (NQ == 2) {
+        if (warp < kTmaWarp) regs_up<Cfg::kSoftRegs>(); else regs_down<Cfg::kRestRegs>();
+    }
     if (!any) {
         // nothing of the line for this CTA
     } else if (warp < kTmaWarp) {
@@ -758,7 +760,7 @@ bool tile_takes(const cbq_paged_cache *c) {
            c->page_stride / c->head_stride < ((int64_t)1 << 31) / (c->pages + 1) - c->kv_heads && encoder() != nullptr;
 }
 
-int tile_plan(const cbq::PagedView &pv, int d, int G, int mode, bool two, int limit, int64_t off, LinePlan *p) {
+int tile_plan(const cbq::PagedView &pv, int d, int G, int mode, bool two, int64_t off, LinePlan *p) {
     int n = 0;
     const int rc = d == 64 ? (two ? grid_of<64, 2>(&n) : grid_of<64, 1>(&n))
                            : (two ? grid_of<128, 2>(&n) : grid_of<128, 1>(&n));
@@ -773,7 +775,7 @@ int tile_plan(const cbq::PagedView &pv, int d, int G, int mode, bool two, int li
     p->geo.keys = d == 64 ? TileCfg<64, 1>::KT : TileCfg<128, 1>::KT;
     p->geo.join = 0;
     p->min_tiles = 2;                  // a part costs its CTA about as much as a tile
-    p->grid = std::min(n * sm_count(), limit);
+    p->grid = n * sm_count();
     return p->grid * 8 <= kCounts && line_room(pv, d, off, p) ? CBQ_OK : CBQ_ERR_UNSUPPORTED;
 }
 
