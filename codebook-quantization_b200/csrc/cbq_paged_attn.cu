@@ -48,6 +48,38 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+// fp32 products on the tensor cores: each factor as the sum of two tf32 values
+// (hi: rounded to 11 bits, lo: the rest, cut to as many by the instruction),
+// x y = hi hi + hi lo + lo hi.  What is left out is 2^-21 of a product, against
+// 2^-24 for an fp32 multiplication.
+__device__ __forceinline__ uint32_t tf32_hi(float x) {
+    uint32_t r;
+    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ uint32_t tf32_lo(float x, uint32_t hi) { return __float_as_uint(x - __uint_as_float(hi)); }
+__device__ __forceinline__ void mma1688(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// c += a b for NB right-hand sides given as (hi, lo) pairs of b0 and b1.
+template <int NB>
+__device__ __forceinline__ void mma_f32(float (*c)[4], const float (&a)[4], const uint32_t (*b)[4]) {
+    uint32_t h[4], l[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        h[i] = tf32_hi(a[i]);
+        l[i] = tf32_lo(a[i], h[i]);
+    }
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+        mma1688(c[nb], l, b[nb][0], b[nb][1]);
+        mma1688(c[nb], h, b[nb][2], b[nb][3]);
+        mma1688(c[nb], h, b[nb][0], b[nb][1]);
+    }
+}
+
 // ------------------------------------------------------------ configuration
 template <typename T, int D, int NB> struct StreamCfg {
     static constexpr bool kF32 = sizeof(T) == 4;
@@ -60,9 +92,7 @@ template <typename T, int D, int NB> struct StreamCfg {
     static constexpr int S = kF32 ? (D == 64 ? 2 : 3) : (D == 64 ? 4 : (D == 256 && NB > 1 ? 2 : 3));   // ring stages of a warp
     static constexpr int kPitch = D + 4;                                // merge rows, padded against bank conflicts
     static constexpr int kMerge = NW * R * (kPitch + 2) * 4;
-    static constexpr int kQ = kF32 ? R * D * 4 : 0;
-    static constexpr int kP = kF32 ? NW * kKeys * R * 4 : 0;
-    static constexpr int kSmem = NW * S * kStage + kMerge + kQ + kP;
+    static constexpr int kSmem = NW * S * kStage + kMerge;
     static constexpr int kSlot = R * D + 2 * R;                         // floats of a workspace slot
 };
 
@@ -156,12 +186,13 @@ __device__ __forceinline__ void join_unit(const LineArgs &a, const Cut &cut, int
     }
 }
 
-// bf16: the warp computes S^T = K Q^T and O^T = V^T P^T with m16n8k16, keys
-// (then dimensions of V) on the 16-row side and the query rows on the 8-column
-// side, so 1..8 query rows waste none of the long side; P^T turns into the
-// second product's operand with two 8x8 register transposes.  fp32: lane l
-// takes key l % 16 and half the 8 query rows for the scores, and D / 32
-// dimensions of all rows for the sums; fp32 FMAs.
+// The warp computes S^T = K Q^T and O^T = V^T P^T with the row-of-16 matrix
+// instructions, keys (then dimensions of V) on the 16-row side and the query
+// rows on the 8-column side, so 1..8 query rows waste none of the long side.
+// bf16: m16n8k16; P^T turns into the second product's operand with two 8x8
+// register transposes.  fp32: m16n8k8 on tf32 pairs (see mma_f32), three
+// products each: about 280 instructions for 16 keys and 8 rows where fp32 FMAs
+// fed from shared memory took 950.
 template <typename T, int D, int NB>
 __global__ void __launch_bounds__(StreamCfg<T, D, NB>::NT) k_paged_stream(const PagedView pv, const LineArgs a) {
     using Cfg = StreamCfg<T, D, NB>;
@@ -170,8 +201,6 @@ __global__ void __launch_bounds__(StreamCfg<T, D, NB>::NT) k_paged_stream(const 
     extern __shared__ __align__(128) uint8_t smem[];
     float *mO = reinterpret_cast<float *>(smem + NW * S * Cfg::kStage);  // [NW][R][kPitch]
     float *mM = mO + NW * R * kPitch, *mL = mM + NW * R;                 // [NW][R] each
-    float *sQ = mL + NW * R;                                             // fp32: [R][D]
-    float *sP = sQ + (kF32 ? R * D : 0);                                 // fp32: [NW][16][R]
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     if (a.wait_first) pdl_wait();
     pdl_launch_dependents();
@@ -229,14 +258,22 @@ __global__ void __launch_bounds__(StreamCfg<T, D, NB>::NT) k_paged_stream(const 
             };
             auto q_row = [&](int r) { return static_cast<const T *>(a.q) + row_at(r, a.qs); };
             const int lim_first = a.mode == kPrefix ? 0 : own_limit(ow, tok0);
-            if constexpr (!kF32) {
-                constexpr int KK = D / 16;
+            {
+                constexpr int KK = D / 16, KF = D / 8;   // steps of 16 (bf16) and 8 (fp32) dimensions
                 const int rq = lane >> 2, cq = (lane & 3) * 2;
-                uint32_t qf[NB][KK][2];
+                // the query rows as the first product's right-hand side; fp32: the values, split at use
+                uint32_t qf[NB][kF32 ? 1 : KK][2];
+                float qv[NB][kF32 ? KF : 1][2];
 #pragma unroll
                 for (int nb = 0; nb < NB; ++nb) {
                     const int r = nb * 8 + rq;
                     const T *qr = q_row(r < nrows ? r : 0);
+                    if constexpr (kF32) {
+#pragma unroll
+                        for (int kk = 0; kk < KF; ++kk)
+#pragma unroll
+                            for (int e = 0; e < 2; ++e) qv[nb][kk][e] = r < nrows ? qr[kk * 8 + e * 4 + (lane & 3)] : 0.f;
+                    } else
 #pragma unroll
                     for (int kk = 0; kk < KK; ++kk) {
                         qf[nb][kk][0] = r < nrows ? *reinterpret_cast<const uint32_t *>(qr + kk * 16 + cq) : 0u;
@@ -265,7 +302,25 @@ __global__ void __launch_bounds__(StreamCfg<T, D, NB>::NT) k_paged_stream(const 
                     float s[NB][4];
 #pragma unroll
                     for (int nb = 0; nb < NB; ++nb) s[nb][0] = s[nb][1] = s[nb][2] = s[nb][3] = 0.f;
-                    {
+                    if constexpr (kF32) {
+                        // a 16-byte row of an 8x8 matrix of halves is 4 floats: the same load serves tf32
+                        const int r = (lane & 7) + (lane & 8), cx = lane >> 4;
+#pragma unroll
+                        for (int kk = 0; kk < KF; ++kk) {
+                            uint32_t af[4], b[NB][4];
+                            ldsm4(kb + r * Cfg::kRowB + (((kk * 2 + cx) ^ (r & 7)) << 4), af);
+#pragma unroll
+                            for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                                for (int e = 0; e < 2; ++e) {
+                                    b[nb][e] = tf32_hi(qv[nb][kk][e]);
+                                    b[nb][e + 2] = tf32_lo(qv[nb][kk][e], b[nb][e]);
+                                }
+                            const float av[4] = {__uint_as_float(af[0]), __uint_as_float(af[1]), __uint_as_float(af[2]),
+                                                 __uint_as_float(af[3])};
+                            mma_f32<NB>(s, av, b);
+                        }
+                    } else {
                         const int r = (lane & 7) + (lane & 8), cx = lane >> 4;
 #pragma unroll
                         for (int kk = 0; kk < KK; ++kk) {
@@ -279,7 +334,7 @@ __global__ void __launch_bounds__(StreamCfg<T, D, NB>::NT) k_paged_stream(const 
                     const int key0 = (pre ? st : st - np) * kKeys;
                     const bool edge = key0 + kKeys > (pre ? ow.plen : lim_first);
                     const int ka = key0 + (lane >> 2), kc = ka + 8;
-                    uint32_t pf[NB][2];
+                    uint32_t pf[NB][2], pw[2][NB][4];        // P as the second product's right-hand side (fp32: by 8 keys)
 #pragma unroll
                     for (int nb = 0; nb < NB; ++nb) {
                         float pr[4];
@@ -309,10 +364,49 @@ __global__ void __launch_bounds__(StreamCfg<T, D, NB>::NT) k_paged_stream(const 
                                 }
                             }
                         }
-                        pf[nb][0] = movm(pack_bf16(pr[0], pr[1]));
-                        pf[nb][1] = movm(pack_bf16(pr[2], pr[3]));
+                        if constexpr (kF32) {
+                            // lane (row l / 4, key l % 4 and key + 4) from the lanes that hold the keys
+                            const int src = (lane & 3) * 4 + (lane >> 3);
+                            const bool odd = lane & 4;
+#pragma unroll
+                            for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+                                for (int e = 0; e < 2; ++e) {
+                                    const float x0 = __shfl_sync(0xffffffffu, pr[ks * 2], src + e * 16);
+                                    const float x1 = __shfl_sync(0xffffffffu, pr[ks * 2 + 1], src + e * 16);
+                                    const float x = odd ? x1 : x0;
+                                    pw[ks][nb][e] = tf32_hi(x);
+                                    pw[ks][nb][e + 2] = tf32_lo(x, pw[ks][nb][e]);
+                                }
+                        } else {
+                            pf[nb][0] = movm(pack_bf16(pr[0], pr[1]));
+                            pf[nb][1] = movm(pack_bf16(pr[2], pr[3]));
+                        }
                     }
-                    {
+                    if constexpr (kF32) {
+                        const uint8_t *vs = smem + (warp * S + it % S) * Cfg::kStage + Cfg::kHalf;
+#pragma unroll
+                        for (int i = 0; i < KK; ++i)
+#pragma unroll
+                            for (int ks = 0; ks < 2; ++ks) {
+                                float av[4], c[NB][4];
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) {
+                                    const int key = ks * 8 + (lane & 3) + (e >> 1) * 4, d = i * 16 + rq + (e & 1) * 8;
+                                    av[e] = *reinterpret_cast<const float *>(vs + key * Cfg::kRowB +
+                                                                             (((d >> 2) ^ (key & 7)) << 4) + (d & 3) * 4);
+                                }
+#pragma unroll
+                                for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                                    for (int e = 0; e < 4; ++e) c[nb][e] = o[nb][i][e];
+                                mma_f32<NB>(c, av, pw[ks]);
+#pragma unroll
+                                for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                                    for (int e = 0; e < 4; ++e) o[nb][i][e] = c[nb][e];
+                            }
+                    } else {
                         const int r = (lane & 7) + ((lane >> 4) << 3), cx = (lane >> 3) & 1;
 #pragma unroll
                         for (int i = 0; i < KK; ++i) {
@@ -343,120 +437,6 @@ __global__ void __launch_bounds__(StreamCfg<T, D, NB>::NT) k_paged_stream(const 
                             dst[i * 16 + 8] = o[nb][i][e + 2];
                         }
                     }
-            } else {
-                constexpr int NC = D / 4, E = D / 32;   // 16-byte chunks of a row; dimensions per lane
-                constexpr int EV = E < 4 ? E : 4;       // contiguous dimensions per load
-                for (int e = tid; e < R * NC; e += NT) {
-                    const int r = e / NC, c = e - r * NC;
-                    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-                    if (r < nrows) v = *reinterpret_cast<const float4 *>(q_row(r) + c * 4);
-                    *reinterpret_cast<float4 *>(sQ + e * 4) = v;
-                }
-                __syncthreads();
-                const int key = lane & 15, rh = (lane >> 4) * 4;     // this lane's key of a stage and first query row
-                int lim[4];
-                float m[4], l[4], o[8][E];
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    lim[r] = a.mode == kPrefix ? 0 : own_limit(ow, token(rh + r));
-                    m[r] = -INFINITY;
-                    l[r] = 0.f;
-                }
-#pragma unroll
-                for (int r = 0; r < 8; ++r)
-#pragma unroll
-                    for (int e = 0; e < E; ++e) o[r][e] = 0.f;
-                float *pw = sP + warp * kKeys * R;
-                for (int t = p.tb; t < p.te; ++t, ++it) {
-                    cp_wait<S - 2>();
-                    __syncwarp();
-                    issue((it + S - 1) % S);
-                    const int st = t * NW + warp;
-                    if (st >= nst) continue;
-                    const uint8_t *kb = smem + (warp * S + it % S) * Cfg::kStage, *vb = kb + Cfg::kHalf;
-                    float s[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 8
-                    for (int c = 0; c < NC; ++c) {
-                        const float4 k4 =
-                            *reinterpret_cast<const float4 *>(kb + key * Cfg::kRowB + ((c ^ (key & 7)) << 4));
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) {
-                            const float4 q4 = *reinterpret_cast<const float4 *>(sQ + (rh + r) * D + c * 4);
-                            s[r] = fmaf(q4.x, k4.x, s[r]);
-                            s[r] = fmaf(q4.y, k4.y, s[r]);
-                            s[r] = fmaf(q4.z, k4.z, s[r]);
-                            s[r] = fmaf(q4.w, k4.w, s[r]);
-                        }
-                    }
-                    const bool pre = st < np;
-                    const int kj = (pre ? st : st - np) * kKeys + key;
-                    float f[4], pr[4];
-                    bool grew = false;
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        const float x = kj < (pre ? ow.plen : lim[r]) ? s[r] * a.sc : -INFINITY;
-                        float mx = x;
-#pragma unroll
-                        for (int d = 1; d < 16; d <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
-                        const float mn = fmaxf(m[r], mx);
-                        const float mu = mn == -INFINITY ? 0.f : mn;
-                        f[r] = ex2(m[r] - mu);
-                        m[r] = mn;
-                        pr[r] = ex2(x - mu);
-                        l[r] = l[r] * f[r] + pr[r];
-                        grew |= f[r] != 1.f;
-                    }
-                    *reinterpret_cast<float4 *>(pw + key * R + rh) = make_float4(pr[0], pr[1], pr[2], pr[3]);
-                    if (__any_sync(0xffffffffu, grew)) {
-#pragma unroll
-                        for (int r = 0; r < 8; ++r) {
-                            const float fr = __shfl_sync(0xffffffffu, f[r & 3], (r >> 2) * 16);
-#pragma unroll
-                            for (int e = 0; e < E; ++e) o[r][e] *= fr;
-                        }
-                    }
-                    __syncwarp();
-#pragma unroll 4
-                    for (int k = 0; k < kKeys; ++k) {
-                        float v[E];
-#pragma unroll
-                        for (int e = 0; e < E; e += EV) {
-                            // dimensions lane*EV + (e/EV)*32*EV ..
-                            const int d0 = lane * EV + (e / EV) * 32 * EV;
-                            const uint8_t *va = vb + k * Cfg::kRowB + (((d0 >> 2) ^ (k & 7)) << 4) + (d0 & 3) * 4;
-                            if constexpr (EV == 4) {
-                                const float4 x = *reinterpret_cast<const float4 *>(va);
-                                v[e] = x.x; v[e + 1] = x.y; v[e + 2] = x.z; v[e + 3] = x.w;
-                            } else {
-                                const float2 x = *reinterpret_cast<const float2 *>(va);
-                                v[e] = x.x; v[e + 1] = x.y;
-                            }
-                        }
-                        const float4 pa = *reinterpret_cast<const float4 *>(pw + k * R);
-                        const float4 pb = *reinterpret_cast<const float4 *>(pw + k * R + 4);
-                        const float pk[8] = {pa.x, pa.y, pa.z, pa.w, pb.x, pb.y, pb.z, pb.w};
-#pragma unroll
-                        for (int r = 0; r < 8; ++r)
-#pragma unroll
-                            for (int e = 0; e < E; ++e) o[r][e] = fmaf(pk[r], v[e], o[r][e]);
-                    }
-                    __syncwarp();                      // pw is rewritten by the next stage
-                }
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    float ls = l[r];
-#pragma unroll
-                    for (int d = 1; d < 16; d <<= 1) ls += __shfl_xor_sync(0xffffffffu, ls, d);
-                    if (key == 0) {
-                        mM[warp * R + rh + r] = m[r];
-                        mL[warp * R + rh + r] = ls;
-                    }
-                }
-#pragma unroll
-                for (int r = 0; r < 8; ++r)
-#pragma unroll
-                    for (int e = 0; e < E; ++e)
-                        mO[(warp * R + r) * kPitch + lane * EV + (e / EV) * 32 * EV + e % EV] = o[r][e];
             }
             __syncthreads();
             // the NW warps' states joined in warp order; a whole unit is the
