@@ -63,9 +63,10 @@ __device__ __forceinline__ void mma1688(float (&c)[4], const uint32_t (&a)[4], u
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// c += a b for NB right-hand sides given as (hi, lo) pairs of b0 and b1.
+// c += a b for NB right-hand sides given as (hi, lo) pairs of b0 and b1; the
+// small terms go to a sum of their own (shorter chains of dependent products).
 template <int NB>
-__device__ __forceinline__ void mma_f32(float (*c)[4], const float (&a)[4], const uint32_t (*b)[4]) {
+__device__ __forceinline__ void mma_f32(float (*c)[4], float (*small)[4], const float (&a)[4], const uint32_t (*b)[4]) {
     uint32_t h[4], l[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -74,8 +75,8 @@ __device__ __forceinline__ void mma_f32(float (*c)[4], const float (&a)[4], cons
     }
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
-        mma1688(c[nb], l, b[nb][0], b[nb][1]);
-        mma1688(c[nb], h, b[nb][2], b[nb][3]);
+        mma1688(small[nb], l, b[nb][0], b[nb][1]);
+        mma1688(small[nb], h, b[nb][2], b[nb][3]);
         mma1688(c[nb], h, b[nb][0], b[nb][1]);
     }
 }
@@ -94,6 +95,7 @@ template <typename T, int D, int NB> struct StreamCfg {
     static constexpr int kMerge = NW * R * (kPitch + 2) * 4;
     static constexpr int kSmem = NW * S * kStage + kMerge;
     static constexpr int kSlot = R * D + 2 * R;                         // floats of a workspace slot
+    static constexpr int kCtas = 2 * (kSmem + 1280) <= 228 * 1024 ? 2 : 1;   // an SM's, that registers are planned for
 };
 
 // Stages of a unit that any of its rows can see.
@@ -194,7 +196,8 @@ __device__ __forceinline__ void join_unit(const LineArgs &a, const Cut &cut, int
 // products each: about 280 instructions for 16 keys and 8 rows where fp32 FMAs
 // fed from shared memory took 950.
 template <typename T, int D, int NB>
-__global__ void __launch_bounds__(StreamCfg<T, D, NB>::NT) k_paged_stream(const PagedView pv, const LineArgs a) {
+__global__ void __launch_bounds__(StreamCfg<T, D, NB>::NT, StreamCfg<T, D, NB>::kCtas)
+    k_paged_stream(const PagedView pv, const LineArgs a) {
     using Cfg = StreamCfg<T, D, NB>;
     constexpr bool kF32 = Cfg::kF32;
     constexpr int R = Cfg::R, NW = Cfg::NW, NT = Cfg::NT, S = Cfg::S, kPitch = Cfg::kPitch;
@@ -214,6 +217,9 @@ __global__ void __launch_bounds__(StreamCfg<T, D, NB>::NT) k_paged_stream(const 
         Piece lp{};
         bool lgo = next_piece(load, pv, a, w1, lp);
         int lt = lp.tb;
+        cons = load;                                   // the first piece is found once
+        Piece p = lp;
+        bool cgo = lgo;
         const uint32_t ring = smem_u32(smem) + warp * S * Cfg::kStage;
         // fills ring slot `slot` with this warp's next stage on the line, or with nothing
         auto issue = [&](int slot) {
@@ -242,8 +248,7 @@ __global__ void __launch_bounds__(StreamCfg<T, D, NB>::NT) k_paged_stream(const 
 #pragma unroll
         for (int i = 0; i < S - 1; ++i) issue(i);
         int it = 0;                                    // ring uses
-        Piece p;
-        while (next_piece(cons, pv, a, w1, p)) {
+        for (; cgo; cgo = next_piece(cons, pv, a, w1, p)) {
             const Owner &ow = cons.ow;
             const int np = (ow.plen + kKeys - 1) / kKeys, nst = unit_stages(ow, p.tt, a);
             // row r of the unit: token tok0 + r / gb, query head head0 + r % gb
@@ -305,6 +310,7 @@ __global__ void __launch_bounds__(StreamCfg<T, D, NB>::NT) k_paged_stream(const 
                     if constexpr (kF32) {
                         // a 16-byte row of an 8x8 matrix of halves is 4 floats: the same load serves tf32
                         const int r = (lane & 7) + (lane & 8), cx = lane >> 4;
+                        float part[3][NB][4] = {};     // odd steps; small terms of even and odd steps
 #pragma unroll
                         for (int kk = 0; kk < KF; ++kk) {
                             uint32_t af[4], b[NB][4];
@@ -318,8 +324,13 @@ __global__ void __launch_bounds__(StreamCfg<T, D, NB>::NT) k_paged_stream(const 
                                 }
                             const float av[4] = {__uint_as_float(af[0]), __uint_as_float(af[1]), __uint_as_float(af[2]),
                                                  __uint_as_float(af[3])};
-                            mma_f32<NB>(s, av, b);
+                            mma_f32<NB>(kk & 1 ? part[0] : s, part[1 + (kk & 1)], av, b);
                         }
+#pragma unroll
+                        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e)
+                                s[nb][e] = (s[nb][e] + part[0][nb][e]) + (part[1][nb][e] + part[2][nb][e]);
                     } else {
                         const int r = (lane & 7) + (lane & 8), cx = lane >> 4;
 #pragma unroll
@@ -386,26 +397,28 @@ __global__ void __launch_bounds__(StreamCfg<T, D, NB>::NT) k_paged_stream(const 
                     if constexpr (kF32) {
                         const uint8_t *vs = smem + (warp * S + it % S) * Cfg::kStage + Cfg::kHalf;
 #pragma unroll
-                        for (int i = 0; i < KK; ++i)
+                        for (int i = 0; i < KK; ++i) {
+                            float c[NB][4], small[NB][4] = {};
+#pragma unroll
+                            for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) c[nb][e] = o[nb][i][e];
 #pragma unroll
                             for (int ks = 0; ks < 2; ++ks) {
-                                float av[4], c[NB][4];
+                                float av[4];
 #pragma unroll
                                 for (int e = 0; e < 4; ++e) {
                                     const int key = ks * 8 + (lane & 3) + (e >> 1) * 4, d = i * 16 + rq + (e & 1) * 8;
                                     av[e] = *reinterpret_cast<const float *>(vs + key * Cfg::kRowB +
                                                                              (((d >> 2) ^ (key & 7)) << 4) + (d & 3) * 4);
                                 }
-#pragma unroll
-                                for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-                                    for (int e = 0; e < 4; ++e) c[nb][e] = o[nb][i][e];
-                                mma_f32<NB>(c, av, pw[ks]);
-#pragma unroll
-                                for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-                                    for (int e = 0; e < 4; ++e) o[nb][i][e] = c[nb][e];
+                                mma_f32<NB>(c, small, av, pw[ks]);
                             }
+#pragma unroll
+                            for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) o[nb][i][e] = c[nb][e] + small[nb][e];
+                        }
                     } else {
                         const int r = (lane & 7) + ((lane >> 4) << 3), cx = (lane >> 3) & 1;
 #pragma unroll
