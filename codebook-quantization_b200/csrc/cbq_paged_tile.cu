@@ -16,21 +16,31 @@
 // A softmax reads S into registers at once, so the next tile's S can be computed
 // while it works; P has columns of its own for that.  TMEM's 512 columns hold,
 // per row block, S (one column per key), P (half) and O (one per dimension): at
-// head_dim 128 that leaves room for 80 keys a tile, at 64 for 128.  With P over
-// S's columns and 128 keys a tile the products of a tile waited for its softmax
-// and the other way round: 943 TFLOP/s at 8192 tokens where this form has RATE.
+// head_dim 128 that leaves room for 80 keys a tile, at 64 for 128.
 //
 // Warp roles: NQ softmax warpgroups (one row block each), a warp for each block's
-// products, a TMA warp (one cp.async.bulk.tensor for 16 rows;
-// K and V tiles alternate in a ring), a warp that walks the line ahead of them
-// and leaves its pieces in shared memory.
+// products (one thread issues, in code that stays uniform to the compiler: with
+// descriptors made in vector registers a product took 90 cycles to issue and
+// the tensor pipe waited), a TMA warp (one cp.async.bulk.tensor for 16 rows; K and
+// V tiles alternate in a ring), a warp that walks the line ahead of them, leaves
+// its pieces in shared memory and fetches Q by TMA.
+//
+// Measured (B200, bf16, head_dim 128): one prompt of 8192 tokens, 32 heads on 8:
+// 552 us = 995 TFLOP/s in a short burst, 0.59 of a plain matrix product; 630 us
+// repeated for seconds, where the power limit takes the clock down.  A tile of
+// 80 keys and 256 rows takes 2250 cycles: the products 1470 (S at 80 keys is bound
+// by shared memory, 52 cycles instead of 40), both softmaxes 1280 of the
+// special-function pipe, plus the latency of a softmax's other steps (900), of
+// which two warps a scheduler hide too little.  Tried and slower: P over S's
+// columns with 128 keys a tile (943 TFLOP/s); two threads a row (950); a part of
+// the exponentials by polynomial on the FMA pipe (950); the blocks taking turns
+// at their exponentials (952); tiles copied by 16-byte asynchronous copies (618).
 // Work is the tile line of cbq_paged_line.cuh, one persistent CTA per part.
 // Every mbarrier wait is bounded; a wait that gives up sets CBQ_FLAG_TIMEOUT,
 // all roles stop at their next wait, and TMEM is released on the way out.
 #include <cuda.h>
 
 #include <mutex>
-#include <type_traits>
 
 #include "cbq_paged_line.cuh"
 
@@ -41,8 +51,6 @@ using namespace cbq;
 constexpr int kBlk = 128;              // rows of a block
 constexpr int kBox = 16;               // rows of a copy; page_size is a multiple
 constexpr float kGrow = 8.f;           // log2 growth of a row's maximum that moves its reference
-
-constexpr int kPoly = 0;               // of 16 weights, computed on the FMA pipe
 
 template <int D, int NQ> struct TileCfg {
     static constexpr int KT = D == 128 ? 80 : 128;                     // keys of a tile
@@ -199,19 +207,6 @@ __device__ __forceinline__ bool warp_wait(uint64_t *bar, uint32_t parity, Bars *
     return ok;
 }
 
-// 2^x, x <= kGrow, on the FMA pipe (the special-function pipe's 16
-// results a cycle and SM are as many as a tile's products take): x = n + f with
-// n the nearest integer (adding 1.5 * 2^23 leaves it in the low mantissa bits),
-// a cubic for 2^f on [-1/2, 1/2] fitted to the least relative error, n added to
-// the exponent.  Relative error 7.5e-5, a twenty-fifth of the rounding to bf16
-// that follows; the sum of the weights takes the same values.
-constexpr float kC0 = 0.99992806f, kC1 = 0.69326097f, kC2 = 0.24261114f, kC3 = 0.05517167f;
-__device__ __forceinline__ float ex2_fma(float x) {
-    x = fmaxf(x, -126.f);
-    const float t = x + 12582912.f, f = x - (t - 12582912.f);
-    const float y = fmaf(f, fmaf(f, fmaf(f, kC3, kC2), kC1), kC0);
-    return __uint_as_float(__float_as_uint(y) + (__float_as_uint(t) << 23));
-}
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float r;
     asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
@@ -390,10 +385,9 @@ __global__ void __launch_bounds__(TileCfg<D, NQ>::kThreads, 1)
                 }
                 const TileAt x = tile_at<KT>(plen, olen, np, t);
                 const int vis = x.pre ? x.have : min(x.have, olim - x.key0);   // visible keys of the tile
-                const bool edge = __any_sync(0xffffffffu, vis < KT);
                 // whether the products with the last P are done: asked here, needed after the weights
                 bool o_done = t > t0 && mbar_test(&bars->o_full[q], (ns - 1) & 1);
-                if (edge) {
+                if (__any_sync(0xffffffffu, vis < KT)) {
 #pragma unroll
                     for (int j = 0; j < KT; ++j)
                         if (j >= vis) s[j] = 0xff800000u;                      // -inf
@@ -413,21 +407,16 @@ __global__ void __launch_bounds__(TileCfg<D, NQ>::kThreads, 1)
                 const float mb = m == -INFINITY ? 0.f : m * sc;
                 float ls[4] = {0.f, 0.f, 0.f, 0.f};
                 uint32_t pk[KT / 2];
-                // kPoly of 16 weights by polynomial (not where keys are hidden: their weight has to be 0)
-                auto weights = [&](auto poly) {
 #pragma unroll
-                    for (int j = 0; j < KT; j += 2) {
-                        float e[2];
+                for (int j = 0; j < KT; j += 2) {
+                    float e[2];
 #pragma unroll
-                        for (int i = 0; i < 2; ++i) {
-                            const float x = fmaf(__uint_as_float(s[j + i]), sc, -mb);
-                            e[i] = decltype(poly)::value && ((j + i) * kPoly) % 16 < kPoly ? ex2_fma(x) : ex2(x);
-                            ls[(j + i) & 3] += e[i];
-                        }
-                        pk[j / 2] = pack_bf16(e[0], e[1]);
+                    for (int i = 0; i < 2; ++i) {
+                        e[i] = ex2(fmaf(__uint_as_float(s[j + i]), sc, -mb));
+                        ls[(j + i) & 3] += e[i];
                     }
-                };
-                if (edge) weights(std::false_type{}); else weights(std::true_type{});
+                    pk[j / 2] = pack_bf16(e[0], e[1]);
+                }
                 l = l * f + ((ls[0] + ls[1]) + (ls[2] + ls[3]));
                 if (t > t0) {
                     // the products with the last P are done: P may be written, O scaled
