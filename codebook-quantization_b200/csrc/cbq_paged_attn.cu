@@ -608,12 +608,10 @@ __device__ __forceinline__ void join_row(const Parts &pa, const Parts &pb, T *ds
 }
 
 // Where every unit left parts: those of the row of owner o's token tl, head (h, gi).
-__device__ __forceinline__ Parts parts_of(const JoinSource &s, const PagedView &pv, int o, const Owner &w, int tl, int h,
-                                          int gi) {
+__device__ __forceinline__ Parts parts_of(const JoinSource &s, int o, const OwnerTiles &t, int tl, int h, int gi) {
     Parts p{};
     p.s = &s;
     const uint64_t c0 = s.cum[o], all = s.cum[s.owners];
-    const OwnerTiles t = owner_tiles(w, s.geo, s.mode);
     const int tt = tl / s.geo.tq;
     if (tl < 0 || tt >= t.tt) return p;
     const uint32_t per = tiles_per_cta((uint32_t)all, (uint32_t)s.grid, (uint32_t)s.min_tiles), tiles = t.of(tt);
@@ -632,20 +630,28 @@ __device__ __forceinline__ Parts parts_of(const JoinSource &s, const PagedView &
 template <typename T, int D>
 __global__ void __launch_bounds__(128) k_join_rows(const PagedView pv, const JoinSource own, const JoinSource pre, int hq,
                                                    void *out) {
-    pdl_launch_dependents();
-    pdl_wait();
+    // lengths and tables were there before the launches that this one waits for (they let
+    // it start after their own wait): the rows' owners are found meanwhile
     const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-    if (row >= (int64_t)pv.tokens * hq) return;
-    const int t = (int)(row / hq), x = (int)(row - (int64_t)t * hq), h = x / own.geo.G, gi = x - h * own.geo.G;
+    const bool in = row < (int64_t)pv.tokens * hq;
+    const int t = in ? (int)(row / hq) : 0, x = in ? (int)(row - (int64_t)t * hq) : 0, h = x / own.geo.G, gi = x - h * own.geo.G;
     const int o = own.mode == kFull && pv.cu ? warp_upper(pv.cu, pv.seqs, t) : t;
     const Owner w = owner_of(pv, own.mode, o);
-    const Parts po = parts_of(own, pv, o, w, t - w.t0, h, gi);
-    Parts pp{};
+    const OwnerTiles tw = owner_tiles(w, own.geo, own.mode);
+    int g = 0;
+    Owner wg{};
+    OwnerTiles tg{};
     if (pre.part) {
-        const int g = warp_upper(pv.gs, pv.groups, t);
-        const Owner wg = owner_of(pv, kPrefix, g);
-        pp = parts_of(pre, pv, g, wg, t - wg.t0, h, gi);
+        g = warp_upper(pv.gs, pv.groups, t);
+        wg = owner_of(pv, kPrefix, g);
+        tg = owner_tiles(wg, pre.geo, kPrefix);
     }
+    pdl_wait();
+    pdl_launch_dependents();
+    if (!in) return;
+    const Parts po = parts_of(own, o, tw, t - w.t0, h, gi);
+    Parts pp{};
+    if (pre.part) pp = parts_of(pre, g, tg, t - wg.t0, h, gi);
     join_row<T, D>(pp, po, static_cast<T *>(out) + row * D);
 }
 
@@ -715,6 +721,24 @@ struct AttnPlan {
     int64_t bytes;
 };
 
+// The prefix's and the own rows' launches on SMs of their own, where both are
+// short: one after the other each pays its launch, plan and first loads (32
+// sequences on a prefix of 8192 rows: 45 us in turn, 38 side by side).  Long ones gain nothing and would wait for the slower of two guesses
+// (256 on 32768: 264 and 285), so they run in turn; so does fp32, whose products
+// and not the bytes take the time.  The times are guessed from the lengths'
+// bounds, own rows at half of theirs, at the rates measured on long ones.
+constexpr double kShareUs = 60.0;
+void share_sms(const cbq_paged_cache *c, const cbq_paged_batch *b, int64_t group_rows, int sms, AttnPlan *p) {
+    const double row = (double)c->kv_heads * c->head_dim * 4;
+    const double keys = (double)b->groups * ((group_rows + p->pre.rows - 1) / p->pre.rows) * p->pv.pcap;   // once per row tile
+    const double pre = p->pre_tile ? 1.2 * keys * c->kv_heads / p->pre.geo.keys / sms : keys * row / 4e6;
+    const double own = 0.5 * (double)b->seqs * p->pv.cap * row / 5e6;
+    if (p->dtype == CBQ_F32 || pre + own > kShareUs) return;
+    const int mine = std::min(std::max((int)(sms * pre / (pre + own + 1e-9) + 0.5), sms / 12), sms - sms / 12);
+    p->pre.grid = std::max(p->pre.grid / sms * mine, 1);
+    p->own.grid = std::max(p->own.grid / sms * (sms - mine), 1);
+}
+
 int plan_attn(const cbq_paged_cache *c, const cbq_paged_batch *b, int64_t tokens, int64_t q_heads, bool extend,
               AttnPlan *p) {
     *p = AttnPlan{};
@@ -759,6 +783,7 @@ int plan_attn(const cbq_paged_cache *c, const cbq_paged_batch *b, int64_t tokens
                         : stream_plan(p->pv, p->dtype, p->d, p->G, group_rows, p->bytes, &p->pre);
         if (e != CBQ_OK) return e;
         p->bytes = p->pre.end;
+        share_sms(c, b, group_rows, sms, p);
     }
     return CBQ_OK;
 }
