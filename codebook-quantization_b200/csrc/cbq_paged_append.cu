@@ -63,12 +63,15 @@ template <> struct Vec16<__nv_bfloat16> {
 // over LPH lanes.  A thread takes kHeads heads at a time: their loads go out
 // before the chain of small loads that finds the token's row and table entries,
 // and the cos / sin values serve all of them.  HBM bounds it: 16384 tokens of 48
-// heads of 128 (419 MB) take 89 us = 4.7 TB/s (147 us with one head a thread and
+// heads of 128 (419 MB) take 82 us = 5.1 TB/s (147 us with one head a thread and
 // the table chain first); one token 3.3 us, a launch and five dependent loads.
-constexpr int kThreads = 128;
-constexpr int kHeads = 3;
+//
+// Two shapes: 128 threads with 3 heads at a time (one token 3.3 us, 16384 tokens
+// 89 us), and from kManyTokens on 64 threads with 6, whose tables serve twice the
+// heads (4.2 and 82 us).
+constexpr int kManyTokens = 2048;
 
-template <typename T, int D>
+template <typename T, int D, int kThreads, int kHeads>
 __global__ void __launch_bounds__(kThreads) k_paged_append(const PagedView pv, const AppendArgs a) {
     constexpr int N = Vec16<T>::N, LPH = D / (2 * N), H = D / 2, HPP = kThreads / LPH;   // heads per pass
     pdl_launch_dependents();
@@ -172,7 +175,10 @@ __global__ void __launch_bounds__(kThreads) k_paged_append(const PagedView pv, c
 
 template <typename T, int D>
 int launch_append(const PagedView &pv, const AppendArgs &a, cudaStream_t s) {
-    CBQ_CUDA_TRY(cbq_host::launch_pdl(k_paged_append<T, D>, dim3((unsigned)pv.tokens), dim3(kThreads), 0, s, pv, a));
+    if (pv.tokens < kManyTokens)
+        CBQ_CUDA_TRY(cbq_host::launch_pdl(k_paged_append<T, D, 128, 3>, dim3((unsigned)pv.tokens), dim3(128), 0, s, pv, a));
+    else
+        CBQ_CUDA_TRY(cbq_host::launch_pdl(k_paged_append<T, D, 64, 6>, dim3((unsigned)pv.tokens), dim3(64), 0, s, pv, a));
     return CBQ_OK;
 }
 

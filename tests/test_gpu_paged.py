@@ -343,6 +343,23 @@ def test_append(dt, d, case, norm):
     assert int(status[0]) == 0
 
 
+@pytest.mark.parametrize("dt", ["bf16", "f32"])
+def test_append_many_tokens(dt):
+    """The shape that thousands of tokens take, with more heads than one pass holds."""
+    dev = need_cuda()
+    s = Setup([1500, 40, 900], new=[1400, 0, 800], d=64, dtype=DT[dt], heads=30, kv_heads=15, page=64, stale=0.0)
+    qkv = torch.randn(s.tokens, 60, 64).to(DT[dt])
+    cos, sin = tables(64, 1500)
+    kp, vp = s.pools(dev)
+    on = qkv.to(dev)
+    got = cbq.PagedKVCache(kp, vp).append_rope(s.batch(cbq, dev), on[:, :30], on[:, 30:45], on[:, 45:], cos.to(dev),
+                                               sin.to(dev))
+    ref, rk, rv = append_oracle(s, qkv[:, :30], qkv[:, 30:45], qkv[:, 45:], cos, sin, 1e-6, None, None)
+    same(got, ref)
+    same(kp, rk)
+    assert torch.equal(vp.cpu(), rv.to(DT[dt]))
+
+
 def test_append_outside_the_tables_writes_nothing():
     dev = need_cuda()
     s = Setup([33, 16, 20, 8], heads=4, kv_heads=2, d=64, stale=0.0)
