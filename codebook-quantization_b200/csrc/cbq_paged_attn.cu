@@ -723,10 +723,11 @@ struct AttnPlan {
 
 // The prefix's and the own rows' launches on SMs of their own, where both are
 // short: one after the other each pays its launch, plan and first loads (32
-// sequences on a prefix of 8192 rows: 45 us in turn, 38 side by side).  Long ones gain nothing and would wait for the slower of two guesses
-// (256 on 32768: 264 and 285), so they run in turn; so does fp32, whose products
-// and not the bytes take the time.  The times are guessed from the lengths'
-// bounds, own rows at half of theirs, at the rates measured on long ones.
+// sequences on a prefix of 8192 rows: 45 us in turn, 38 side by side).  Long
+// ones gain nothing and would wait for the slower of two guesses (256 on 32768:
+// 264 and 285), so they run in turn; so does fp32, whose products and not the
+// bytes take the time.  The times are guessed from the lengths' bounds, own
+// rows at half of theirs, at the rates measured on long ones.
 constexpr double kShareUs = 60.0;
 void share_sms(const cbq_paged_cache *c, const cbq_paged_batch *b, int64_t group_rows, int sms, AttnPlan *p) {
     const double row = (double)c->kv_heads * c->head_dim * 4;
