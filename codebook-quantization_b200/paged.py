@@ -155,6 +155,11 @@ class PagedKVCache:
         self._key = (tuple(k_pages.shape), self.dtype)
         self._index = k_pages.get_device()
 
+    def _batch(self, batch: PagedBatch) -> None:
+        """The kernels dereference the batch's addresses: they have to be this device's."""
+        if batch.device != self.device:
+            raise ValueError(f"the batch is on {batch.device}, the cache on {self.device}")
+
     def _rows(self, t: torch.Tensor, name: str, heads: int) -> int:
         """Checks [tokens, heads, head_dim] of the cache's dtype, heads and
         head_dim contiguous; the stride from token to token."""
@@ -175,6 +180,7 @@ class PagedKVCache:
         at the tokens' positions, write k and v to the cache, return the rotated
         q.  ``eps`` < 0: no RMSNorm; weights fp32 [d] or None (ones); cos / sin
         fp32 [positions, d] (``qwen3_decode.rope_tables``)."""
+        self._batch(batch)
         tokens, heads, d = q.shape
         qs, ks, vs = self._rows(q, "q", heads), self._rows(k, "k", self.kv_heads), self._rows(v, "v", self.kv_heads)
         if k.shape[0] != tokens or v.shape[0] != tokens:
@@ -204,6 +210,7 @@ class PagedKVCache:
     def workspace_bytes(self, batch: PagedBatch, tokens: int, heads: int, extend: bool) -> int:
         """Bytes of the zero-filled scratch one attention call needs; a
         ``workspace=`` tensor may serve calls of any shape that do not overlap."""
+        self._batch(batch)
         key = (self._key, tokens, heads, extend)
         n = batch._ws.get(key)
         if n is None:
@@ -213,6 +220,7 @@ class PagedKVCache:
 
     def _attend(self, name: str, extend: bool, batch: PagedBatch, q: torch.Tensor, scale: Optional[float],
                 out: Optional[torch.Tensor], workspace: Optional[torch.Tensor]) -> torch.Tensor:
+        self._batch(batch)
         tokens, heads, d = q.shape
         stride = self._rows(q, "q", heads)
         if out is None:
@@ -222,6 +230,9 @@ class PagedKVCache:
         stream = _stream(self._index)
         if workspace is None:
             workspace = self._scratch(stream, self.workspace_bytes(batch, tokens, heads, extend))
+        elif (workspace.device != self.device or workspace.dtype is not torch.uint8 or
+              not workspace.is_contiguous()):
+            raise ValueError(f"workspace: contiguous uint8 on {self.device} expected")
         _run(name, self._addr, batch._addr, tokens, q.data_ptr(), stride, heads, d ** -0.5 if scale is None else scale,
              out.data_ptr(), workspace.data_ptr(), workspace.numel(), stream)
         return out

@@ -91,3 +91,51 @@ def test_python_refusals():
                   ((t, n), dict(status=n)), ((t.T.contiguous().T, n), {})):
         with pytest.raises(ValueError):
             cbq.PagedBatch(*a, **kw)
+
+
+class Stub:
+    """A cache whose tensors are on the CPU and whose library calls are
+    recorded instead of made: what reaches the library, without a GPU."""
+
+    def __init__(self, monkeypatch, shape=(4, 2, 16, 64), strides=None):
+        self.calls = []
+        monkeypatch.setattr(cbq.paged, "_run", lambda name, *a: self.calls.append(name))
+        monkeypatch.setattr(cbq.paged, "_stream", lambda i: 0)
+        k = torch.zeros(shape) if strides is None else torch.empty_strided(shape, strides)
+        monkeypatch.setattr(cbq.paged.torch.Tensor, "is_cuda", True, raising=False)
+        self.cache = cbq.PagedKVCache(k, k.clone() if strides is None else torch.empty_strided(shape, strides))
+        self.ws = torch.zeros(1 << 20, dtype=torch.uint8)
+
+    def attend(self, b, **kw):
+        return self.cache.attend_decode(b, torch.zeros(2, 4, 64), **{"workspace": self.ws, **kw})
+
+    def append(self, b):
+        k = torch.zeros(2, 2, 64)
+        t = torch.zeros(8, 64)
+        return self.cache.append_rope(b, torch.zeros(2, 4, 64), k, k, t, t)
+
+
+def tables(device="cpu"):
+    return torch.zeros(2, 3, dtype=torch.int32, device=device), torch.zeros(2, dtype=torch.int32, device=device)
+
+
+def test_a_batch_on_another_device_is_refused(monkeypatch):
+    s = Stub(monkeypatch)
+    far = cbq.PagedBatch(*tables("meta"))
+    for call in (s.attend, s.append, lambda b: s.cache.workspace_bytes(b, 2, 4, False),
+                 lambda b: s.cache.attend_extend(b, torch.zeros(2, 4, 64), workspace=s.ws)):
+        with pytest.raises(ValueError):
+            call(far)
+    assert not s.calls
+    s.attend(cbq.PagedBatch(*tables()))
+    s.append(cbq.PagedBatch(*tables()))
+    assert s.calls == ["cbq_paged_attn_decode", "cbq_paged_append_rope"]
+
+
+@pytest.mark.parametrize("ws", [torch.empty(1 << 16, dtype=torch.uint8, device="meta"), torch.zeros(1 << 16),
+                                torch.zeros(1 << 17, dtype=torch.uint8)[::2]], ids=["device", "dtype", "strided"])
+def test_a_workspace_of_another_kind_is_refused(monkeypatch, ws):
+    s = Stub(monkeypatch)
+    with pytest.raises(ValueError):
+        s.attend(cbq.PagedBatch(*tables()), workspace=ws)
+    assert not s.calls
