@@ -67,6 +67,16 @@ def _ints(t: Optional[torch.Tensor], name: str, ndim: int, device: torch.device)
     return t
 
 
+def _row_stride(t: torch.Tensor, name: str) -> int:
+    """Entries from row to row of a table (a single row has none to step to).
+    Rows that overlap (an expanded row has stride 0) are not a layout the kernels take."""
+    n, width = t.shape
+    if n <= 1:
+        return width
+    _need(t.stride(0) >= width, f"{name}: rows {t.stride(0)} entries apart overlap ({width} wide); make it contiguous")
+    return t.stride(0)
+
+
 class PagedBatch:
     """The sequences of a step.
 
@@ -109,9 +119,9 @@ class PagedBatch:
         big = 0x7fffff00
         raw = struct.pack(
             "<qqqqqqqqqqqqqqq", n, ptr(cu_tokens), ptr(kv_lens), ptr(page_table), page_table.shape[1],
-            max(page_table.stride(0), page_table.shape[1]), big if max_kv_len is None else int(max_kv_len), groups,
+            _row_stride(page_table, "page_table"), big if max_kv_len is None else int(max_kv_len), groups,
             ptr(group_starts), ptr(prefix_lens), ptr(prefix_table), prefix_table.shape[1] if groups else 0,
-            max(prefix_table.stride(0), prefix_table.shape[1]) if groups else 0,
+            _row_stride(prefix_table, "prefix_table") if groups else 0,
             big if max_prefix_len is None else int(max_prefix_len), ptr(status))
         self._desc = ct.create_string_buffer(raw, len(raw))
         self._addr = ct.addressof(self._desc)

@@ -139,3 +139,27 @@ def test_a_workspace_of_another_kind_is_refused(monkeypatch, ws):
     with pytest.raises(ValueError):
         s.attend(cbq.PagedBatch(*tables()), workspace=ws)
     assert not s.calls
+
+
+def strides_of(b):
+    f = struct.unpack("<15q", b._desc.raw)
+    return f[5], f[12]                                 # table_stride, prefix_stride
+
+
+def test_tables_whose_rows_overlap_are_refused():
+    """An expanded row was read with a stride of its width, past its storage."""
+    n, gs, pl = torch.zeros(4, dtype=torch.int32), torch.tensor([0, 2, 4], dtype=torch.int32), torch.zeros(
+        2, dtype=torch.int32)
+    row = torch.zeros(1, 3, dtype=torch.int32)
+    for table in (row.expand(4, -1), torch.zeros(12, dtype=torch.int32).unfold(0, 6, 2)):
+        with pytest.raises(ValueError):
+            cbq.PagedBatch(table, n)
+        with pytest.raises(ValueError):
+            cbq.PagedBatch(torch.zeros(4, 3, dtype=torch.int32), n, group_starts=gs, prefix_lens=pl,
+                           prefix_table=table[:2])
+    assert strides_of(cbq.PagedBatch(row.expand(4, -1).contiguous(), n)) == (3, 0)
+    wide = torch.zeros(4, 9, dtype=torch.int32)
+    one = cbq.PagedBatch(wide[:, :3], n, group_starts=gs, prefix_lens=pl, prefix_table=wide[:2, 4:8])
+    assert strides_of(one) == (9, 9)
+    assert strides_of(cbq.PagedBatch(row.expand(1, -1), n[:1])) == (3, 0)
+    assert strides_of(cbq.PagedBatch(torch.zeros(4, 0, dtype=torch.int32), n)) == (1, 0)
