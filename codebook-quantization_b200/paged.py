@@ -50,6 +50,7 @@ def _run(name: str, *args) -> None:
 # torch.cuda.current_stream builds a Stream object; the raw handle is all that is passed on
 _stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
 _capturing = torch.cuda.is_current_stream_capturing
+_current = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
 def _need(ok: bool, what: str) -> None:
@@ -190,6 +191,9 @@ class PagedKVCache:
         at the tokens' positions, write k and v to the cache, return the rotated
         q.  ``eps`` < 0: no RMSNorm; weights fp32 [d] or None (ones); cos / sin
         fp32 [positions, d] (``qwen3_decode.rope_tables``)."""
+        if _current() != self._index:                  # the library launches on the current device
+            with torch.cuda.device(self._index):
+                return self.append_rope(batch, q, k, v, cos, sin, eps, q_weight, k_weight, out)
         self._batch(batch)
         tokens, heads, d = q.shape
         qs, ks, vs = self._rows(q, "q", heads), self._rows(k, "k", self.kv_heads), self._rows(v, "v", self.kv_heads)
@@ -220,6 +224,9 @@ class PagedKVCache:
     def workspace_bytes(self, batch: PagedBatch, tokens: int, heads: int, extend: bool) -> int:
         """Bytes of the zero-filled scratch one attention call needs; a
         ``workspace=`` tensor may serve calls of any shape that do not overlap."""
+        if _current() != self._index:
+            with torch.cuda.device(self._index):
+                return self.workspace_bytes(batch, tokens, heads, extend)
         self._batch(batch)
         key = (self._key, tokens, heads, extend)
         n = batch._ws.get(key)
@@ -230,6 +237,9 @@ class PagedKVCache:
 
     def _attend(self, name: str, extend: bool, batch: PagedBatch, q: torch.Tensor, scale: Optional[float],
                 out: Optional[torch.Tensor], workspace: Optional[torch.Tensor]) -> torch.Tensor:
+        if _current() != self._index:
+            with torch.cuda.device(self._index):
+                return self._attend(name, extend, batch, q, scale, out, workspace)
         self._batch(batch)
         tokens, heads, d = q.shape
         stride = self._rows(q, "q", heads)

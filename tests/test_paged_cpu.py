@@ -1,4 +1,5 @@
 """What the paged-cache operators refuse, on the host, before any CUDA call."""
+import contextlib
 import ctypes as ct
 import struct
 
@@ -98,8 +99,9 @@ class Stub:
     recorded instead of made: what reaches the library, without a GPU."""
 
     def __init__(self, monkeypatch, shape=(4, 2, 16, 64), strides=None):
-        self.calls = []
-        monkeypatch.setattr(cbq.paged, "_run", lambda name, *a: self.calls.append(name))
+        self.calls, self.device = [], -1               # a CPU tensor's device number
+        monkeypatch.setattr(cbq.paged, "_run", lambda name, *a: self.calls.append((name, self.device)))
+        monkeypatch.setattr(cbq.paged, "_current", lambda: self.device, raising=False)
         monkeypatch.setattr(cbq.paged, "_stream", lambda i: 0)
         k = torch.zeros(shape) if strides is None else torch.empty_strided(shape, strides)
         monkeypatch.setattr(cbq.paged.torch.Tensor, "is_cuda", True, raising=False)
@@ -129,7 +131,7 @@ def test_a_batch_on_another_device_is_refused(monkeypatch):
     assert not s.calls
     s.attend(cbq.PagedBatch(*tables()))
     s.append(cbq.PagedBatch(*tables()))
-    assert s.calls == ["cbq_paged_attn_decode", "cbq_paged_append_rope"]
+    assert [c for c, _ in s.calls] == ["cbq_paged_attn_decode", "cbq_paged_append_rope"]
 
 
 @pytest.mark.parametrize("ws", [torch.empty(1 << 16, dtype=torch.uint8, device="meta"), torch.zeros(1 << 16),
@@ -163,3 +165,25 @@ def test_tables_whose_rows_overlap_are_refused():
     assert strides_of(one) == (9, 9)
     assert strides_of(cbq.PagedBatch(row.expand(1, -1), n[:1])) == (3, 0)
     assert strides_of(cbq.PagedBatch(torch.zeros(4, 0, dtype=torch.int32), n)) == (1, 0)
+
+
+def test_calls_run_on_the_device_of_the_cache(monkeypatch):
+    """The library launches on the current device, which may be another one."""
+    s = Stub(monkeypatch)
+    entered = []
+
+    @contextlib.contextmanager
+    def device(index):
+        entered.append(index)
+        was, s.device = s.device, index
+        yield
+        s.device = was
+
+    monkeypatch.setattr(torch.cuda, "device", device)
+    s.device = 3
+    s.attend(cbq.PagedBatch(*tables()))
+    s.append(cbq.PagedBatch(*tables()))
+    assert [d for _, d in s.calls] == [-1, -1] and entered == [-1, -1] and s.device == 3
+    s.device = -1
+    s.attend(cbq.PagedBatch(*tables()))
+    assert len(entered) == 2
