@@ -94,11 +94,13 @@ __global__ void __launch_bounds__(kThreads) k_paged_append(const PagedView pv, c
         }
     };
     fetch(0);
-    // the token's sequence, row, position and page
+    // the token's sequence, row, position and page; a token outside cu[0] .. cu[seqs] - 1
+    // (a captured step with fewer tokens than it was captured for) has no row
     int s = t, row;
     if (pv.cu) {
         s = warp_upper(pv.cu, pv.seqs, t);
-        row = pv.lens[s] - pv.cu[s + 1] + t;
+        const int first = pv.cu[s], end = pv.cu[s + 1];
+        row = t >= first && t < end ? pv.lens[s] - end + t : -1;
     } else {
         row = pv.lens[s] - 1;
     }

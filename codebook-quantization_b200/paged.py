@@ -83,7 +83,9 @@ class PagedBatch:
 
     ``page_table`` int32 [seqs, width], ``kv_lens`` int32 [seqs] (rows of each
     sequence, its new tokens included); ``cu_tokens`` int32 [seqs + 1]: where
-    each sequence's new tokens begin (None: one token each).  Shared prefixes:
+    each sequence's new tokens begin (None: one token each); tokens outside
+    ``cu_tokens[0] .. cu_tokens[-1] - 1`` belong to no sequence (a captured
+    step may hold fewer than it was captured for).  Shared prefixes:
     group g holds the sequences ``group_starts[g] .. group_starts[g+1] - 1``
     and its prefix the first ``prefix_lens[g]`` rows of the pages in
     ``prefix_table[g]``.  ``max_kv_len`` / ``max_prefix_len`` bound the values

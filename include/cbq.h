@@ -561,7 +561,8 @@ typedef struct cbq_paged_cache {
 
 typedef struct cbq_paged_batch {
     int64_t seqs;                       /* at most 65536 */
-    const int32_t *cu_tokens_dev;       /* [seqs + 1] first new token of each sequence; NULL: one each */
+    const int32_t *cu_tokens_dev;       /* [seqs + 1] first new token of each sequence, never falling; tokens before
+                                           cu[0] or from cu[seqs] on belong to none; NULL: one each */
     const int32_t *kv_lens_dev;         /* [seqs] rows of each sequence, its new tokens included */
     const int32_t *page_table_dev;      /* [seqs][table_stride], table_width entries in use */
     int64_t table_width, table_stride;
@@ -584,8 +585,9 @@ typedef struct cbq_paged_batch {
  * token's row of the cache: row kv_lens[s] - T_s + i for the i-th of the T_s
  * new tokens of sequence s.  fp32 throughout, each value rounded once.  A
  * token whose row is negative (a sequence that is switched off has kv_len 0)
- * is skipped and its q_out row is zero; so is one whose row, page or position
- * lies outside the tables, which also sets CBQ_FLAG_CORRUPT. */
+ * or that belongs to no sequence is skipped and its q_out row is zero; so is
+ * one whose row, page or position lies outside the tables, which also sets
+ * CBQ_FLAG_CORRUPT. */
 int cbq_paged_append_rope(const cbq_paged_cache *cache, const cbq_paged_batch *batch, int64_t tokens,
                           const void *q_dev, int64_t q_stride, const void *k_dev, int64_t k_stride,
                           const void *v_dev, int64_t v_stride, int64_t q_heads, float eps,

@@ -378,3 +378,30 @@ def test_append_outside_the_tables_writes_nothing():
     kp[page], vp[page] = k0[page], v0[page]
     assert torch.equal(kp, k0) and torch.equal(vp, v0)
     assert int(status[0]) & L.FLAG_CORRUPT and int(status[2]) == 3
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f32"])
+@pytest.mark.parametrize("pad", [(0, 5), (3, 0), (2, 2100)], ids=str)
+def test_append_skips_tokens_of_no_sequence(dt, pad):
+    """Tokens before the first sequence's or behind the last one's: nothing
+    written (the table's unused entries name another sequence's page), zeros back."""
+    dev = need_cuda()
+    s = Setup([20, 30, 12], new=[7, 1, 12], heads=4, kv_heads=2, d=64, dtype=DT[dt], slack=200, stale=0.0)
+    s.table = torch.where(s.table < 0, s.table[0, 0], s.table)
+    before, behind = pad
+    n = s.tokens + before + behind
+    qkv = torch.randn(n, 8, 64).to(DT[dt])
+    mine = qkv[before:before + s.tokens]
+    cos, sin = tables(64, 3000)
+    kp, vp = s.pools(dev)
+    status = cbq.PagedBatch.new_status(dev)
+    b = s.batch(cbq, dev, status=status)
+    b.cu_tokens.add_(before)
+    on = qkv.to(dev)
+    got = cbq.PagedKVCache(kp, vp).append_rope(b, on[:, :4], on[:, 4:6], on[:, 6:], cos.to(dev), sin.to(dev))
+    ref, rk, rv = append_oracle(s, mine[:, :4], mine[:, 4:6], mine[:, 6:], cos, sin, 1e-6, None, None)
+    same(got[before:before + s.tokens], ref)
+    same(kp, rk)
+    assert torch.equal(vp.cpu(), rv.to(DT[dt]))
+    assert not got[:before].any() and not got[before + s.tokens:].any()
+    assert int(status[0]) == 0
