@@ -218,7 +218,9 @@ __global__ void __launch_bounds__(StreamCfg<T, D, NB>::NT, StreamCfg<T, D, NB>::
     Cursor cons{};
     uint32_t w1 = 0, per = 1;
     __shared__ int last;
+    const Ends ends = token_ends(pv, a);
     const bool any = plan_line<NT>(pv, a, cons, w1, per);
+    zero_rest<T>(pv, a, ends, D, NT);
     if (any) {
         Cursor load = cons;
         Piece lp{};
@@ -607,13 +609,15 @@ __device__ __forceinline__ void join_row(const Parts &pa, const Parts &pb, T *ds
     }
 }
 
-// Where every unit left parts: those of the row of owner o's token tl, head (h, gi).
-__device__ __forceinline__ Parts parts_of(const JoinSource &s, int o, const OwnerTiles &t, int tl, int h, int gi) {
+// Where every unit left parts: those of the row of token tok, head (h, gi), of
+// owner o; none where the token is not the owner's.
+__device__ __forceinline__ Parts parts_of(const JoinSource &s, int o, const Owner &w, const OwnerTiles &t, int tok, int h,
+                                          int gi) {
     Parts p{};
     p.s = &s;
     const uint64_t c0 = s.cum[o], all = s.cum[s.owners];
-    const int tt = tl / s.geo.tq;
-    if (tl < 0 || tt >= t.tt) return p;
+    const int tl = tok - w.t0, tt = tl / s.geo.tq;
+    if (tl < 0 || tl >= w.nt) return p;
     const uint32_t per = tiles_per_cta((uint32_t)all, (uint32_t)s.grid, (uint32_t)s.min_tiles), tiles = t.of(tt);
     const int nhc = s.geo.hc, hc = nhc > 1 ? gi / s.rows : 0;
     const uint32_t u = (uint32_t)((h * t.tt + tt) * nhc + hc);
@@ -649,9 +653,9 @@ __global__ void __launch_bounds__(128) k_join_rows(const PagedView pv, const Joi
     pdl_wait();
     pdl_launch_dependents();
     if (!in) return;
-    const Parts po = parts_of(own, o, tw, t - w.t0, h, gi);
+    const Parts po = parts_of(own, o, w, tw, t, h, gi);
     Parts pp{};
-    if (pre.part) pp = parts_of(pre, g, tg, t - wg.t0, h, gi);
+    if (pre.part) pp = parts_of(pre, g, wg, tg, t, h, gi);
     join_row<T, D>(pp, po, static_cast<T *>(out) + row * D);
 }
 

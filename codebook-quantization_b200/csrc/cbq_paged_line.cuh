@@ -160,6 +160,30 @@ __device__ __forceinline__ OwnerTiles owner_tiles(const Owner &w, const LineGeo 
     return t;
 }
 
+// Extend: the tokens before the first sequence's and behind the last one's
+// belong to none; their rows of the result (a.hq * d elements each) are zeros.
+// `hi` and `lo` are asked for before the plan, whose own loads hide theirs.
+struct Ends {
+    int lo, hi;
+};
+__device__ __forceinline__ Ends token_ends(const PagedView &pv, const LineArgs &a) {
+    Ends e{0, pv.tokens};
+    if (a.direct && a.mode == kFull && pv.cu) {
+        e.lo = pv.cu[0];
+        e.hi = pv.cu[pv.seqs];
+    }
+    return e;
+}
+template <typename T>
+__device__ __forceinline__ void zero_rest(const PagedView &pv, const LineArgs &a, Ends e, int d, int threads) {
+    const int lo = clampi(e.lo, 0, pv.tokens), hi = clampi(e.hi, lo, pv.tokens);
+    if (lo == 0 && hi == pv.tokens) return;
+    const int64_t row = (int64_t)a.hq * d * (int)sizeof(T) / 16, skip = (hi - lo) * row;   // in 16 bytes
+    const int64_t n = pv.tokens * row - skip;
+    for (int64_t i = (int64_t)blockIdx.x * threads + threadIdx.x; i < n; i += (int64_t)gridDim.x * threads)
+        static_cast<uint4 *>(a.out)[i < lo * row ? i : i + skip] = make_uint4(0u, 0u, 0u, 0u);
+}
+
 struct Piece {
     int h, tt, hc, tiles, tb, te;      // a unit of the cursor's owner, its tiles, the piece [tb, te) of them
 };

@@ -321,7 +321,9 @@ __global__ void __launch_bounds__(TileCfg<D, NQ>::kThreads, 1)
     const uint32_t tmem = __shfl_sync(0xffffffffu, bars->tmem, 0);
     Cursor c{};
     uint32_t w1 = 0, per = 1;
+    const Ends ends = token_ends(pv, a);
     const bool any = plan_line<Cfg::kThreads>(pv, a, c, w1, per);
+    zero_rest<__nv_bfloat16>(pv, a, ends, D, Cfg::kThreads);
 
     // The i-th piece (0 where the line ends or a wait gave up); done(i) gives its place back.
     auto work = [&](uint32_t i) -> const Work * {

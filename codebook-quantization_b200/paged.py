@@ -282,5 +282,5 @@ class PagedKVCache:
                       out: Optional[torch.Tensor] = None, workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
         """q [tokens, heads, d], the sequences' new tokens one after the other
         (``cu_tokens``) -> [tokens, heads, d]; token i of sequence s sees the
-        prefix and the rows up to its own."""
+        prefix and the rows up to its own; tokens of no sequence give zeros."""
         return self._attend("cbq_paged_attn_extend", True, batch, q, scale, out, workspace)

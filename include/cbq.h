@@ -620,7 +620,8 @@ int cbq_paged_attn_decode(const cbq_paged_cache *cache, const cbq_paged_batch *b
 
 /* Attention of any number of new tokens per sequence (cu_tokens_dev; NULL:
  * one each) over the prefix and the sequence's own rows, causally: the i-th
- * of the T_s new tokens sees the prefix and own rows 0 .. kv_lens[s] - T_s + i.
+ * of the T_s new tokens sees the prefix and own rows 0 .. kv_lens[s] - T_s + i;
+ * a token that belongs to no sequence gives zeros.
  * Otherwise as cbq_paged_attn_decode.  A non-finite value in a later row of
  * the same sequence may reach earlier tokens of the same call. */
 int cbq_paged_attn_extend(const cbq_paged_cache *cache, const cbq_paged_batch *batch, int64_t tokens,

@@ -405,3 +405,68 @@ def test_append_skips_tokens_of_no_sequence(dt, pad):
     assert torch.equal(vp.cpu(), rv.to(DT[dt]))
     assert not got[:before].any() and not got[before + s.tokens:].any()
     assert int(status[0]) == 0
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f32"])
+@pytest.mark.parametrize("pad", [(0, 5), (3, 0), (2, 300)], ids=str)
+@pytest.mark.parametrize("kv,new", [([20, 30, 12], [7, 1, 12]), ([700, 50], [600, 50]), ([2000], [100]), ([8, 8], [0, 0])],
+                         ids=["few", "many", "long", "none"])
+def test_extend_gives_zeros_for_tokens_of_no_sequence(dt, kv, new, pad):
+    """Row and tile kernel, results written by the units and by the join."""
+    dev = need_cuda()
+    s = Setup(kv, new=new, heads=8, kv_heads=2, d=64, dtype=DT[dt], page=64)
+    before, behind = pad
+    n = s.tokens + before + behind
+    k, v = s.pools(dev)
+    b = s.batch(cbq, dev)
+    b.cu_tokens.add_(before)
+    q = torch.randn(n, 8, 64, device=dev).to(DT[dt])
+    q[before:before + s.tokens] = s.q.to(dev)
+    out = torch.full_like(q, float("nan"))
+    cbq.PagedKVCache(k, v).attend_extend(b, q, out=out)
+    assert not out[:before].any() and not out[before + s.tokens:].any()
+    if s.tokens:
+        check_attention(out[before:before + s.tokens], *s.attention(64 ** -0.5, True))
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f32"])
+def test_captured_step_with_fewer_tokens_than_captured(dt):
+    """Append and extend in one graph; the token counts change between replays."""
+    dev = need_cuda()
+    n = 24
+    s = Setup([40, 24, 9], new=[10, 8, 6], heads=4, kv_heads=2, d=64, dtype=DT[dt], stale=0.0, slack=2)
+    s.table = torch.where(s.table < 0, s.table[0, 0], s.table)
+    cos, sin = (t.to(dev) for t in tables(64, 200))
+    kp, vp = s.pools(dev)
+    b, c = s.batch(cbq, dev), cbq.PagedKVCache(kp, vp)
+    qkv = torch.randn(n, 8, 64, device=dev).to(DT[dt])
+    out = torch.empty(n, 4, 64, dtype=DT[dt], device=dev)
+
+    def step():
+        q = c.append_rope(b, qkv[:, :4], qkv[:, 4:6], qkv[:, 6:], cos, sin)
+        c.attend_extend(b, q, out=out)
+        return q
+
+    k0, v0 = kp.clone(), vp.clone()
+    step()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        rotated = step()
+    for new in ([10, 8, 6], [1, 1, 1], [3, 0, 0], [0, 0, 0], [10, 8, 6]):
+        kp.copy_(k0)
+        vp.copy_(v0)
+        s.new, s.tokens = new, sum(new)
+        b.cu_tokens.copy_(torch.tensor([0] + torch.tensor(new).cumsum(0).tolist(), dtype=torch.int32))
+        g.replay()
+        torch.cuda.synchronize()
+        on = qkv[:s.tokens].cpu()
+        s.k, s.v = k0.cpu(), v0.cpu()
+        ref, rk, rv = append_oracle(s, on[:, :4], on[:, 4:6], on[:, 6:], cos.cpu(), sin.cpu(), 1e-6, None, None)
+        same(rotated[:s.tokens], ref)
+        same(kp, rk)
+        assert torch.equal(vp.cpu(), rv.to(DT[dt]))
+        assert not rotated[s.tokens:].any() and not out[s.tokens:].any()
+        if s.tokens:
+            s.k, s.v, s.q = kp.cpu(), vp.cpu(), rotated[:s.tokens].cpu()
+            check_attention(out[:s.tokens], *s.attention(64 ** -0.5, True))
