@@ -822,6 +822,15 @@ int join_launch(const AttnPlan &p, const LineArgs &own, const JoinSource &so, co
     return CBQ_OK;
 }
 
+// Held over a call's launches: they pass parts to one another through the
+// workspace, which another thread's call on the same stream may share, and in
+// stream order that call must come before all of them or behind.
+std::mutex &launch_mutex(cudaStream_t s) {
+    static std::mutex mu[64];
+    const uintptr_t h = reinterpret_cast<uintptr_t>(s);
+    return mu[(h ^ h >> 6 ^ h >> 12) & 63];
+}
+
 int paged_attn(const cbq_paged_cache *c, const cbq_paged_batch *b, int64_t tokens, const void *q, int64_t q_stride,
                int64_t q_heads, float scale, void *out, void *ws, int64_t ws_bytes, bool extend, cudaStream_t s) {
     AttnPlan p;
@@ -847,6 +856,7 @@ int paged_attn(const cbq_paged_cache *c, const cbq_paged_batch *b, int64_t token
                           reinterpret_cast<const uint64_t *>(w + lp.cum_off), lp.slots, lp.owners, lp.grid, lp.min_tiles,
                           lp.rows, lp.tile_rows, lp.mode, lp.geo};
     };
+    std::lock_guard<std::mutex> guard(launch_mutex(s));
     if (p.prefix) {
         if ((rc = run_line(c, p, p.pre, p.pre_tile, line_args(p.pre, a, w), s)) != CBQ_OK) return rc;
         a.wait_first = 0;                              // the prefix launch passed its wait before this one can start

@@ -28,7 +28,8 @@ from . import _lib
 __all__ = ["PagedKVCache", "PagedBatch"]
 
 # Zero-filled scratch of the attention calls, one growing buffer per stream: calls
-# on one stream do not overlap, and each leaves its arrival counters zero.
+# on one stream do not overlap (the library keeps a call's launches together,
+# whatever other host threads do), and each leaves its arrival counters zero.
 _WORKSPACES = {}
 
 _F32 = torch.float32

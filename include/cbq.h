@@ -598,7 +598,8 @@ int cbq_paged_append_rope(const cbq_paged_cache *cache, const cbq_paged_batch *b
  * cbq_paged_attn_extend (extend = 1).  The caller zero-fills the workspace
  * once; every call leaves its arrival counters zero, so calls of any shape may
  * share one, as long as they do not overlap on the GPU (the same stream is
- * fine).  After CBQ_FLAG_TIMEOUT it has to be zeroed again.  -1: arguments the
+ * fine, from several host threads too: the launches of a call stay together).
+ * After CBQ_FLAG_TIMEOUT it has to be zeroed again.  -1: arguments the
  * functions refuse. */
 int64_t cbq_paged_attn_workspace_bytes(const cbq_paged_cache *cache, const cbq_paged_batch *batch,
                                        int64_t tokens, int64_t q_heads, int extend);

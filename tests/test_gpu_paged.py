@@ -2,6 +2,8 @@
 over shared prefixes, attention of prompts, each against a 64-bit oracle that
 works sequence by sequence; bounds as derived in ``paged_helpers``."""
 import math
+import sys
+import threading
 
 import pytest
 import torch
@@ -470,3 +472,40 @@ def test_captured_step_with_fewer_tokens_than_captured(dt):
         if s.tokens:
             s.k, s.v, s.q = kp.cpu(), vp.cpu(), rotated[:s.tokens].cpu()
             check_attention(out[:s.tokens], *s.attention(64 ** -0.5, True))
+
+
+def test_threads_that_share_a_stream():
+    """A call is up to three launches over the stream's scratch; those of another
+    thread's call must not come between them."""
+    dev = need_cuda()
+    cases = [(Setup([40, 0, 300, 17], groups=[(4, 500)], heads=8, kv_heads=2, d=128, seed=1), "decode"),
+             (Setup([(9 * i) % 90 for i in range(30)], groups=[(10, 90), (20, 700)], heads=8, kv_heads=2, d=64, seed=2),
+              "decode"),
+             (Setup([700, 90], new=[60, 30], heads=8, kv_heads=2, d=128, seed=3), "extend"),
+             (Setup([25, 600], groups=[(2, 77)], heads=8, kv_heads=2, d=64, dtype=torch.float32, seed=4), "decode")]
+    calls = []
+    for s, op in cases:
+        k, v = s.pools(dev)
+        c, b, q = cbq.PagedKVCache(k, v), s.batch(cbq, dev, decode=op == "decode"), s.q.to(dev)
+        f = c.attend_decode if op == "decode" else c.attend_extend
+        calls.append((f, b, q, f(b, q)))
+    torch.cuda.synchronize()
+    wrong, interval = [], sys.getswitchinterval()
+    start = threading.Barrier(len(calls))
+
+    def work(i):
+        f, b, q, want = calls[i]
+        start.wait()
+        outs = [f(b, q) for _ in range(300)]
+        wrong.append(sum(not torch.equal(o, want) for o in outs))
+
+    sys.setswitchinterval(1e-6)
+    try:
+        threads = [threading.Thread(target=work, args=(i,)) for i in range(len(calls))]
+        for t in threads:
+            t.start()
+        for t in threads:
+            t.join()
+    finally:
+        sys.setswitchinterval(interval)
+    assert wrong == [0] * len(calls)
