@@ -218,9 +218,10 @@ __global__ void __launch_bounds__(StreamCfg<T, D, NB>::NT, StreamCfg<T, D, NB>::
     Cursor cons{};
     uint32_t w1 = 0, per = 1;
     __shared__ int last;
+    __shared__ LineStart start;
     const Ends ends = token_ends(pv, a);
-    const bool any = plan_line<NT>(pv, a, cons, w1, per);
-    zero_rest<T>(pv, a, ends, D, NT);
+    const bool any = plan_line<NT>(pv, a, start, cons, w1, per);
+    zero_rest<T, D>(pv, a, ends);
     if (any) {
         Cursor load = cons;
         Piece lp{};

@@ -162,7 +162,7 @@ __device__ __forceinline__ OwnerTiles owner_tiles(const Owner &w, const LineGeo 
 
 // Extend: the tokens before the first sequence's and behind the last one's
 // belong to none; their rows of the result (a.hq * d elements each) are zeros.
-// `hi` and `lo` are asked for before the plan, whose own loads hide theirs.
+// They are asked for before the plan, whose own loads hide theirs.
 struct Ends {
     int lo, hi;
 };
@@ -174,14 +174,17 @@ __device__ __forceinline__ Ends token_ends(const PagedView &pv, const LineArgs &
     }
     return e;
 }
-template <typename T>
-__device__ __forceinline__ void zero_rest(const PagedView &pv, const LineArgs &a, Ends e, int d, int threads) {
-    const int lo = clampi(e.lo, 0, pv.tokens), hi = clampi(e.hi, lo, pv.tokens);
-    if (lo == 0 && hi == pv.tokens) return;
-    const int64_t row = (int64_t)a.hq * d * (int)sizeof(T) / 16, skip = (hi - lo) * row;   // in 16 bytes
-    const int64_t n = pv.tokens * row - skip;
-    for (int64_t i = (int64_t)blockIdx.x * threads + threadIdx.x; i < n; i += (int64_t)gridDim.x * threads)
-        static_cast<uint4 *>(a.out)[i < lo * row ? i : i + skip] = make_uint4(0u, 0u, 0u, 0u);
+// `row`: 16-byte pieces of a row.
+static __device__ __noinline__ void zero_rows(void *out, int lo, int hi, int tokens, int row) {
+    lo = clampi(lo, 0, tokens);
+    hi = clampi(hi, lo, tokens);
+    const int64_t head = (int64_t)lo * row, skip = (int64_t)(hi - lo) * row, n = (int64_t)tokens * row - skip;
+    for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (int64_t)gridDim.x * blockDim.x)
+        static_cast<uint4 *>(out)[i < head ? i : i + skip] = make_uint4(0u, 0u, 0u, 0u);
+}
+template <typename T, int D>
+__device__ __forceinline__ void zero_rest(const PagedView &pv, const LineArgs &a, Ends e) {
+    if (e.lo > 0 || e.hi < pv.tokens) zero_rows(a.out, e.lo, e.hi, pv.tokens, a.hq * (D * (int)sizeof(T) / 16));
 }
 
 struct Piece {
@@ -280,14 +283,21 @@ __host__ __device__ __forceinline__ uint32_t tiles_per_cta(uint32_t W, uint32_t 
     return per > least ? per : least;
 }
 
-// Of this CTA: its part [c.w, w1) of the line and the owner it begins in;
-// false: nothing to do.  Unless direct, CTA 0 leaves the sums before each owner
-// in a.cum.  All NT threads call it.
+// A CTA's part of the line, in shared memory.
+struct LineStart {
+    Cursor c;
+    uint32_t w1, per;
+};
+
+// Of this CTA: its part [c.w, w1) of the line and the owner it begins in (left
+// in `start` too); false: nothing to do.  Unless direct, CTA 0 leaves the sums
+// before each owner in a.cum.  All NT threads call it.
 template <int NT>
-__device__ __forceinline__ bool plan_line(const PagedView &pv, const LineArgs &a, Cursor &c, uint32_t &w1, uint32_t &per) {
+__device__ __forceinline__ bool plan_line(const PagedView &pv, const LineArgs &a, LineStart &start, Cursor &c, uint32_t &w1,
+                                          uint32_t &per) {
     constexpr int NW = NT / 32;
     __shared__ uint64_t red[2 * NW];
-    __shared__ Cursor at;                              // written by the thread whose owner holds w0
+    Cursor &at = start.c;                              // written by the thread whose owner holds w0
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const bool writer = blockIdx.x == 0 && !a.direct;
     const uint32_t per_unit = (uint32_t)(pv.kv_heads * a.geo.hc);
@@ -349,6 +359,8 @@ __device__ __forceinline__ bool plan_line(const PagedView &pv, const LineArgs &a
                 at.ow = w;
                 at.tl = tl;
                 at.p.tiles = 0;
+                start.w1 = w1;
+                start.per = per;
             }
         }
         run += all;

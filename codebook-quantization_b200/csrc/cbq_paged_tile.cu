@@ -271,13 +271,33 @@ __device__ __forceinline__ void join_block(const LineArgs &a, const Cut &cut, in
     }
 }
 
+// The arrivals that a softmax warp still owes at cut units once a wait has
+// given up (it made those of its first `done` pieces), so that the counters are
+// zero after such a call too.  Every CTA walks its own part, whatever the
+// others did; a unit that is joined from parts nobody wrote is reported.
+__device__ __noinline__ void settle(const PagedView &pv, const LineArgs &a, const LineStart &st, uint32_t done) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, tb = kBlk / a.geo.G;
+    const int q = warp >> 2, rt = ((warp & 3) * 32 + lane) / a.geo.G;
+    Cursor c = st.c;
+    Piece p{};
+    for (uint32_t i = 0; next_piece(c, pv, a, st.w1, p); ++i) {
+        const bool live = rt < tb && p.tt * a.geo.tq + q * tb + rt < c.ow.nt;
+        if (i < done || (p.tb == 0 && p.te == p.tiles) || !__any_sync(0xffffffffu, live)) continue;
+        const Cut cut = cut_of(c, p, st.per);
+        uint32_t *cnt = a.count + cut.i0 * 8 + warp;
+        if (lane == 0 && atomicAdd(cnt, 1u) == (uint32_t)(cut.n - 1)) *cnt = 0u;
+        __syncwarp();
+    }
+}
+
 template <int N> __device__ __forceinline__ void regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N> __device__ __forceinline__ void regs_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 
 template <int D, int NQ>
 __global__ void __launch_bounds__(TileCfg<D, NQ>::kThreads, 1)
     k_paged_tile(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
-                 const __grid_constant__ CUtensorMap qmap, const PagedView pv, const LineArgs a) {
+                 const __grid_constant__ CUtensorMap qmap, const __grid_constant__ PagedView pv,
+                 const __grid_constant__ LineArgs a) {
     using Cfg = TileCfg<D, NQ>;
     constexpr int kSlots = Cfg::kSlots, kTileB = Cfg::kTileB, KT = Cfg::KT;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -322,8 +342,9 @@ __global__ void __launch_bounds__(TileCfg<D, NQ>::kThreads, 1)
     Cursor c{};
     uint32_t w1 = 0, per = 1;
     const Ends ends = token_ends(pv, a);
-    const bool any = plan_line<Cfg::kThreads>(pv, a, c, w1, per);
-    zero_rest<__nv_bfloat16>(pv, a, ends, D, Cfg::kThreads);
+    __shared__ LineStart start;
+    const bool any = plan_line<Cfg::kThreads>(pv, a, start, c, w1, per);
+    zero_rest<__nv_bfloat16, D>(pv, a, ends);
 
     // The i-th piece (0 where the line ends or a wait gave up); done(i) gives its place back.
     auto work = [&](uint32_t i) -> const Work * {
@@ -503,6 +524,7 @@ __global__ void __launch_bounds__(TileCfg<D, NQ>::kThreads, 1)
             ++nw;
             w = work(nw);
         }
+        if (a.direct && *(volatile int *)&bars->abort_flag) settle(pv, a, start, nw);
     } else if (warp == kTmaWarp) {
         // ------------------------------------------------------------- K and V tiles
         uint32_t n = 0, nw = 0;                        // tiles issued (K and V), pieces

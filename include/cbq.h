@@ -599,8 +599,8 @@ int cbq_paged_append_rope(const cbq_paged_cache *cache, const cbq_paged_batch *b
  * once; every call leaves its arrival counters zero, so calls of any shape may
  * share one, as long as they do not overlap on the GPU (the same stream is
  * fine, from several host threads too: the launches of a call stay together).
- * After CBQ_FLAG_TIMEOUT it has to be zeroed again.  -1: arguments the
- * functions refuse. */
+ * A call that sets CBQ_FLAG_TIMEOUT leaves them zero too; its result is not
+ * to be used.  -1: arguments the functions refuse. */
 int64_t cbq_paged_attn_workspace_bytes(const cbq_paged_cache *cache, const cbq_paged_batch *batch,
                                        int64_t tokens, int64_t q_heads, int extend);
 

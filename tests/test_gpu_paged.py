@@ -509,3 +509,17 @@ def test_threads_that_share_a_stream():
     finally:
         sys.setswitchinterval(interval)
     assert wrong == [0] * len(calls)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_counters_are_zero_after_every_call(d):
+    """What lets calls of any shape share a workspace: its first 16 KB count arrivals."""
+    dev = need_cuda()
+    ws = torch.zeros(64 << 20, dtype=torch.uint8, device=dev)
+    for kv, new, heads in (([700, 90], [600, 90], 8), ([3000], [1], 8), ([64] * 20, [64] * 20, 4), ([900] * 3, None, 4)):
+        s = Setup(kv, new=new, heads=heads, kv_heads=2, d=d, page=64)
+        k, v = s.pools(dev)
+        c, b = cbq.PagedKVCache(k, v), s.batch(cbq, dev, decode=new is None)
+        f = c.attend_decode if new is None else c.attend_extend
+        check_attention(f(b, s.q.to(dev), workspace=ws), *s.attention(d ** -0.5, new is not None))
+        assert not ws[:16384].any()
