@@ -91,7 +91,8 @@ class PagedBatch:
     and its prefix the first ``prefix_lens[g]`` rows of the pages in
     ``prefix_table[g]``.  ``max_kv_len`` / ``max_prefix_len`` bound the values
     the two length tensors will ever hold (default: what the tables can name).
-    ``status`` int32 [4]: see :meth:`new_status` and :func:`check_status`.
+    ``status`` int32 [4]: what calls record there, see :func:`check_status`
+    (None: one of the batch's own; :meth:`check` reads it).
     The tensors are kept, not copied: write new values into them in place."""
 
     def __init__(self, page_table: torch.Tensor, kv_lens: torch.Tensor, cu_tokens: Optional[torch.Tensor] = None,
@@ -118,6 +119,8 @@ class PagedBatch:
             _need(group_starts.shape[0] == groups + 1 and prefix_table.shape[0] == groups,
                   "group_starts needs one entry more than prefix_lens, prefix_table one row for each")
         _need(status is None or status.shape[0] == 4, "status must have four entries")
+        if status is None:
+            self.status = status = self.new_status(dev)
         self.groups = groups
         ptr = lambda t: 0 if t is None else t.data_ptr()  # noqa: E731
         big = 0x7fffff00
@@ -134,12 +137,21 @@ class PagedBatch:
     @staticmethod
     def new_status(device) -> torch.Tensor:
         """A status word for ``status=``: flags, first row, count, spare."""
-        return torch.tensor([0, -1, 0, 0], dtype=torch.int32, device=device)
+        s = torch.zeros(4, dtype=torch.int32, device=device)
+        s[1] = -1
+        return s
+
+    def check(self) -> None:
+        """:func:`check_status` of this batch's calls (reads the device)."""
+        check_status(self.status)
 
 
 def check_status(status: torch.Tensor) -> None:
-    """Raise if a call recorded lengths or pages outside the tables (reads the device)."""
+    """Raise if a call recorded a device-side wait that ran out (its result is
+    not to be used) or lengths or pages outside the tables (reads the device)."""
     flags = int(status[0].item())
+    if flags & _lib.FLAG_TIMEOUT:
+        raise _lib.CbqError("paged cache", _lib.CBQ_ERR_TIMEOUT)
     if flags:
         raise _lib.CbqError("paged cache", _lib.CBQ_ERR_CORRUPT)
 

@@ -187,3 +187,19 @@ def test_calls_run_on_the_device_of_the_cache(monkeypatch):
     s.device = -1
     s.attend(cbq.PagedBatch(*tables()))
     assert len(entered) == 2
+
+
+@pytest.mark.parametrize("flags,rc", [(0, None), (L.FLAG_CORRUPT, L.CBQ_ERR_CORRUPT),
+                                      (L.FLAG_TIMEOUT, L.CBQ_ERR_TIMEOUT),
+                                      (L.FLAG_TIMEOUT | L.FLAG_CORRUPT, L.CBQ_ERR_TIMEOUT)], ids=str)
+def test_status_tells_what_was_recorded(flags, rc):
+    b = cbq.PagedBatch(*tables())                      # a status of its own
+    assert struct.unpack("<15q", b._desc.raw)[14] == b.status.data_ptr() and b.status.tolist() == [0, -1, 0, 0]
+    b.status[0] = flags
+    for check in (b.check, lambda: cbq.paged.check_status(b.status)):
+        if rc is None:
+            check()
+        else:
+            with pytest.raises(L.CbqError) as e:
+                check()
+            assert e.value.status == rc
