@@ -20,7 +20,7 @@ import torch
 
 from . import _lib
 from .gpu_accelerated_functions import device_stream
-from .paged import PagedBatch, PagedKVCache
+from .paged import PagedBatch, PagedKVCache, check_status
 from .qwen3 import CompressedQwen3Weights
 from .qwen3_decode import rope_tables
 
@@ -104,7 +104,7 @@ class PagedQwen3:
                  graph: bool = True) -> torch.Tensor:
         """Greedy tokens [len(prompts), n_new] after each prompt (1-D token
         ids, one token at least); ``prefix``: token ids that stand before all
-        of them, computed and kept once."""
+        of them, computed and kept once.  Raises if a kernel reported an error."""
         lens = [int(p.numel()) for p in prompts]
         plen = 0 if prefix is None else int(prefix.numel())
         if not lens or min(lens) < 1 or n_new < 1:
@@ -112,11 +112,13 @@ class PagedQwen3:
         if plen + max(lens) + n_new > self.max_len:
             raise ValueError("sequence longer than max_len")
         held: List[List[int]] = []
+        status = PagedBatch.new_status(self.dev)
         try:
             shared = {}
             if plen:
                 held.append(self._take(plen))
-                b = PagedBatch(self._table(held[:1]), self._ints([plen]), cu_tokens=self._ints([0, plen]), max_kv_len=plen)
+                b = PagedBatch(self._table(held[:1]), self._ints([plen]), cu_tokens=self._ints([0, plen]), max_kv_len=plen,
+                               status=status)
                 self.forward(prefix.to(self.dev).long(), b, decode=False)
                 shared = dict(group_starts=self._ints([0, len(lens)]), prefix_lens=self._ints([plen]),
                               prefix_table=self._table(held[:1]), max_prefix_len=plen)
@@ -126,12 +128,12 @@ class PagedQwen3:
             table, kv = self._table(own), self._ints(lens)
             cu = self._ints([0] + torch.tensor(lens).cumsum(0).tolist())
             # the prompts in one pass, then one token of each at a time
-            b = PagedBatch(table, kv, cu_tokens=cu, max_kv_len=max(lens), **shared)
+            b = PagedBatch(table, kv, cu_tokens=cu, max_kv_len=max(lens), status=status, **shared)
             h = self.forward(torch.cat([p.reshape(-1) for p in prompts]).to(self.dev).long(), b, decode=False)
             nxt = torch.zeros(len(lens), dtype=torch.int64, device=self.dev)
             self._pick(h.index_select(0, cu[1:].long() - 1), nxt)
             out = torch.empty(len(lens), n_new, dtype=torch.int64, device=self.dev)
-            b = PagedBatch(table, kv, max_kv_len=max(lens) + n_new, **shared)
+            b = PagedBatch(table, kv, max_kv_len=max(lens) + n_new, status=status, **shared)
 
             def step():
                 kv.add_(1)
@@ -153,6 +155,7 @@ class PagedQwen3:
                 else:
                     step()
             torch.cuda.synchronize(self.dev)
+            check_status(status)
             return out
         finally:
             for pages in held:

@@ -60,3 +60,17 @@ def test_refusals():
     with pytest.raises(RuntimeError):
         m.generate([torch.arange(30), torch.arange(30)], 20)
     assert len(m.free) == 4
+
+
+@pytest.mark.parametrize("graph", [False, True], ids=["eager", "graph"])
+def test_an_error_that_a_kernel_reports_is_raised(graph):
+    """A table entry outside the pool (nothing is read or written there)."""
+    dev = need_cuda()
+    m = qp.PagedQwen3(q3.CompressedQwen3Weights(TINY, dev, seed=5), pages=4, page_size=16, max_len=64)
+    prompts = [torch.arange(5), torch.arange(9)]
+    m.generate(prompts, 4, graph=graph)
+    table = m._table
+    m._table = lambda rows: table(rows) + 4
+    with pytest.raises(cbq._lib.CbqError) as e:
+        m.generate(prompts, 4, graph=graph)
+    assert e.value.status == cbq._lib.CBQ_ERR_CORRUPT and len(m.free) == 4
