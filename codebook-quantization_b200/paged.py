@@ -178,7 +178,7 @@ class PagedKVCache:
                           _CODES[k_pages.dtype])
         self._desc = ct.create_string_buffer(raw, len(raw))
         self._addr = ct.addressof(self._desc)
-        self._key = (tuple(k_pages.shape), self.dtype)
+        self._key = (tuple(k_pages.shape), st, self.dtype)      # what a plan depends on
         self._index = k_pages.get_device()
 
     def _batch(self, batch: PagedBatch) -> None:

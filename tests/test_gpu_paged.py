@@ -523,3 +523,24 @@ def test_counters_are_zero_after_every_call(d):
         f = c.attend_decode if new is None else c.attend_extend
         check_attention(f(b, s.q.to(dev), workspace=ws), *s.attention(d ** -0.5, new is not None))
         assert not ws[:16384].any()
+
+
+@pytest.mark.parametrize("op", ["decode", "extend"])
+def test_one_batch_over_pools_of_different_layouts(op):
+    """Padded pages go to the row kernel, whole ones to the tile kernel: other workspaces."""
+    dev = need_cuda()
+    s = Setup([300, 200, 500], new=None if op == "decode" else [300, 200, 100], groups=[(3, 90)], heads=32, kv_heads=4,
+              d=128)
+    b, q = s.batch(cbq, dev, decode=op == "decode"), s.q.to(dev)
+    shape, each = s.k.shape, s.k[0].numel()
+    padded = []
+    for x in (s.k, s.v):
+        t = torch.empty(shape[0], each + 8, dtype=x.dtype, device=dev)[:, :each].unflatten(1, shape[1:])
+        t.copy_(x)
+        padded.append(t)
+    ref = s.attention(s.d ** -0.5, op == "extend")
+    for k, v in (padded, s.pools(dev), padded):
+        c = cbq.PagedKVCache(k, v)
+        f = c.attend_decode if op == "decode" else c.attend_extend
+        n = c.workspace_bytes(b, s.tokens, 32, op == "extend")
+        check_attention(f(b, q, workspace=torch.zeros(n, dtype=torch.uint8, device=dev)), *ref)

@@ -203,3 +203,13 @@ def test_status_tells_what_was_recorded(flags, rc):
             with pytest.raises(L.CbqError) as e:
                 check()
             assert e.value.status == rc
+
+
+def test_workspace_sizes_are_kept_by_layout(monkeypatch):
+    """The kernel, and so the size, depends on the strides too."""
+    shape, asked = (4, 2, 16, 64), []
+    monkeypatch.setattr(L, "query", lambda name, cache, *a: asked.append(cache) or len(asked))
+    flat, padded = (Stub(monkeypatch, shape, (n, 1024, 64, 1)).cache for n in (2048, 2056))
+    b = cbq.PagedBatch(*tables())
+    got = [c.workspace_bytes(b, 2, 4, True) for c in (padded, flat, padded, flat)]
+    assert got == [1, 2, 1, 2] and asked == [padded._addr, flat._addr]
