@@ -79,7 +79,17 @@ def _row_stride(t: torch.Tensor, name: str) -> int:
     return t.stride(0)
 
 
-class PagedBatch:
+class _Held:
+    """The kernels read the tensors by the addresses that they had when the
+    object was made: an attribute cannot be set to another tensor later."""
+
+    def __setattr__(self, name: str, value) -> None:
+        if name in self.__dict__ and self.__dict__[name] is not value:      # ``b.kv_lens += 1`` sets the same one
+            raise AttributeError(f"{name} is read by its address: write into it in place, or make a new object")
+        object.__setattr__(self, name, value)
+
+
+class PagedBatch(_Held):
     """The sequences of a step.
 
     ``page_table`` int32 [seqs, width], ``kv_lens`` int32 [seqs] (rows of each
@@ -107,7 +117,7 @@ class PagedBatch:
         self.group_starts = _ints(group_starts, "group_starts", 1, dev)
         self.prefix_lens = _ints(prefix_lens, "prefix_lens", 1, dev)
         self.prefix_table = _ints(prefix_table, "prefix_table", 2, dev)
-        self.status = _ints(status, "status", 1, dev)
+        _ints(status, "status", 1, dev)
         self.seqs = n = kv_lens.shape[0]
         _need(page_table.shape[0] == n, f"page_table has {page_table.shape[0]} rows for {n} sequences")
         _need(cu_tokens is None or cu_tokens.shape[0] == n + 1, "cu_tokens must have one entry more than kv_lens")
@@ -119,8 +129,7 @@ class PagedBatch:
             _need(group_starts.shape[0] == groups + 1 and prefix_table.shape[0] == groups,
                   "group_starts needs one entry more than prefix_lens, prefix_table one row for each")
         _need(status is None or status.shape[0] == 4, "status must have four entries")
-        if status is None:
-            self.status = status = self.new_status(dev)
+        self.status = status = self.new_status(dev) if status is None else status
         self.groups = groups
         ptr = lambda t: 0 if t is None else t.data_ptr()  # noqa: E731
         big = 0x7fffff00
@@ -156,7 +165,7 @@ def check_status(status: torch.Tensor) -> None:
         raise _lib.CbqError("paged cache", _lib.CBQ_ERR_CORRUPT)
 
 
-class PagedKVCache:
+class PagedKVCache(_Held):
     """One layer's keys and values: ``k_pages``, ``v_pages`` [pages, kv_heads,
     page_size, head_dim] (fp32 or bf16, head_dim contiguous, equal strides; a
     pool stored as [pages, page_size, kv_heads, head_dim] is passed transposed)."""

@@ -213,3 +213,15 @@ def test_workspace_sizes_are_kept_by_layout(monkeypatch):
     b = cbq.PagedBatch(*tables())
     got = [c.workspace_bytes(b, 2, 4, True) for c in (padded, flat, padded, flat)]
     assert got == [1, 2, 1, 2] and asked == [padded._addr, flat._addr]
+
+
+def test_held_tensors_cannot_be_replaced(monkeypatch):
+    """A replaced tensor was freed while the kernels went on reading its address."""
+    c, (t, n) = Stub(monkeypatch).cache, tables()
+    b = cbq.PagedBatch(t, n)
+    for o, name in ((b, "kv_lens"), (b, "page_table"), (b, "cu_tokens"), (b, "status"), (c, "k_pages"), (c, "v_pages")):
+        with pytest.raises(AttributeError):
+            setattr(o, name, tables()[1])
+    b.kv_lens += 1
+    b.kv_lens[0] = 5
+    assert n.tolist() == [5, 1] and b.kv_lens is n
