@@ -105,6 +105,76 @@ __device__ __forceinline__ int unit_stages(const Owner &w, int tt, const LineArg
     return np + (own_limit(w, min((tt + 1) * a.geo.tq, w.nt) - 1) + kKeys - 1) / kKeys;
 }
 
+// A warp's share of a piece once more, row by row by fp32 FMAs on the cached
+// values themselves.  The tf32 pair of an infinity, or of a value that rounds to
+// one, is NaN or two infinities of opposite sign, and every product it enters
+// comes out NaN: a warp that ends a piece with a NaN leaves what this finds
+// instead (an infinity or a NaN that remains is the formula's).  Rare and slow;
+// checking once a piece costs under 1 us
+// a call (two prefixes 26 -> 27 us, 2000 new tokens 2.42 ms as before; a check of every
+// product took 10 to 18 %).
+struct ExactPiece {
+    const float *q, *k, *v;            // of the unit's first row; of its kv head
+    const int32_t *ptab, *otab;
+    int64_t qs, page_stride, row_stride;
+    int pages, ps_shift, plen, olen, np, st0, st1, step;   // stages st0, st0 + step, ..
+    int tok0, nt, gb, nrows;
+    bool own;                          // whether own rows count
+    float sc;
+    float *o, *m, *l;                  // of the warp, in shared memory
+    int pitch;
+};
+template <int D> __device__ __noinline__ void exact_piece(const ExactPiece x) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll 1
+    for (int r = 0; r < x.nrows; ++r) {
+        const int tk = r / x.gb;
+        const float *q = x.q + tk * x.qs + (int64_t)(r - tk * x.gb) * D;
+        const int lim = x.own ? clampi(x.olen - x.nt + x.tok0 + tk + 1, 0, x.olen) : 0;
+        float m = -INFINITY, l = 0.f, o[D / 32];
+#pragma unroll
+        for (int e = 0; e < D / 32; ++e) o[e] = 0.f;
+#pragma unroll 1
+        for (int st = x.st0; st < x.st1; st += x.step) {
+            const bool pre = st < x.np;
+            const int key0 = (pre ? st : st - x.np) * kKeys, n = min((pre ? x.plen : lim) - key0, kKeys);
+            if (n <= 0) continue;
+            const int page = __ldg((pre ? x.ptab : x.otab) + (key0 >> x.ps_shift));
+            const bool ok = page >= 0 && page < x.pages;               // else rows of zeros
+            const int64_t off = (ok ? page : 0) * x.page_stride + (int64_t)(key0 & ((1 << x.ps_shift) - 1)) * x.row_stride;
+            float s = -INFINITY;
+            if (lane < n) {
+                s = 0.f;
+                const float *k = x.k + off + lane * x.row_stride;
+#pragma unroll 1
+                for (int d = 0; d < D && ok; ++d) s = fmaf(q[d], k[d], s);
+                s *= x.sc;
+            }
+            float mx = s;
+#pragma unroll
+            for (int d = 16; d > 0; d >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
+            const float mn = fmaxf(m, mx), mu = mn == -INFINITY ? 0.f : mn, f = ex2(m - mu);
+            const float w = lane < n ? ex2(s - mu) : 0.f;
+            m = mn;
+            l = l * f + warp_sum(w);
+#pragma unroll
+            for (int e = 0; e < D / 32; ++e) o[e] *= f;
+#pragma unroll 1
+            for (int j = 0; j < n && ok; ++j) {
+                const float wj = __shfl_sync(0xffffffffu, w, j), *v = x.v + off + j * x.row_stride + lane;
+#pragma unroll
+                for (int e = 0; e < D / 32; ++e) o[e] = fmaf(wj, v[e * 32], o[e]);
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < D / 32; ++e) x.o[r * x.pitch + e * 32 + lane] = o[e];
+        if (lane == 0) {
+            x.m[r] = m;
+            x.l[r] = l;
+        }
+    }
+}
+
 // One warp's 16 keys starting at `key0` of a table, into its slot: K then V,
 // 16-byte chunks exchanged within groups of 8 by the row (no bank conflicts
 // for the fragment reads).  Rows at or after `lim` are zero-filled, not read,
@@ -441,6 +511,7 @@ __global__ void __launch_bounds__(StreamCfg<T, D, NB>::NT, StreamCfg<T, D, NB>::
                     }
                 }
                 // this warp's (m, l, o) for the merge
+                bool odd = false;
 #pragma unroll
                 for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
@@ -453,13 +524,35 @@ __global__ void __launch_bounds__(StreamCfg<T, D, NB>::NT, StreamCfg<T, D, NB>::
                             mM[warp * R + r] = m[nb][e];
                             mL[warp * R + r] = ls;
                         }
+                        if constexpr (kF32) odd |= ls != ls;
                         float *dst = mO + (warp * R + r) * kPitch + rq;
 #pragma unroll
                         for (int i = 0; i < KK; ++i) {
                             dst[i * 16] = o[nb][i][e];
                             dst[i * 16 + 8] = o[nb][i][e + 2];
+                            if constexpr (kF32) odd |= o[nb][i][e] != o[nb][i][e] || o[nb][i][e + 2] != o[nb][i][e + 2];
                         }
                     }
+                if constexpr (kF32) {
+                    if (__builtin_expect(__any_sync(0xffffffffu, odd), 0)) {
+                        ExactPiece x;
+                        x.q = q_row(0);
+                        x.k = static_cast<const float *>(pv.k) + p.h * pv.head_stride;
+                        x.v = static_cast<const float *>(pv.v) + p.h * pv.head_stride;
+                        x.ptab = pv.ptable + ow.group * pv.ptable_stride;
+                        x.otab = pv.table + cons.o * pv.table_stride;
+                        x.qs = a.qs; x.page_stride = pv.page_stride; x.row_stride = pv.row_stride;
+                        x.pages = pv.pages; x.ps_shift = pv.ps_shift; x.plen = ow.plen; x.olen = ow.olen; x.np = np;
+                        x.st0 = p.tb * NW + warp; x.st1 = min(p.te * NW, nst); x.step = NW;
+                        x.tok0 = tok0; x.nt = ow.nt; x.gb = gb; x.nrows = nrows;
+                        x.own = a.mode != kPrefix;
+                        x.sc = a.sc;
+                        x.o = mO + warp * R * kPitch; x.m = mM + warp * R; x.l = mL + warp * R;
+                        x.pitch = kPitch;
+                        __syncwarp();
+                        exact_piece<D>(x);
+                    }
+                }
             }
             __syncthreads();
             // the NW warps' states joined in warp order; a whole unit is the

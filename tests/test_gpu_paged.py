@@ -544,3 +544,41 @@ def test_one_batch_over_pools_of_different_layouts(op):
         f = c.attend_decode if op == "decode" else c.attend_extend
         n = c.workspace_bytes(b, s.tokens, 32, op == "extend")
         check_attention(f(b, q, workspace=torch.zeros(n, dtype=torch.uint8, device=dev)), *ref)
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f32"])
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("op", ["decode", "extend"])
+@pytest.mark.parametrize("what", ["inf value", "-inf value", "-inf key", "lowest key", "largest query"])
+def test_infinities_and_largest_values_inside_the_lengths(what, op, d, dt):
+    """A visible value of inf gives inf where its weight is not 0; a key of -inf
+    or of the type's lowest value takes its row out; a prefix and own rows."""
+    dev = need_cuda()
+    new = None if op == "decode" else [40, 2, 17]
+    s = Setup([90, 100, 67], new=new, groups=[(3, 50)], heads=4, kv_heads=2, d=d, dtype=DT[dt])
+    slack = s.attention(d ** -0.5, op == "extend")[2]
+    top = torch.finfo(DT[dt]).max
+    number = {"inf": math.inf, "-inf": -math.inf, "largest": top, "lowest": -top}[what.split()[0]]
+    pages = ((s.table[0, 0], 5), (s.table[1, 3], 2), (s.ptable[0, 1], 9), (s.table[2, 0], 3))
+    if what.endswith("query"):
+        # one query's largest element against keys of 0 but for a small one: scores stay finite
+        s.k[..., 7] = torch.where(s.k[..., 7].isnan(), s.k[..., 7], torch.zeros_like(s.k[..., 7]))
+        s.k[pages[0][0], :, pages[0][1], 7] = 2.0 ** -124
+        s.q[:, :, 7] = number
+    for page, line in pages:
+        if what.endswith("value"):
+            s.v[page, :, line, 7] = number
+        elif what.endswith("key"):
+            s.k[page, :, line, 7] = number
+            s.q[:, :, 7] = 0.25
+    ref, spread, changed = s.attention(d ** -0.5, op == "extend")
+    # what bounds the scores' errors: a key that is taken out does not count, one element of the others moved
+    slack = changed if not what.endswith("key") else 2 * slack
+    got = run(s, op, dev)
+    finite = ref.isfinite()
+    assert torch.equal(got.double().cpu()[~finite], ref[~finite])
+    if what.endswith("inf value"):
+        assert not finite.all()
+    u = 2.0 ** -8 if dt == "bf16" else 2.0 ** -23
+    tol = u * ref.abs() + ((2.0 ** -8 if dt == "bf16" else 0.0) + slack) * spread + 1e-30
+    assert bool(((got.double().cpu() - ref).abs()[finite] <= tol[finite]).all())
