@@ -4,8 +4,8 @@
 //
 // For a query row q and its visible keys j: x_j = scale log2(e) q.k_j,
 // m = max x_j, l = sum 2^(x_j - m), o = sum 2^(x_j - m) v_j / l.  A part of the
-// keys gives (m, l, unnormalised o); parts join as M = max m, each l and o
-// scaled by 2^(m - M) and added.  m, l and o are fp32 everywhere.
+// keys gives (m, l, unnormalised o), both sums smaller by 2^kHead; parts join as
+// M = max m, each l and o scaled by 2^(m - M) and added.  m, l and o are fp32 everywhere.
 //
 // k_paged_stream is the kernel for few query rows per kv head: the cache is
 // read once and its bytes bound it.  A CTA whose part of the line (see
@@ -154,7 +154,7 @@ template <int D> __device__ __noinline__ void exact_piece(const ExactPiece x) {
 #pragma unroll
             for (int d = 16; d > 0; d >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
             const float mn = fmaxf(m, mx), mu = mn == -INFINITY ? 0.f : mn, f = ex2(m - mu);
-            const float w = lane < n ? ex2(s - mu) : 0.f;
+            const float w = lane < n ? ex2(s - (mu + kHead)) : 0.f;
             m = mn;
             l = l * f + warp_sum(w);
 #pragma unroll
@@ -442,10 +442,10 @@ __global__ void __launch_bounds__(StreamCfg<T, D, NB>::NT, StreamCfg<T, D, NB>::
                             for (int d = 4; d < 32; d <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
                             const float mn = fmaxf(m[nb][e], mx);
                             const float mu = mn == -INFINITY ? 0.f : mn;     // no key yet: 2^(-inf - 0) = 0
-                            const float f = ex2(m[nb][e] - mu);
+                            const float f = ex2(m[nb][e] - mu), mk = mu + kHead;
                             m[nb][e] = mn;
-                            pr[e] = ex2(x0 - mu);
-                            pr[e + 2] = ex2(x1 - mu);
+                            pr[e] = ex2(x0 - mk);
+                            pr[e + 2] = ex2(x1 - mk);
                             l[nb][e] = l[nb][e] * f + (pr[e] + pr[e + 2]);
                             if (__any_sync(0xffffffffu, f != 1.f)) {
 #pragma unroll

@@ -18,6 +18,12 @@ namespace cbq {
 
 constexpr float kLog2e = 1.4426950408889634f;
 
+// Weights are taken as 2^(x - m - kHead): a sum of up to 2^16 of the largest
+// finite values (2^8 in the tile kernel, whose weights run up to 2^8 above a
+// reference m) stays finite until l, smaller by the same factor, divides it.
+// What is lost lies below 2^-110, of a weight or of a value.
+constexpr float kHead = 16.f;
+
 enum LineMode : int {
     kOwn = 0,                          // owner = sequence, keys = its own rows (decode)
     kPrefix = 1,                       // owner = group, keys = its prefix, rows = all its sequences' (decode)

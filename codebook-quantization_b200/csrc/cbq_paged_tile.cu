@@ -5,11 +5,11 @@
 // A unit's query rows (whole tokens, the G heads of a kv head side by side) lie
 // in NQ blocks of 128.  Per key tile and row block:
 //   S = Q K^T          tcgen05.mma, Q and K in shared memory, S fp32 in TMEM
-//   P = 2^(sc S - m)   one thread per row, S from TMEM, P (bf16) to TMEM
+//   P = 2^(sc S - m - kHead)   one thread per row, S from TMEM, P (bf16) to TMEM
 //   O += P V           tcgen05.mma with P from TMEM, O fp32 in TMEM
 // The running maximum m of a row is only moved when a tile exceeds it by more
 // than 2^kGrow: until then the weights are taken relative to the old one (they
-// stay below 2^kGrow, and sums and O are fp32), so O is rescaled in TMEM a few
+// stay below 2^(kGrow - kHead), and sums and O are fp32), so O is rescaled in TMEM a few
 // times per unit instead of once per tile.  The result does not depend on m
 // beyond rounding: o = (sum 2^(x - m) v) / (sum 2^(x - m)).
 //
@@ -427,7 +427,7 @@ __global__ void __launch_bounds__(TileCfg<D, NQ>::kThreads, 1)
                 const bool grow = (mn - m) * sc > kGrow;                       // false where both are -inf
                 const float f = grow ? ex2((m - mn) * sc) : 1.f;               // 0 from -inf
                 if (grow) m = mn;
-                const float mb = m == -INFINITY ? 0.f : m * sc;
+                const float mb = m == -INFINITY ? 0.f : fmaf(m, sc, kHead);
                 float ls[4] = {0.f, 0.f, 0.f, 0.f};
                 uint32_t pk[KT / 2];
 #pragma unroll

@@ -549,7 +549,8 @@ def test_one_batch_over_pools_of_different_layouts(op):
 @pytest.mark.parametrize("dt", ["bf16", "f32"])
 @pytest.mark.parametrize("d", [64, 128, 256])
 @pytest.mark.parametrize("op", ["decode", "extend"])
-@pytest.mark.parametrize("what", ["inf value", "-inf value", "-inf key", "lowest key", "largest query"])
+@pytest.mark.parametrize("what", ["inf value", "-inf value", "largest value", "lowest value", "-inf key", "lowest key",
+                                  "largest query"])
 def test_infinities_and_largest_values_inside_the_lengths(what, op, d, dt):
     """A visible value of inf gives inf where its weight is not 0; a key of -inf
     or of the type's lowest value takes its row out; a prefix and own rows."""
