@@ -65,12 +65,13 @@ inline int paged_view(const cbq_paged_cache *c, const cbq_paged_batch *b, int64_
     if (c->pages > 0 && (!c->k_dev || !c->v_dev || (reinterpret_cast<uintptr_t>(c->k_dev) & 15) ||
                          (reinterpret_cast<uintptr_t>(c->v_dev) & 15)))
         return CBQ_ERR_ARG;
-    if (!b->kv_lens_dev || !b->page_table_dev || b->table_width < 0 || b->table_stride < b->table_width ||
+    // a table without columns (its address may be null) names no rows
+    if (!b->kv_lens_dev || (!b->page_table_dev && b->table_width) || b->table_width < 0 || b->table_stride < b->table_width ||
         b->max_kv_len < 0)
         return CBQ_ERR_ARG;
     if ((!b->cu_tokens_dev && tokens != b->seqs)) return CBQ_ERR_ARG;
-    if (b->groups && (!b->group_starts_dev || !b->prefix_lens_dev || !b->prefix_table_dev || b->prefix_width < 0 ||
-                      b->prefix_stride < b->prefix_width || b->max_prefix_len < 0))
+    if (b->groups && (!b->group_starts_dev || !b->prefix_lens_dev || (!b->prefix_table_dev && b->prefix_width) ||
+                      b->prefix_width < 0 || b->prefix_stride < b->prefix_width || b->max_prefix_len < 0))
         return CBQ_ERR_ARG;
     if (b->table_width * c->page_size > 0x7fffff00 || (b->groups && b->prefix_width * c->page_size > 0x7fffff00))
         return CBQ_ERR_UNSUPPORTED;

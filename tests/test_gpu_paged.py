@@ -583,3 +583,27 @@ def test_infinities_and_largest_values_inside_the_lengths(what, op, d, dt):
     u = 2.0 ** -8 if dt == "bf16" else 2.0 ** -23
     tol = u * ref.abs() + ((2.0 ** -8 if dt == "bf16" else 0.0) + slack) * spread + 1e-30
     assert bool(((got.double().cpu() - ref).abs()[finite] <= tol[finite]).all())
+
+
+@pytest.mark.parametrize("op", ["decode", "extend"])
+@pytest.mark.parametrize("dt", ["bf16", "f32"])
+def test_tables_without_columns(op, dt):
+    """No own rows at all, or no prefix: an empty table, whose address may be null."""
+    dev = need_cuda()
+    new = None if op == "decode" else [40, 2]
+    s = Setup([0, 0], new=new, groups=[(1, 30), (1, 70)], heads=4, kv_heads=2, d=64, dtype=DT[dt])
+    s.table = s.table[:, :0]
+    verify(s, op, dev)
+    s = Setup([50, 9], new=new, groups=[(1, 0), (1, 0)], heads=4, kv_heads=2, d=64, dtype=DT[dt])
+    s.ptable = s.ptable[:, :0]
+    verify(s, op, dev)
+    s = Setup([0, 0], new=new, heads=4, kv_heads=2, d=64, dtype=DT[dt])
+    s.table = s.table[:, :0]
+    assert not verify(s, op, dev).any()
+    qkv = torch.randn(s.tokens, 8, 64, device=dev).to(DT[dt])
+    cos, sin = tables(64, 8)
+    kp, vp = s.pools(dev)
+    before = kp.clone()
+    got = cbq.PagedKVCache(kp, vp).append_rope(s.batch(cbq, dev, decode=op == "decode"), qkv[:, :4], qkv[:, 4:6],
+                                               qkv[:, 6:], cos.to(dev), sin.to(dev))
+    assert not got.any() and torch.equal(kp.nan_to_num(7.0), before.nan_to_num(7.0))
