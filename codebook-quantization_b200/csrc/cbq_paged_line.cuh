@@ -317,6 +317,11 @@ __device__ __forceinline__ bool plan_line(const PagedView &pv, const LineArgs &a
         tl = owner_tiles(w, a.geo, a.mode);
         return (uint64_t)(per_unit * (uint32_t)tl.tt) << 32 | per_unit * tl.all();
     };
+    // prefixes that are cut to their table, where they are not owners (a decode call without
+    // room for any prefix has no line of them)
+    if (blockIdx.x == 0 && pv.groups && (a.mode == kFull || (a.mode == kOwn && pv.pcap == 0)))
+        for (int g = tid; g < pv.groups; g += NT)
+            if (pv.plens[g] > pv.pcap) report(pv.status, CBQ_FLAG_CORRUPT, (uint32_t)g);
     // owners beyond the first NT: their sum first, the first NT below in one scan
     uint64_t rest = 0;
     for (int o = tid + NT; o < a.owners; o += NT) rest += weight(o);

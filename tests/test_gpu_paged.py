@@ -607,3 +607,26 @@ def test_tables_without_columns(op, dt):
     got = cbq.PagedKVCache(kp, vp).append_rope(s.batch(cbq, dev, decode=op == "decode"), qkv[:, :4], qkv[:, 4:6],
                                                qkv[:, 6:], cos.to(dev), sin.to(dev))
     assert not got.any() and torch.equal(kp.nan_to_num(7.0), before.nan_to_num(7.0))
+
+
+@pytest.mark.parametrize("op", ["decode", "extend"])
+@pytest.mark.parametrize("dt", ["bf16", "f32"])
+@pytest.mark.parametrize("rows", [48, 0])
+def test_prefixes_above_their_table_are_cut_and_reported(rows, op, dt):
+    dev = need_cuda()
+    s = Setup([48, 33, 60], new=None if op == "decode" else [40, 33, 2], groups=[(1, 16), (2, rows)], heads=4, kv_heads=2,
+              d=64, dtype=DT[dt])
+    if rows == 0:
+        s.plens[0], s.groups = 0, [(1, 0), (2, 0)]
+        s.ptable = s.ptable[:, :0]                     # a table that names nothing
+    ref = s.attention(s.d ** -0.5, op == "extend")
+    status = cbq.PagedBatch.new_status(dev)
+    b = s.batch(cbq, dev, decode=op == "decode", status=status)
+    k, v = s.pools(dev)
+    c, q = cbq.PagedKVCache(k, v), s.q.to(dev)
+    f = c.attend_decode if op == "decode" else c.attend_extend
+    check_attention(f(b, q), *ref)
+    assert int(status[0]) == 0
+    b.prefix_lens[1] = 1000
+    check_attention(f(b, q), *ref)
+    assert int(status[0]) == L.FLAG_CORRUPT and int(status[1]) == 1
