@@ -261,17 +261,14 @@ __device__ __forceinline__ void join_unit(const LineArgs &a, const Cut &cut, int
 // The warp computes S^T = K Q^T and O^T = V^T P^T with the row-of-16 matrix
 // instructions, keys (then dimensions of V) on the 16-row side and the query
 // rows on the 8-column side, so 1..8 query rows waste none of the long side.
-// bf16: m16n8k16; P^T turns into the second product's operand with 8x8 register
-// transposes, as two bf16 terms (the rounded weight and the rounded rest, 2^-16 of
-// it left out): one term alone left an error of 2.1e-3 where rounding the result
-// takes 1.66e-3, and the second product costs little here, where bytes bound it (64
-// ragged sequences 169 -> 171 us).  fp32: m16n8k8 on tf32 pairs (see mma_f32), three
+// bf16: m16n8k16; P^T turns into the second product's operand with two 8x8
+// register transposes.  fp32: m16n8k8 on tf32 pairs (see mma_f32), three
 // products each: about 280 instructions for 16 keys and 8 rows where fp32 FMAs
 // fed from shared memory took 950.
 //
 // Each warp copies its own 16 keys of a tile into its own ring (no barrier in the
 // loop).  HBM bounds long sequences: 64 ragged ones of up to 8192 keys, 8 kv heads
-// of 128 (960 MB), take 171 us = 5.6 TB/s, 0.87 of a copy's rate, with two CTAs an
+// of 128 (960 MB), take 168 us = 5.7 TB/s, 0.88 of a copy's rate, with two CTAs an
 // SM and 16 KB in flight per warp.  Short work is a chain of latencies: 1000 keys
 // of one sequence (4 MB) take 10 us, of which the plan 2, the first loads 3, the
 // tile 1, arrival and joining 3.
@@ -428,7 +425,7 @@ __global__ void __launch_bounds__(StreamCfg<T, D, NB>::NT, StreamCfg<T, D, NB>::
                     const int key0 = (pre ? st : st - np) * kKeys;
                     const bool edge = key0 + kKeys > (pre ? ow.plen : lim_first);
                     const int ka = key0 + (lane >> 2), kc = ka + 8;
-                    uint32_t pf[NB][4], pw[2][NB][4];        // P as the second product's right-hand side (fp32: by 8 keys)
+                    uint32_t pf[NB][2], pw[2][NB][4];        // P as the second product's right-hand side (fp32: by 8 keys)
 #pragma unroll
                     for (int nb = 0; nb < NB; ++nb) {
                         float pr[4];
@@ -473,13 +470,8 @@ __global__ void __launch_bounds__(StreamCfg<T, D, NB>::NT, StreamCfg<T, D, NB>::
                                     pw[ks][nb][e + 2] = tf32_lo(x, pw[ks][nb][e]);
                                 }
                         } else {
-#pragma unroll
-                            for (int e = 0; e < 2; ++e) {
-                                const uint32_t hi = pack_bf16(pr[e * 2], pr[e * 2 + 1]);
-                                pf[nb][e] = movm(hi);
-                                pf[nb][e + 2] = movm(pack_bf16(pr[e * 2] - __uint_as_float(hi << 16),
-                                                               pr[e * 2 + 1] - __uint_as_float(hi & 0xffff0000u)));
-                            }
+                            pf[nb][0] = movm(pack_bf16(pr[0], pr[1]));
+                            pf[nb][1] = movm(pack_bf16(pr[2], pr[3]));
                         }
                     }
                     if constexpr (kF32) {
@@ -514,10 +506,7 @@ __global__ void __launch_bounds__(StreamCfg<T, D, NB>::NT, StreamCfg<T, D, NB>::
                             uint32_t af[4];
                             ldsm4t(vb + r * Cfg::kRowB + (((i * 2 + cx) ^ (r & 7)) << 4), af);
 #pragma unroll
-                            for (int nb = 0; nb < NB; ++nb) {
-                                mma16816(o[nb][i], af, pf[nb][2], pf[nb][3]);
-                                mma16816(o[nb][i], af, pf[nb][0], pf[nb][1]);
-                            }
+                            for (int nb = 0; nb < NB; ++nb) mma16816(o[nb][i], af, pf[nb][0], pf[nb][1]);
                         }
                     }
                 }

@@ -611,8 +611,7 @@ int64_t cbq_paged_attn_workspace_bytes(const cbq_paged_cache *cache, const cbq_p
  * group's prefix is read once for all its sequences.  A sequence with nothing
  * to read gives zeros.  Rows outside the lengths are never used, whatever they
  * hold.  Scores, softmax and sums in fp32; bf16: products of bf16 on the
- * tensor cores, the softmax weights as two bf16 terms where up to 16 query rows
- * share a kv head's keys, rounded to one where more do; fp32: products of tf32
+ * tensor cores (the softmax weights rounded to bf16); fp32: products of tf32
  * pairs (2^-21 of a product is left out; infinities and values that tf32 cannot
  * hold by plain fp32 arithmetic).  The split of the keys depends on the
  * lengths and the SM count only: the same call gives the same bits.

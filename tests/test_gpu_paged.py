@@ -630,16 +630,3 @@ def test_prefixes_above_their_table_are_cut_and_reported(rows, op, dt):
     b.prefix_lens[1] = 1000
     check_attention(f(b, q), *ref)
     assert int(status[0]) == L.FLAG_CORRUPT and int(status[1]) == 1
-
-
-@pytest.mark.parametrize("d", [64, 128, 256])
-@pytest.mark.parametrize("heads,groups", [(2, []), (8, []), (4, [(2, 300), (4, 77)]), (32, [])], ids=str)
-def test_few_rows_in_bf16_are_rounded_once(heads, groups, d):
-    """bf16 holds 8 bits: the result's own rounding moves it by at most 2^-8 of
-    itself; weights as two bf16 terms leave out at most 2^-16 of each, in fp32 sums."""
-    dev = need_cuda()
-    s = Setup([1, 16, 17, 0, 33, 2000], groups=groups, heads=heads, kv_heads=2, d=d)
-    ref, spread, slack = s.attention(d ** -0.5, False)
-    got = run(s, "decode", dev).double().cpu()
-    tol = 2.0 ** -8 * ref.abs() + (2.0 ** -16 + slack) * spread * (1 + 2.0 ** -8) + 1e-30
-    assert bool(((got - ref).abs() <= tol).all())
