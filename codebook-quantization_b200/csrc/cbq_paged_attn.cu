@@ -262,7 +262,12 @@ __device__ __forceinline__ void join_unit(const LineArgs &a, const Cut &cut, int
 // instructions, keys (then dimensions of V) on the 16-row side and the query
 // rows on the 8-column side, so 1..8 query rows waste none of the long side.
 // bf16: m16n8k16; P^T turns into the second product's operand with two 8x8
-// register transposes.  fp32: m16n8k8 on tf32 pairs (see mma_f32), three
+// register transposes, rounded to bf16 like the values it multiplies, while l sums
+// it unrounded: against 64 bits the results are off by 2.1e-3 where the rounding of
+// an exact one takes 1.66e-3.  A second bf16 term brings that back to 1.66e-3, but
+// a value of inf then meets terms of both signs; with those pieces worked out again
+// (exact_piece) it costs 64 ragged sequences 169 -> 173 us, 16 of 4 new tokens 102
+// -> 108, head_dim 256 86 -> 91.  fp32: m16n8k8 on tf32 pairs (see mma_f32), three
 // products each: about 280 instructions for 16 keys and 8 rows where fp32 FMAs
 // fed from shared memory took 950.
 //
