@@ -9,7 +9,7 @@
 // the fp32 result rounded once whatever the activation type.
 #include <algorithm>
 
-#include "cbq_paged.cuh"
+#include "cbq_paged_line.cuh"
 
 namespace {
 
@@ -63,14 +63,17 @@ template <> struct Vec16<__nv_bfloat16> {
 // over LPH lanes.  A thread takes kHeads heads at a time: their loads go out
 // before the chain of small loads that finds the token's row and table entries,
 // and the cos / sin values serve all of them.  HBM bounds it: 16384 tokens of 48
-// heads of 128 (419 MB) take 82 us = 5.1 TB/s (147 us with one head a thread and
-// the table chain first); one token 3.3 us, a launch and five dependent loads.
+// heads of 128 (419 MB) take 84 us = 5.0 TB/s (147 us with one head a thread and
+// the table chain first); one token 3.5 us, a launch and five dependent loads.
 //
-// Two shapes: 128 threads with 3 heads at a time (one token 3.3 us, 16384 tokens
-// 89 us), and from kManyTokens on 64 threads with 6, whose tables serve twice the
-// heads (4.2 and 82 us).
-constexpr int kManyTokens = 2048;
-
+// Two shapes: 128 threads with 3 heads at a time, and 64 with 6, whose tables
+// serve twice the heads and of which more fit an SM (bf16: 8 to 5, fp32: 10 to 7),
+// but whose waves take longer.  The one whose waves add up to less is taken, a wave
+// of the second counted as 1.25 of the first.  Measured with 4 + 2 to 64 + 16 heads
+// of 64 to 256, in units of the first's time: one wave each 1.05 to 1.35; two waves to
+// one (bf16 780 to 1100 tokens, fp32 1100 to 1470) 0.75 to 0.9 (fp32 heads of 128 and
+// 256: 0.95 to 1.0); two each 1.0 to 1.27; 16384 tokens bf16 0.77 to 0.94, fp32 0.95 to
+// 1.02.
 template <typename T, int D, int kThreads, int kHeads>
 __global__ void __launch_bounds__(kThreads) k_paged_append(const PagedView pv, const AppendArgs a) {
     constexpr int N = Vec16<T>::N, LPH = D / (2 * N), H = D / 2, HPP = kThreads / LPH;   // heads per pass
@@ -177,7 +180,16 @@ __global__ void __launch_bounds__(kThreads) k_paged_append(const PagedView pv, c
 
 template <typename T, int D>
 int launch_append(const PagedView &pv, const AppendArgs &a, cudaStream_t s) {
-    if (pv.tokens < kManyTokens)
+    const int64_t sms = cbq_host::sm_count();
+    bool narrow = false;
+    if (pv.tokens > sms) {                             // else one CTA an SM, whatever the shape
+        int w = 0, n = 0, rc;
+        if ((rc = cbq_host::resident_ctas(reinterpret_cast<const void *>(k_paged_append<T, D, 128, 3>), 128, 0, &w)) != CBQ_OK ||
+            (rc = cbq_host::resident_ctas(reinterpret_cast<const void *>(k_paged_append<T, D, 64, 6>), 64, 0, &n)) != CBQ_OK)
+            return rc;
+        narrow = 5 * ((pv.tokens + n * sms - 1) / (n * sms)) < 4 * ((pv.tokens + w * sms - 1) / (w * sms));
+    }
+    if (!narrow)
         CBQ_CUDA_TRY(cbq_host::launch_pdl(k_paged_append<T, D, 128, 3>, dim3((unsigned)pv.tokens), dim3(128), 0, s, pv, a));
     else
         CBQ_CUDA_TRY(cbq_host::launch_pdl(k_paged_append<T, D, 64, 6>, dim3((unsigned)pv.tokens), dim3(64), 0, s, pv, a));

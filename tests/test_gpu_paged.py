@@ -630,3 +630,21 @@ def test_prefixes_above_their_table_are_cut_and_reported(rows, op, dt):
     b.prefix_lens[1] = 1000
     check_attention(f(b, q), *ref)
     assert int(status[0]) == L.FLAG_CORRUPT and int(status[1]) == 1
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f32"])
+@pytest.mark.parametrize("tokens", [148, 149, 741, 1037, 1185, 1481, 2221])
+def test_append_around_the_waves(dt, tokens):
+    """Both shapes of the kernel, on either side of what the GPU holds at once."""
+    dev = need_cuda()
+    s = Setup([tokens + 5, 3], new=[tokens - 2, 2], d=64, dtype=DT[dt], heads=3, kv_heads=1, page=64, stale=0.0)
+    qkv = torch.randn(tokens, 5, 64).to(DT[dt])
+    cos, sin = tables(64, tokens + 5)
+    kp, vp = s.pools(dev)
+    on = qkv.to(dev)
+    got = cbq.PagedKVCache(kp, vp).append_rope(s.batch(cbq, dev), on[:, :3], on[:, 3:4], on[:, 4:], cos.to(dev),
+                                               sin.to(dev))
+    ref, rk, rv = append_oracle(s, qkv[:, :3], qkv[:, 3:4], qkv[:, 4:], cos, sin, 1e-6, None, None)
+    same(got, ref)
+    same(kp, rk)
+    assert torch.equal(vp.cpu(), rv.to(DT[dt]))
