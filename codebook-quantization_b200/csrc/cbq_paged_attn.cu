@@ -814,7 +814,15 @@ int stream_plan(const PagedView &pv, int dtype, int d, int G, int64_t rows, int6
     return cbq_host::line_room(pv, d, off, p) ? CBQ_OK : CBQ_ERR_UNSUPPORTED;
 }
 
-constexpr int kStreamRows = 16;       // query rows per kv head up to which k_paged_stream is the faster kernel
+// Query rows per kv head up to which k_paged_stream is the faster kernel (row /
+// tile kernel, us, 1 to 8 heads a kv head, 2 to 8 kv heads).  Head_dim 128: 8 rows
+// of 16 sequences on 4000 keys 63 / 70, of 64 on 2000 127 / 117 (46 / 51 with 4 kv
+// heads); 12 rows 113 / 73 and 199 / 121.  Few units leave both kernels to cut the
+// keys, and the tile kernel's longer chain shows: 16 rows of one sequence on 2000
+// keys 13 / 21, on 20000 37 / 38, 24 rows 18 / 21 and 56 / 39; a prefix of 2000
+// rows 24 / 25, of 16000 43 / 37 and (2 kv heads) 35 / 43.  Head_dim 64: 16 rows of 16
+// sequences 53 / 53, of 64 103 / 103, 24 rows 73 / 60.
+int stream_rows(int d, int64_t units) { return d == 128 && units > 16 ? 8 : 16; }
 
 struct AttnPlan {
     PagedView pv;
@@ -862,12 +870,12 @@ int plan_attn(const cbq_paged_cache *c, const cbq_paged_batch *b, int64_t tokens
     // query rows that share a kv head's keys, on the mean of the owners
     const int64_t own_rows = extend ? (tokens * p->G + b->seqs - 1) / b->seqs : p->G;
     p->own.mode = extend ? kFull : kOwn;
-    p->own_tile = tile && extend && own_rows > kStreamRows;
+    p->own_tile = tile && extend && own_rows > stream_rows(p->d, b->seqs * c->kv_heads);
     const int sms = cbq_host::sm_count();
     int64_t group_rows = 0;
     if (p->prefix) {
         group_rows = ((int64_t)b->seqs + b->groups - 1) / b->groups * p->G;
-        p->pre_tile = tile && group_rows > kStreamRows;
+        p->pre_tile = tile && group_rows > stream_rows(p->d, b->groups * c->kv_heads);
     }
     p->own.direct = !p->prefix;
     if (p->own_tile) {

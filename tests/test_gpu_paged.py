@@ -648,3 +648,21 @@ def test_append_around_the_waves(dt, tokens):
     same(got, ref)
     same(kp, rk)
     assert torch.equal(vp.cpu(), rv.to(DT[dt]))
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("seqs", [1, 5, 20])
+@pytest.mark.parametrize("new", [2, 4, 6])
+def test_extend_a_few_tokens_of_each_sequence(d, seqs, new):
+    """8 to 24 query rows a kv head, few units and many: either kernel."""
+    dev = need_cuda()
+    verify(Setup([200 + 7 * i for i in range(seqs)], new=[new] * seqs, heads=16, kv_heads=4, d=d), "extend", dev)
+
+
+def test_a_prompt_chunk_among_single_tokens():
+    """Continuous batching: one kernel for the batch, by its mean."""
+    dev = need_cuda()
+    for chunk, singles in ((300, 40), (900, 20)):
+        kv = [chunk + 50] + [(37 * i) % 300 + 1 for i in range(singles)]
+        verify(Setup(kv, new=[chunk] + [1] * singles, groups=[(singles + 1, 40)], heads=8, kv_heads=2, d=128, page=32),
+               "extend", dev)
