@@ -834,11 +834,14 @@ struct AttnPlan {
 
 // The prefix's and the own rows' launches on SMs of their own, where both are
 // short: one after the other each pays its launch, plan and first loads (32
-// sequences on a prefix of 8192 rows: 45 us in turn, 38 side by side).  Long
-// ones gain nothing and would wait for the slower of two guesses (256 on 32768:
-// 264 and 285), so they run in turn; so does fp32, whose products and not the
-// bytes take the time.  The times are guessed from the lengths' bounds, own
-// rows at half of theirs, at the rates measured on long ones.
+// sequences on a prefix of 8192 rows: 50 us in turn, 39 side by side).  Long
+// ones gain nothing and would wait for the slower of two guesses (256 of 1024 own
+// rows on 32768: 260 in turn, 284 side by side), so they run in turn; so does fp32,
+// whose products and not the bytes take the time.  The times are guessed from the
+// lengths' bounds, own rows at half of theirs, at the rates measured on long ones.
+// Of 36 shapes (4 to 256 sequences, 2 or 8 kv heads, head_dim 64 or 128) the guess
+// takes the faster side for 30, loses 2 to 8 % on 5, and 27 % where 256 sequences
+// own next to nothing (256 of 100 rows on 32768, 2 kv heads: 75 in turn, 95).
 constexpr double kShareUs = 60.0;
 void share_sms(const cbq_paged_cache *c, const cbq_paged_batch *b, int64_t group_rows, int sms, AttnPlan *p) {
     const double row = (double)c->kv_heads * c->head_dim * 4;

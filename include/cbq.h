@@ -566,13 +566,13 @@ typedef struct cbq_paged_batch {
     const int32_t *kv_lens_dev;         /* [seqs] rows of each sequence, its new tokens included */
     const int32_t *page_table_dev;      /* [seqs][table_stride], table_width entries in use */
     int64_t table_width, table_stride;
-    int64_t max_kv_len;                 /* no kv_lens value is larger (table_width * page_size does) */
+    int64_t max_kv_len;                 /* bound of the kv_lens values; larger ones are cut (table_width * page_size does) */
     int64_t groups;                     /* 0: no shared prefixes; at most seqs */
     const int32_t *group_starts_dev;    /* [groups + 1], 0 .. seqs, never falling */
     const int32_t *prefix_lens_dev;     /* [groups] */
     const int32_t *prefix_table_dev;    /* [groups][prefix_stride], prefix_width entries in use */
     int64_t prefix_width, prefix_stride;
-    int64_t max_prefix_len;             /* no prefix_lens value is larger */
+    int64_t max_prefix_len;             /* bound of the prefix_lens values, likewise */
     uint32_t *status_dev;               /* uint32_t[4] as elsewhere, or NULL */
 } cbq_paged_batch;
 
@@ -614,7 +614,8 @@ int64_t cbq_paged_attn_workspace_bytes(const cbq_paged_cache *cache, const cbq_p
  * tensor cores (the softmax weights rounded to bf16); fp32: products of tf32
  * pairs (2^-21 of a product is left out; infinities and values that tf32 cannot
  * hold by plain fp32 arithmetic).  The split of the keys depends on the
- * lengths and the SM count only: the same call gives the same bits.
+ * lengths, on their bounds (max_kv_len, max_prefix_len, the tables' widths) and on
+ * the SM count only: the same call gives the same bits, a wider table may not.
  * Hq / Hkv <= 64. */
 int cbq_paged_attn_decode(const cbq_paged_cache *cache, const cbq_paged_batch *batch, int64_t tokens,
                           const void *q_dev, int64_t q_stride, int64_t q_heads, float scale, void *out_dev,

@@ -666,3 +666,32 @@ def test_a_prompt_chunk_among_single_tokens():
         kv = [chunk + 50] + [(37 * i) % 300 + 1 for i in range(singles)]
         verify(Setup(kv, new=[chunk] + [1] * singles, groups=[(singles + 1, 40)], heads=8, kv_heads=2, d=128, page=32),
                "extend", dev)
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f32"])
+def test_extend_and_append_past_32_bits(dt):
+    """Rows at the end of a pool of more than 2^31 elements, by both kernels."""
+    dev = need_cuda()
+    page, d, hkv = 256, 128, 8
+    pages = (1 << 31) // (page * d * hkv) + 40
+    k = torch.empty(pages, hkv, page, d, dtype=DT[dt], device=dev)
+    v = torch.empty_like(k)
+    for new in ([300, 213], [3, 1]):
+        s = Setup([700, 513], new=new, groups=[(2, 300)], heads=16, kv_heads=hkv, d=d, page=page, dtype=DT[dt], stale=0.0)
+        far = pages - s.pages
+        k[far:] = s.k.to(dev)
+        v[far:] = s.v.to(dev)
+        s.table = torch.where(s.table >= 0, s.table + far, s.table)
+        s.ptable = torch.where(s.ptable < 1 << 20, s.ptable + far, s.ptable)
+        b, c = s.batch(cbq, dev), cbq.PagedKVCache(k, v)
+        near = (s.table - far, s.ptable - far)
+        s.table, s.ptable = (torch.where(t < 0, -1, t) for t in near)
+        check_attention(c.attend_extend(b, s.q.to(dev)), *s.attention(d ** -0.5, True))
+        qkv = torch.randn(s.tokens, 32, d).to(DT[dt])
+        cos, sin = tables(d, 1100)
+        on = qkv.to(dev)
+        got = c.append_rope(b, on[:, :16], on[:, 16:24], on[:, 24:], cos.to(dev), sin.to(dev))
+        ref, rk, rv = append_oracle(s, qkv[:, :16], qkv[:, 16:24], qkv[:, 24:], cos, sin, 1e-6, None, None)
+        same(got, ref)
+        same(k[far:], rk)
+        assert torch.equal(v[far:].cpu(), rv.to(DT[dt]))

@@ -74,3 +74,25 @@ def test_an_error_that_a_kernel_reports_is_raised(graph):
     with pytest.raises(cbq._lib.CbqError) as e:
         m.generate(prompts, 4, graph=graph)
     assert e.value.status == cbq._lib.CBQ_ERR_CORRUPT and len(m.free) == 4
+
+
+def test_bf16_hidden_states_follow_fp32():
+    """The same prompts and one decode step in both types: about 20 roundings of
+    2^-9 a layer on the way, two layers, each of them random."""
+    dev = need_cuda()
+    W = q3.CompressedQwen3Weights(TINY, dev, seed=5)
+    g = torch.Generator().manual_seed(3)
+    lens, hidden = [40, 3, 100], {}
+    ids = torch.randint(0, TINY.vocab, (sum(lens),), generator=g).to(dev)
+    nxt = torch.randint(0, TINY.vocab, (3,), generator=g).to(dev)
+    for dt in (torch.float32, torch.bfloat16):
+        m = qp.PagedQwen3(W, pages=16, page_size=16, max_len=128, act_dtype=dt)
+        table, kv = m._table([m._take(n + 1) for n in lens]), m._ints(lens)
+        b = cbq.PagedBatch(table, kv, cu_tokens=m._ints([0, 40, 43, 143]))
+        first = m.forward(ids, b, decode=False).double()
+        kv.add_(1)
+        b = cbq.PagedBatch(table, kv)
+        hidden[dt] = first, m.forward(nxt, b, decode=True).double()
+        b.check()
+    for want, got in zip(*hidden.values()):
+        assert float((got - want).norm() / want.norm()) < (2 * 20) ** 0.5 * 2.0 ** -8
