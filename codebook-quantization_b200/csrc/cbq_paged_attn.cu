@@ -273,7 +273,7 @@ __device__ __forceinline__ void join_unit(const LineArgs &a, const Cut &cut, int
 //
 // Each warp copies its own 16 keys of a tile into its own ring (no barrier in the
 // loop).  HBM bounds long sequences: 64 ragged ones of up to 8192 keys, 8 kv heads
-// of 128 (960 MB), take 168 us = 5.7 TB/s, 0.88 of a copy's rate, with two CTAs an
+// of 128 (960 MB), take 170 us = 5.7 TB/s, 0.88 of a copy's rate, with two CTAs an
 // SM and 16 KB in flight per warp.  Short work is a chain of latencies: 1000 keys
 // of one sequence (4 MB) take 10 us, of which the plan 2, the first loads 3, the
 // tile 1, arrival and joining 3.

@@ -17,7 +17,7 @@
 // unrounded: against 64 bits the results are off by 2.3e-3 where the rounding of an
 // exact one takes 1.66e-3.  The rest as a second bf16 term brings that back to
 // 1.66e-3, but takes P's columns and product twice (64 keys a tile): 706 us instead
-// of 568 for a prompt of 8192 tokens, 292 instead of 268 for 256 sequences on a
+// of 566 for a prompt of 8192 tokens, 292 instead of 265 for 256 sequences on a
 // prefix of 32768 rows.  The usual choice, one term, is kept.
 //
 // A softmax reads S into registers at once, so the next tile's S can be computed
@@ -33,15 +33,16 @@
 // its pieces in shared memory and fetches Q by TMA.
 //
 // Measured (B200, bf16, head_dim 128): one prompt of 8192 tokens, 32 heads on 8:
-// 552 us = 995 TFLOP/s in a short burst, 0.59 of a plain matrix product; 630 us
-// repeated for seconds, where the power limit takes the clock down.  A tile of
-// 80 keys and 256 rows takes 2250 cycles: the products 1470 (S at 80 keys is bound
-// by shared memory, 52 cycles instead of 40), both softmaxes 1280 of the
-// special-function pipe, plus the latency of a softmax's other steps (900), of
-// which two warps a scheduler hide too little.  Tried and slower: P over S's
-// columns with 128 keys a tile (943 TFLOP/s); two threads a row (950); a part of
-// the exponentials by polynomial on the FMA pipe (950); the blocks taking turns
-// at their exponentials (952); tiles copied by 16-byte asynchronous copies (618).
+// 564 us = 975 TFLOP/s in a short burst (SM clock 1965 MHz), 0.58 of a plain matrix
+// product; 615 us = 894 TFLOP/s repeated for seconds, where the power limit takes the
+// clock to about 1815 MHz.  A tile of 80 keys and 256 rows takes 2250 cycles: the
+// products 1470 (S at 80 keys is bound by shared memory, 52 cycles instead of 40), both
+// softmaxes 1280 of the special-function pipe, plus the latency of a softmax's other
+// steps (900), of which two warps a scheduler hide too little.  Tried and slower (when
+// this form ran at 995 TFLOP/s): P over S's columns with 128 keys a tile (943); two
+// threads a row (950); a part of the exponentials by polynomial on the FMA pipe (950);
+// the blocks taking turns at their exponentials (952); tiles copied by 16-byte
+// asynchronous copies (618).
 // Work is the tile line of cbq_paged_line.cuh, one persistent CTA per part.
 // Every mbarrier wait is bounded; a wait that gives up sets CBQ_FLAG_TIMEOUT,
 // all roles stop at their next wait, and TMEM is released on the way out.
