@@ -111,7 +111,10 @@ __global__ void __launch_bounds__(kThreads) k_paged_append(const PagedView pv, c
     bool ok = row >= 0 && row < pv.cap;
     if (ok) page = pv.table[s * pv.table_stride + (row >> pv.ps_shift)];
     int64_t pos = row;
-    if (pv.groups) pos += pv.plens[warp_upper(pv.gs, pv.groups, s)];
+    if (pv.groups) {
+        const int g = warp_upper(pv.gs, pv.groups, s), plen = pv.plens[g];
+        if (s >= pv.gs[g] && s < pv.gs[g + 1]) pos += plen;            // else in no group
+    }
     ok = ok && pos >= 0 && pos < a.rope_len && page >= 0 && page < pv.pages;
     if (!ok && row >= 0 && threadIdx.x == 0) report(pv.status, CBQ_FLAG_CORRUPT, (uint32_t)t);
     const int line = row & ((1 << pv.ps_shift) - 1);

@@ -96,8 +96,11 @@ __device__ __forceinline__ Owner owner_of(const PagedView &pv, int mode, int o) 
     }
     w.olen = clampi(pv.lens[o], 0, pv.cap);
     if (mode == kFull && pv.groups) {
-        w.group = upper(pv.gs, pv.groups, o);
-        w.plen = clampi(pv.plens[w.group], 0, pv.pcap);
+        const int g = upper(pv.gs, pv.groups, o);
+        if (o >= pv.gs[g] && o < pv.gs[g + 1]) {       // else in no group
+            w.group = g;
+            w.plen = clampi(pv.plens[g], 0, pv.pcap);
+        }
     }
     return w;
 }

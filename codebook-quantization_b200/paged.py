@@ -99,7 +99,7 @@ class PagedBatch(_Held):
     step may hold fewer than it was captured for).  Shared prefixes:
     group g holds the sequences ``group_starts[g] .. group_starts[g+1] - 1``
     and its prefix the first ``prefix_lens[g]`` rows of the pages in
-    ``prefix_table[g]``.  ``max_kv_len`` / ``max_prefix_len`` bound the values
+    ``prefix_table[g]``; a sequence in no group has none.  ``max_kv_len`` / ``max_prefix_len`` bound the values
     the two length tensors will ever hold (default: what the tables can name).
     ``status`` int32 [4]: what calls record there, see :func:`check_status`
     (None: one of the batch's own; :meth:`check` reads it).

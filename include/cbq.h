@@ -568,7 +568,7 @@ typedef struct cbq_paged_batch {
     int64_t table_width, table_stride;
     int64_t max_kv_len;                 /* bound of the kv_lens values; larger ones are cut (table_width * page_size does) */
     int64_t groups;                     /* 0: no shared prefixes; at most seqs */
-    const int32_t *group_starts_dev;    /* [groups + 1], 0 .. seqs, never falling */
+    const int32_t *group_starts_dev;    /* [groups + 1], never falling; sequences outside them have no prefix */
     const int32_t *prefix_lens_dev;     /* [groups] */
     const int32_t *prefix_table_dev;    /* [groups][prefix_stride], prefix_width entries in use */
     int64_t prefix_width, prefix_stride;

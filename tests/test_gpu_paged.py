@@ -695,3 +695,30 @@ def test_extend_and_append_past_32_bits(dt):
         same(got, ref)
         same(k[far:], rk)
         assert torch.equal(v[far:].cpu(), rv.to(DT[dt]))
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f32"])
+@pytest.mark.parametrize("new", [1, 30])
+@pytest.mark.parametrize("inside", [(1, 2), (0, 2), (3, 2), (2, 0)], ids=str)
+def test_sequences_in_no_group_have_no_prefix(inside, new, dt):
+    """Groups that begin behind the first sequence or end before the last one."""
+    dev = need_cuda()
+    first, n = inside
+    s = Setup([40, 90, 31, 64, 300], new=[new] * 5, groups=[(first, 0), (n, 70), (5 - first - n, 0)], heads=4, kv_heads=2,
+              d=64, dtype=DT[dt], stale=0.0)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+    shared = dict(group_starts=i32([first, first + n]), prefix_lens=i32([70]), prefix_table=s.ptable[1:2].to(dev))
+    cu = i32([new * i for i in range(6)])
+    k, v = s.pools(dev)
+    c, b = cbq.PagedKVCache(k, v), cbq.PagedBatch(s.table.to(dev), i32(s.kv), cu_tokens=cu, **shared)
+    check_attention(c.attend_extend(b, s.q.to(dev)), *s.attention(64 ** -0.5, True))
+    if new == 1:
+        check_attention(c.attend_decode(b, s.q.to(dev)), *s.attention(64 ** -0.5, False))
+    qkv = torch.randn(s.tokens, 8, 64).to(DT[dt])
+    cos, sin = tables(64, 400)
+    on = qkv.to(dev)
+    got = c.append_rope(b, on[:, :4], on[:, 4:6], on[:, 6:], cos.to(dev), sin.to(dev))
+    ref, rk, rv = append_oracle(s, qkv[:, :4], qkv[:, 4:6], qkv[:, 6:], cos, sin, 1e-6, None, None)
+    same(got, ref)
+    same(k, rk)
+    b.check()
